@@ -53,6 +53,9 @@ enum vdb_bf_precision {
     VDB_BF_BF16_RERANK = 2 /* bf16 MFMA candidate pass (wider margin) + exact f32 re-rank */
 };
 
+/* Element type of device buffers that may hold other than f32 (rows4, kv_memory). */
+enum vdb_dtype { VDB_F32 = 0, VDB_F16 = 1, VDB_BF16 = 2 };
+
 const char* vdb_last_error(void);
 /* Number of visible HIP devices (0 when none; never fails). */
 int vdb_device_count(void);
@@ -254,6 +257,28 @@ int vdb_bf_search_batch_filtered(const vdb_bruteforce* bf, const float* queries,
                                  float* out_dist, uint64_t* out_label);
 /* The label of every stored row, in storage order (bruteforce.hpp:156-157); cap >= count. */
 int vdb_bf_labels(const vdb_bruteforce* bf, uint64_t* out, size_t cap);
+
+/* ---- base rows held in 4 bits (no reference counterpart) ----------------------------
+ *
+ * The exact scan's inner product over rows of 4.25 bits a value: a coarse score of every row, for one or a few queries.
+ * A row of `dim` values is ceil(dim / 32) groups of 32 columns.  A group is 16 bytes of e2m1 codes (the column of the
+ * lower index in the low nibble; sign, 2 exponent bits, 1 mantissa bit: 0, 0.5, 1, 1.5, 2, 3, 4, 6) and one scale byte e,
+ * and stands for code * 2^(e - 127); e = 255 makes the group NaN.  Columns past `dim` in the last group are never used.
+ *   d_codes  [n][ceil(dim / 32)][16]  16-byte aligned, DEVICE;   d_scales [n][ceil(dim / 32)], DEVICE
+ * All calls are asynchronous on `stream`, use the current device, allocate nothing and may be captured.
+ * n < 2^31, 1 <= dim <= 2^20, nq <= 65535; n = 0 or nq = 0 does nothing. */
+/* rows [n][dim] of `dtype`, row_stride elements apart -> codes and scales: the smallest power of two under which the
+ * group's largest magnitude is at most 6; codes rounded to nearest, ties to even.  A group with an infinity or a NaN is NaN;
+ * magnitudes above 6 * 2^125 (2.55e38) saturate to it, so that every value is finite in f32. */
+int vdb_rows4_pack_device(const void* d_rows, int dtype, size_t n, size_t dim, size_t row_stride, uint8_t* d_codes,
+                          uint8_t* d_scales, void* stream);
+/* The values that codes and scales stand for, [n][dim] f32. */
+int vdb_rows4_unpack_device(const uint8_t* d_codes, const uint8_t* d_scales, size_t n, size_t dim, float* d_out, void* stream);
+/* d_out[m][r] = sum over the columns of x[m] * value[r], [nq][n] f32 (so the framework's inner-product distance is
+ * 1 - d_out, space_ip.hpp:13-18).  x [nq][dim] of `dtype`, x_stride elements apart.  No bit of x is lost (f32 and f16
+ * values are split into bf16 parts); products are exact, sums are f32. */
+int vdb_rows4_products_device(const uint8_t* d_codes, const uint8_t* d_scales, size_t n, size_t dim, const void* d_x, int dtype,
+                              size_t nq, size_t x_stride, float* d_out, void* stream);
 
 /* ---- shard merge (no reference counterpart) --------------------------- */
 

@@ -16,6 +16,7 @@ VDB_OK, VDB_ERR_INVALID, VDB_ERR_RUNTIME, VDB_ERR_NO_DEVICE, VDB_ERR_UNSUPPORTED
 L2, IP = 0, 1
 SUM_SEQ, SUM_TREE64 = 0, 1
 BF_FP32, BF_BF16, BF_BF16_RERANK = 0, 1, 2
+F32, F16, BF16 = 0, 1, 2
 
 _f32p = C.POINTER(C.c_float)
 _u64p = C.POINTER(C.c_uint64)
@@ -84,6 +85,9 @@ SIGNATURES = {
     "vdb_comm_size": (C.c_int, [_vp]),
     "vdb_comm_rank": (C.c_int, [_vp]),
     "vdb_sharded_search_batch_device": (C.c_int, [_vp, _vp, _vp, C.c_size_t, C.c_size_t, _vp, _vp, _vp]),
+    "vdb_rows4_pack_device": (C.c_int, [_vp, C.c_int, C.c_size_t, C.c_size_t, C.c_size_t, _vp, _vp, _vp]),
+    "vdb_rows4_unpack_device": (C.c_int, [_vp, _vp, C.c_size_t, C.c_size_t, _vp, _vp]),
+    "vdb_rows4_products_device": (C.c_int, [_vp, _vp, C.c_size_t, C.c_size_t, _vp, C.c_int, C.c_size_t, C.c_size_t, _vp, _vp]),
     "vdb_merge_topk_device": (C.c_int, [_vp, _vp, C.c_size_t, C.c_size_t, C.c_size_t, _vp, _vp, _vp]),
 }
 

@@ -1745,6 +1745,73 @@ int vdb_sharded_search_batch_device(const vdb_index* shard, vdb_comm* comm, cons
     });
 }
 
+// ---- rows held in 4 bits ------------------------------------------------------------------
+
+}  // extern "C"
+
+namespace {
+
+void check_rows4(size_t n, size_t dim, int dtype) {
+    if (dtype != VDB_F32 && dtype != VDB_F16 && dtype != VDB_BF16) throw std::invalid_argument("unknown element type");
+    if (dim == 0 || dim > (1u << 20)) throw std::invalid_argument("rows4: dim must be in 1..2^20");
+    if (n >= (1ull << 31)) throw std::invalid_argument("rows4: n must be below 2^31");
+}
+
+void check_aligned(const void* p, size_t to, const char* what) {
+    if (!p) throw std::invalid_argument(std::string("null buffer: ") + what);
+    if ((uintptr_t)p % to) throw std::invalid_argument(std::string(what) + " must be aligned to " + std::to_string(to) + " bytes");
+}
+
+size_t dtype_size(int dtype) { return dtype == VDB_F32 ? 4 : 2; }
+
+}  // namespace
+
+extern "C" {
+
+int vdb_rows4_pack_device(const void* d_rows, int dtype, size_t n, size_t dim, size_t row_stride, uint8_t* d_codes, uint8_t* d_scales,
+                          void* stream) {
+    return guarded([&] {
+        check_rows4(n, dim, dtype);
+        if (n == 0) return (int)VDB_OK;
+        check_aligned(d_rows, dtype_size(dtype), "rows");
+        check_aligned(d_codes, 16, "codes");
+        check_aligned(d_scales, 1, "scales");
+        std::string err;
+        const int rc = launch_rows4_pack(d_rows, dtype, n, (uint32_t)dim, row_stride, d_codes, d_scales, (hipStream_t)stream, &err);
+        return rc ? set_error(rc, err) : (int)VDB_OK;
+    });
+}
+
+int vdb_rows4_unpack_device(const uint8_t* d_codes, const uint8_t* d_scales, size_t n, size_t dim, float* d_out, void* stream) {
+    return guarded([&] {
+        check_rows4(n, dim, VDB_F32);
+        if (n == 0) return (int)VDB_OK;
+        check_aligned(d_codes, 16, "codes");
+        check_aligned(d_scales, 1, "scales");
+        check_aligned(d_out, 4, "out");
+        std::string err;
+        const int rc = launch_rows4_unpack(d_codes, d_scales, n, (uint32_t)dim, d_out, (hipStream_t)stream, &err);
+        return rc ? set_error(rc, err) : (int)VDB_OK;
+    });
+}
+
+int vdb_rows4_products_device(const uint8_t* d_codes, const uint8_t* d_scales, size_t n, size_t dim, const void* d_x, int dtype, size_t nq,
+                              size_t x_stride, float* d_out, void* stream) {
+    return guarded([&] {
+        check_rows4(n, dim, dtype);
+        if (nq > 65535) throw std::invalid_argument("rows4: at most 65535 queries per call");
+        if (n == 0 || nq == 0) return (int)VDB_OK;
+        check_aligned(d_codes, 16, "codes");
+        check_aligned(d_scales, 1, "scales");
+        check_aligned(d_x, dtype_size(dtype), "queries");
+        check_aligned(d_out, 4, "out");
+        std::string err;
+        const int rc = launch_rows4_products(d_codes, d_scales, (uint32_t)n, (uint32_t)dim, d_x, dtype, (uint32_t)nq, x_stride, d_out,
+                                             (hipStream_t)stream, &err);
+        return rc ? set_error(rc, err) : (int)VDB_OK;
+    });
+}
+
 // ---- shard merge ------------------------------------------------------------------------
 
 int vdb_merge_topk_device(const float* d_dist, const uint64_t* d_label, size_t n_lists, size_t nq, size_t k,

@@ -161,4 +161,12 @@ int launch_bf_mfma(const BfDeviceData& d, int precision, const float* d_queries,
 int launch_merge_topk(const float* d_dist, const uint64_t* d_label, uint32_t n_lists, uint32_t nq, uint32_t k,
                       float* d_out_dist, uint64_t* d_out_label, hipStream_t stream, std::string* err);
 
+// ---- rows held in 4 bits (rows4.hip) --------------------------------------------------------
+// codes [n][groups][16], scales [n][groups], groups = ceil(dim / 32); dtype: vdb_dtype; strides in elements.
+int launch_rows4_products(const uint8_t* d_codes, const uint8_t* d_scales, uint32_t n, uint32_t dim, const void* d_x, int dtype, uint32_t nq,
+                          uint64_t x_stride, float* d_out, hipStream_t stream, std::string* err);
+int launch_rows4_pack(const void* d_rows, int dtype, uint64_t n, uint32_t dim, uint64_t row_stride, uint8_t* d_codes, uint8_t* d_scales,
+                      hipStream_t stream, std::string* err);
+int launch_rows4_unpack(const uint8_t* d_codes, const uint8_t* d_scales, uint64_t n, uint32_t dim, float* d_out, hipStream_t stream, std::string* err);
+
 }  // namespace vdb

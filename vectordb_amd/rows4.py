@@ -1,0 +1,111 @@
+"""Base rows held in 4 bits on the GPU, and the products of a few queries with all of them.
+
+Beside ``BruteforceSearch``: the same scan over every row, in 4.25 bits a value instead of 32 - a coarse score to pick
+candidates by, or the scores themselves where that precision will do.  Everything runs on CUDA tensors and on torch's
+current stream of their device (include/vdb_index.h, vdb_rows4_*)."""
+from __future__ import annotations
+
+from . import _lib
+from ._lib import BF16, F16, F32, check
+
+
+def dtype_code(t, what: str) -> int:
+    import torch
+
+    code = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}.get(t.dtype)
+    if code is None:
+        raise ValueError(f"{what}: float32, float16 or bfloat16, got {t.dtype}")
+    return code
+
+
+class on_device:
+    """Makes a tensor's device current for the call, and gives its current stream."""
+
+    __slots__ = ("index", "prev")
+
+    def __init__(self, device):
+        self.index = device.index
+
+    def __enter__(self):
+        import torch
+
+        self.prev = torch.cuda.current_device()
+        if self.prev != self.index:
+            torch.cuda.set_device(self.index)
+        return torch.cuda.current_stream().cuda_stream
+
+    def __exit__(self, *exc):
+        if self.prev != self.index:
+            import torch
+
+            torch.cuda.set_device(self.prev)
+
+
+class Rows4:
+    """``codes`` [n, ceil(dim / 32) * 16] uint8 and ``scales`` [n, ceil(dim / 32)] uint8, contiguous CUDA tensors in the
+    layout that include/vdb_index.h describes: e2m1 codes, a power-of-two scale for every 32 columns of a row."""
+
+    def __init__(self, codes, scales, dim: int):
+        import torch
+
+        groups = (int(dim) + 31) // 32
+        if dim < 1:
+            raise ValueError("dim must be positive")
+        if codes.dtype != torch.uint8 or scales.dtype != torch.uint8 or not codes.is_cuda or codes.device != scales.device:
+            raise ValueError("codes and scales: uint8 CUDA tensors on one device")
+        if codes.dim() != 2 or tuple(codes.shape) != (scales.shape[0], groups * 16) or tuple(scales.shape[1:]) != (groups,):
+            raise ValueError(f"expected codes [n, {groups * 16}] and scales [n, {groups}], got {tuple(codes.shape)} and {tuple(scales.shape)}")
+        if not (codes.is_contiguous() and scales.is_contiguous()):
+            raise ValueError("codes and scales must be contiguous")
+        self._l = _lib.lib()
+        self.codes, self.scales, self.dim = codes, scales, int(dim)
+
+    @classmethod
+    def pack(cls, rows) -> "Rows4":
+        """Rounds rows [n, dim] (float32, float16 or bfloat16) to 4 bits."""
+        import torch
+
+        if not rows.is_cuda or rows.dim() != 2:
+            raise ValueError("rows: a CUDA tensor [n, dim]")
+        t = dtype_code(rows, "rows")
+        if rows.stride(1) != 1 or rows.stride(0) < 0:
+            rows = rows.contiguous()
+        n, dim = rows.shape
+        groups = (dim + 31) // 32
+        out = cls(torch.empty((n, groups * 16), dtype=torch.uint8, device=rows.device),
+                  torch.empty((n, groups), dtype=torch.uint8, device=rows.device), dim)
+        with on_device(rows.device) as stream:
+            check(out._l.vdb_rows4_pack_device(rows.data_ptr(), t, n, dim, rows.stride(0), out.codes.data_ptr(), out.scales.data_ptr(), stream))
+        return out
+
+    def __len__(self) -> int:
+        return self.codes.shape[0]
+
+    def unpack(self):
+        """The values that the codes stand for, [n, dim] float32."""
+        import torch
+
+        out = torch.empty((len(self), self.dim), dtype=torch.float32, device=self.codes.device)
+        with on_device(out.device) as stream:
+            check(self._l.vdb_rows4_unpack_device(self.codes.data_ptr(), self.scales.data_ptr(), len(self), self.dim, out.data_ptr(), stream))
+        return out
+
+    def products(self, queries, out=None):
+        """Inner products of queries [nq, dim] (or [dim]) with every row: [nq, n] (or [n]) float32, into ``out`` if given."""
+        import torch
+
+        x = queries if queries.dim() == 2 else queries.unsqueeze(0)
+        if queries.dim() not in (1, 2) or x.shape[1] != self.dim or x.device != self.codes.device:
+            raise ValueError(f"expected queries [nq, {self.dim}] on {self.codes.device}, got {tuple(queries.shape)} on {queries.device}")
+        t = dtype_code(x, "queries")
+        if x.stride(1) != 1 or x.stride(0) < 0:
+            x = x.contiguous()
+        nq, n = x.shape[0], len(self)
+        if out is None:
+            out = torch.empty((nq, n) if queries.dim() == 2 else (n,), dtype=torch.float32, device=x.device)
+        elif out.dtype != torch.float32 or out.device != x.device or out.numel() != nq * n or not out.is_contiguous():
+            raise ValueError(f"out: a contiguous float32 tensor of {nq} x {n} on {x.device}")
+        with on_device(x.device) as stream:
+            check(self._l.vdb_rows4_products_device(self.codes.data_ptr(), self.scales.data_ptr(), n, self.dim, x.data_ptr(), t, nq, x.stride(0),
+                                                    out.data_ptr(), stream))
+        return out

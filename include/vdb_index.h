@@ -280,6 +280,65 @@ int vdb_rows4_unpack_device(const uint8_t* d_codes, const uint8_t* d_scales, siz
 int vdb_rows4_products_device(const uint8_t* d_codes, const uint8_t* d_scales, size_t n, size_t dim, const void* d_x, int dtype,
                               size_t nq, size_t x_stride, float* d_out, void* stream);
 
+/* ---- keys and values of language-model contexts, held in 8 bits (no reference counterpart) -------------
+ *
+ * Rows that an index finds, in the form in which a model reads them: for every token and head a key and a value of `dim`
+ * numbers.  The memory is cut into pages of page_tokens tokens; a sequence's token t lies in page table[t / page_tokens],
+ * row t % page_tokens.  Codes are e4m3 (no infinities; 0x7F and 0xFF are NaN) and stand for code * scale, one f32 scale
+ * per page, head and side (keys, values).
+ * All calls are asynchronous on `stream`, use the current device, allocate nothing and may be captured.  Two appends that
+ * touch one page must not overlap, nor an append and a read of the same page. */
+typedef struct vdb_kv_memory {
+    void* k;         /* [pages][heads][page_tokens][dim] e4m3, 16-byte aligned, DEVICE */
+    void* v;         /* likewise */
+    float* k_scale;  /* [pages][heads], positive and finite where a page holds tokens */
+    float* v_scale;
+    size_t pages;        /* < 2^31 */
+    size_t heads;        /* key / value heads, 1..32767 */
+    size_t page_tokens;  /* a power of two, 16..1024 */
+    size_t dim;          /* a multiple of 32, 32..256 */
+} vdb_kv_memory;
+typedef struct vdb_kv_batch {
+    const int32_t* table;    /* [count][table_width] page numbers; tokens of a page outside 0..pages-1 are absent */
+    const int32_t* lengths;  /* [count] tokens of each sequence, the new ones INCLUDED */
+    const int32_t* offsets;  /* [count + 1], ascending: rows offsets[b] .. offsets[b + 1] - 1 of the new tokens' arrays are the
+                              * last tokens of sequence b (rows of no sequence are left alone; a sequence whose rows do not lie
+                              * in 0..tokens-1 has none).  NULL: row b is sequence b's last token, and tokens = count */
+    size_t count;            /* sequences, at most 65535 */
+    size_t table_width;      /* pages a row of the table has room for, >= 1 */
+    size_t tokens;           /* rows of the new tokens' arrays, < 2^31 */
+    size_t max_new;          /* most new tokens of any sequence (a size for launches: a wrong one costs time, not correctness) */
+} vdb_kv_batch;
+/* Stores the new tokens' keys and values k, v [tokens][heads][dim] of `dtype` (strides in elements, multiples of 8;
+ * 16-byte aligned; a head's numbers contiguous).  Tokens at negative positions, beyond the table or in absent pages are not
+ * stored.  A page's scale becomes the smallest power of two under which the new rows' largest finite magnitude is at most
+ * 448 (and at least 2^-100), or stays if the page held tokens before and its scale is larger already; where it grows, the
+ * older rows are rounded to it again.  Rounding is to nearest, ties to even; an infinity or a NaN is stored as NaN.
+ * With rot_dims != 0 (a multiple of 16, at most dim) the first rot_dims numbers of every key, and of every query, are turned
+ * by the angles of the token's position: cos, sin [positions][rot_dims / 2] f32, 16-byte aligned; the pair is (d, d + rot_dims / 2),
+ * or (2 i, 2 i + 1) with interleaved != 0; (x, y) becomes (x cos - y sin, y cos + x sin) in f32.  A position beyond the
+ * tables: its key and value are not stored and its query is NaN.
+ * q nullable [tokens][q_heads][dim] of `dtype` (strides as above) -> q_out [tokens][q_heads][dim], turned, rounded once; rows
+ * of no sequence are copied.  q_out must not overlap q.  Needs rot_dims != 0. */
+int vdb_kv_append_device(const vdb_kv_memory* memory, const vdb_kv_batch* batch, int dtype, const void* d_k, size_t k_token_stride,
+                         size_t k_head_stride, const void* d_v, size_t v_token_stride, size_t v_head_stride, const float* d_cos,
+                         const float* d_sin, size_t positions, size_t rot_dims, int interleaved, const void* d_q, size_t q_token_stride,
+                         size_t q_head_stride, size_t q_heads, void* d_q_out, void* stream);
+/* Attention of the new tokens' queries q [tokens][q_heads][dim] of `dtype` (strides as above) over the memory:
+ *   out = softmax(scale * q . k) v   over the tokens the query sees, [tokens][q_heads][dim] of `dtype`, 16-byte aligned
+ *   lse nullable [tokens][q_heads] f32: the natural logarithm of the softmax's sum
+ * Query head h reads key head h / (q_heads / heads).  The query at position t sees the present tokens 0..t, with window != 0
+ * only the last `window` of them.  With select [count][heads][n_select] (needs offsets = NULL and window = 0) it sees those
+ * token numbers instead, in any order, each as often as it is listed; numbers outside 0..lengths[b]-1 are skipped, so a
+ * search's padding needs no care.  A query that sees nothing gives zeros and -infinity.
+ * A token that a query does not see has no effect on its result, whatever it holds.
+ * workspace: vdb_kv_attend_workspace() bytes of DEVICE memory, 16-byte aligned, free again once the stream has passed the
+ * call; any contents.  Calls that may overlap need workspaces of their own. */
+size_t vdb_kv_attend_workspace(const vdb_kv_memory* memory, const vdb_kv_batch* batch, size_t q_heads, size_t n_select);
+int vdb_kv_attend_device(const vdb_kv_memory* memory, const vdb_kv_batch* batch, int dtype, const void* d_q, size_t q_token_stride,
+                         size_t q_head_stride, size_t q_heads, float scale, size_t window, const int64_t* d_select, size_t n_select,
+                         void* d_out, float* d_lse, void* d_workspace, size_t workspace_bytes, void* stream);
+
 /* ---- shard merge (no reference counterpart) --------------------------- */
 
 /* Merge G per-shard result lists into one: inputs [G][nq][k] (each row ascending, padded

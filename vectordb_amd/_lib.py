@@ -23,6 +23,19 @@ _u64p = C.POINTER(C.c_uint64)
 _u32p = C.POINTER(C.c_uint32)
 _vp = C.c_void_p
 
+class KvMemoryStruct(C.Structure):  # vdb_kv_memory
+    _fields_ = [("k", _vp), ("v", _vp), ("k_scale", _vp), ("v_scale", _vp), ("pages", C.c_size_t), ("heads", C.c_size_t),
+                ("page_tokens", C.c_size_t), ("dim", C.c_size_t)]
+
+
+class KvBatchStruct(C.Structure):  # vdb_kv_batch
+    _fields_ = [("table", _vp), ("lengths", _vp), ("offsets", _vp), ("count", C.c_size_t), ("table_width", C.c_size_t),
+                ("tokens", C.c_size_t), ("max_new", C.c_size_t)]
+
+
+_kvp = [C.POINTER(KvMemoryStruct), C.POINTER(KvBatchStruct)]
+_sz = C.c_size_t
+
 # name -> (restype, argtypes); one entry per declaration of include/vdb_index.h
 SIGNATURES = {
     "vdb_last_error": (C.c_char_p, []),
@@ -88,6 +101,9 @@ SIGNATURES = {
     "vdb_rows4_pack_device": (C.c_int, [_vp, C.c_int, C.c_size_t, C.c_size_t, C.c_size_t, _vp, _vp, _vp]),
     "vdb_rows4_unpack_device": (C.c_int, [_vp, _vp, C.c_size_t, C.c_size_t, _vp, _vp]),
     "vdb_rows4_products_device": (C.c_int, [_vp, _vp, C.c_size_t, C.c_size_t, _vp, C.c_int, C.c_size_t, C.c_size_t, _vp, _vp]),
+    "vdb_kv_append_device": (C.c_int, _kvp + [C.c_int, _vp, _sz, _sz, _vp, _sz, _sz, _vp, _vp, _sz, _sz, C.c_int, _vp, _sz, _sz, _sz, _vp, _vp]),
+    "vdb_kv_attend_workspace": (C.c_size_t, _kvp + [_sz, _sz]),
+    "vdb_kv_attend_device": (C.c_int, _kvp + [C.c_int, _vp, _sz, _sz, _sz, C.c_float, _sz, _vp, _sz, _vp, _vp, _vp, _sz, _vp]),
     "vdb_merge_topk_device": (C.c_int, [_vp, _vp, C.c_size_t, C.c_size_t, C.c_size_t, _vp, _vp, _vp]),
 }
 

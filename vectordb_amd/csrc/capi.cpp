@@ -1812,6 +1812,157 @@ int vdb_rows4_products_device(const uint8_t* d_codes, const uint8_t* d_scales, s
     });
 }
 
+// ---- keys and values in 8 bits -------------------------------------------------------------
+
+}  // extern "C"
+
+namespace {
+
+KvMemory kv_memory(const vdb_kv_memory* m) {
+    if (!m) throw std::invalid_argument("null memory");
+    if (m->page_tokens < 16 || m->page_tokens > 1024 || (m->page_tokens & (m->page_tokens - 1)))
+        throw std::invalid_argument("kv memory: page_tokens must be a power of two in 16..1024");
+    if (m->dim < 32 || m->dim > 256 || m->dim % 32) throw std::invalid_argument("kv memory: dim must be a multiple of 32 in 32..256");
+    if (m->heads < 1 || m->heads > 32767) throw std::invalid_argument("kv memory: heads must be in 1..32767");
+    if (m->pages >= (1ull << 31)) throw std::invalid_argument("kv memory: pages must be below 2^31");
+    uint32_t shift = 4;
+    while ((1u << shift) < m->page_tokens) ++shift;
+    return KvMemory{m->k, m->v, m->k_scale, m->v_scale, m->pages, (uint32_t)m->heads, (uint32_t)m->page_tokens, shift, (uint32_t)m->dim};
+}
+
+KvBatch kv_batch(const vdb_kv_batch* b) {
+    if (!b) throw std::invalid_argument("null batch");
+    if (b->count > 65535) throw std::invalid_argument("kv batch: at most 65535 sequences per call");
+    if (b->table_width < 1 || b->table_width >= (1ull << 31)) throw std::invalid_argument("kv batch: table_width must be in 1..2^31-1");
+    if (b->tokens >= (1ull << 31)) throw std::invalid_argument("kv batch: tokens must be below 2^31");
+    if (!b->offsets && b->tokens != b->count) throw std::invalid_argument("kv batch: without offsets every sequence has one new token");
+    return KvBatch{b->table, b->lengths, b->offsets, b->tokens, (uint32_t)b->count, (uint32_t)b->table_width};
+}
+
+uint32_t kv_max_new(const vdb_kv_batch* b) { return b->offsets ? (uint32_t)std::min(std::max<size_t>(b->max_new, 1), b->tokens) : 1; }
+
+void check_kv_pointers(const KvMemory& m, const KvBatch& b) {
+    check_aligned(m.k, 16, "k");
+    check_aligned(m.v, 16, "v");
+    check_aligned(m.k_scale, 4, "k_scale");
+    check_aligned(m.v_scale, 4, "v_scale");
+    check_aligned(b.table, 4, "table");
+    check_aligned(b.lengths, 4, "lengths");
+    if (b.offsets) check_aligned(b.offsets, 4, "offsets");
+}
+
+void check_kv_rows(const void* p, size_t token_stride, size_t head_stride, const char* what) {
+    check_aligned(p, 16, what);
+    if (token_stride % 8 || head_stride % 8) throw std::invalid_argument(std::string(what) + ": strides must be multiples of 8 elements");
+}
+
+void check_kv_dtype(int dtype) {
+    if (dtype != VDB_F32 && dtype != VDB_F16 && dtype != VDB_BF16) throw std::invalid_argument("unknown element type");
+}
+
+KvAttendArgs kv_attend_args(const vdb_kv_memory* memory, const vdb_kv_batch* batch, size_t q_heads, size_t n_select) {
+    KvAttendArgs a{};
+    a.mem = kv_memory(memory);
+    a.batch = kv_batch(batch);
+    if (q_heads < 1 || q_heads % a.mem.heads || q_heads / a.mem.heads > 65535)
+        throw std::invalid_argument("kv attend: q_heads must be a multiple of the memory's heads");
+    if (n_select >= (1ull << 31)) throw std::invalid_argument("kv attend: n_select must be below 2^31");
+    a.q_heads = (uint32_t)q_heads;
+    a.n_select = (uint32_t)n_select;
+    return a;
+}
+
+}  // namespace
+
+extern "C" {
+
+int vdb_kv_append_device(const vdb_kv_memory* memory, const vdb_kv_batch* batch, int dtype, const void* d_k, size_t k_token_stride,
+                         size_t k_head_stride, const void* d_v, size_t v_token_stride, size_t v_head_stride, const float* d_cos,
+                         const float* d_sin, size_t positions, size_t rot_dims, int interleaved, const void* d_q, size_t q_token_stride,
+                         size_t q_head_stride, size_t q_heads, void* d_q_out, void* stream) {
+    return guarded([&] {
+        KvAppendArgs a{};
+        a.mem = kv_memory(memory);
+        a.batch = kv_batch(batch);
+        check_kv_dtype(dtype);
+        if (rot_dims % 16 || rot_dims > a.mem.dim) throw std::invalid_argument("kv append: rot_dims must be a multiple of 16, at most dim");
+        if (d_q && !rot_dims) throw std::invalid_argument("kv append: queries are taken to be turned, and rot_dims is 0");
+        if (d_q && (q_heads < 1 || q_heads > (1u << 20))) throw std::invalid_argument("kv append: q_heads must be in 1..2^20");
+        if (a.batch.count == 0 || a.batch.tokens == 0) return (int)VDB_OK;
+        check_kv_pointers(a.mem, a.batch);
+        check_kv_rows(d_k, k_token_stride, k_head_stride, "keys");
+        check_kv_rows(d_v, v_token_stride, v_head_stride, "values");
+        if (rot_dims) {
+            check_aligned(d_cos, 16, "cos");
+            check_aligned(d_sin, 16, "sin");
+        }
+        if (d_q) {
+            check_kv_rows(d_q, q_token_stride, q_head_stride, "queries");
+            check_aligned(d_q_out, 16, "q_out");
+        }
+        a.k = d_k;
+        a.v = d_v;
+        a.k_token = k_token_stride;
+        a.k_head = k_head_stride;
+        a.v_token = v_token_stride;
+        a.v_head = v_head_stride;
+        a.cos = d_cos;
+        a.sin = d_sin;
+        a.positions = positions;
+        a.rot = (uint32_t)rot_dims;
+        a.interleaved = interleaved != 0;
+        a.q = d_q;
+        a.q_token = q_token_stride;
+        a.q_head = q_head_stride;
+        a.q_heads = (uint32_t)q_heads;
+        a.q_out = d_q_out;
+        std::string err;
+        const int rc = launch_kv_append(a, dtype, kv_max_new(batch), (hipStream_t)stream, &err);
+        return rc ? set_error(rc, err) : (int)VDB_OK;
+    });
+}
+
+size_t vdb_kv_attend_workspace(const vdb_kv_memory* memory, const vdb_kv_batch* batch, size_t q_heads, size_t n_select) {
+    size_t bytes = 0;
+    (void)guarded([&] {
+        const KvAttendArgs a = kv_attend_args(memory, batch, q_heads, n_select);
+        bytes = kv_attend_workspace_bytes(a, kv_max_new(batch));
+        return (int)VDB_OK;
+    });
+    return bytes;
+}
+
+int vdb_kv_attend_device(const vdb_kv_memory* memory, const vdb_kv_batch* batch, int dtype, const void* d_q, size_t q_token_stride,
+                         size_t q_head_stride, size_t q_heads, float scale, size_t window, const int64_t* d_select, size_t n_select,
+                         void* d_out, float* d_lse, void* d_workspace, size_t workspace_bytes, void* stream) {
+    return guarded([&] {
+        KvAttendArgs a = kv_attend_args(memory, batch, q_heads, d_select ? n_select : 0);
+        check_kv_dtype(dtype);
+        if (window >= (1ull << 31)) throw std::invalid_argument("kv attend: window must be below 2^31");
+        if (d_select && (a.batch.offsets || window)) throw std::invalid_argument("kv attend: selected tokens go with one new token per sequence and no window");
+        if (a.batch.count == 0 || a.batch.tokens == 0) return (int)VDB_OK;
+        check_kv_pointers(a.mem, a.batch);
+        check_kv_rows(d_q, q_token_stride, q_head_stride, "queries");
+        check_aligned(d_out, 16, "out");
+        if (d_select) check_aligned(d_select, 8, "select");
+        if (d_lse) check_aligned(d_lse, 4, "lse");
+        const size_t need = kv_attend_workspace_bytes(a, kv_max_new(batch));
+        if (need) check_aligned(d_workspace, 16, "workspace");
+        if (workspace_bytes < need) throw std::invalid_argument("kv attend: the workspace is smaller than vdb_kv_attend_workspace()");
+        a.q = d_q;
+        a.q_token = q_token_stride;
+        a.q_head = q_head_stride;
+        a.scale = scale;
+        a.window = (int64_t)window;
+        a.select = d_select;
+        a.out = d_out;
+        a.lse = d_lse;
+        std::string err;
+        const int rc = launch_kv_attend(a, dtype, kv_max_new(batch), d_workspace, (hipStream_t)stream, &err);
+        return rc ? set_error(rc, err) : (int)VDB_OK;
+    });
+}
+
 // ---- shard merge ------------------------------------------------------------------------
 
 int vdb_merge_topk_device(const float* d_dist, const uint64_t* d_label, size_t n_lists, size_t nq, size_t k,

@@ -169,4 +169,50 @@ int launch_rows4_pack(const void* d_rows, int dtype, uint64_t n, uint32_t dim, u
                       hipStream_t stream, std::string* err);
 int launch_rows4_unpack(const uint8_t* d_codes, const uint8_t* d_scales, uint64_t n, uint32_t dim, float* d_out, hipStream_t stream, std::string* err);
 
+// ---- key / value memory in 8 bits (kv_append.hip, kv_attend.hip) -------------------------------
+struct KvMemory {  // vdb_kv_memory
+    void *k, *v;               // [pages][heads][page_tokens][dim] e4m3
+    float *k_scale, *v_scale;  // [pages][heads]
+    uint64_t pages;
+    uint32_t heads, page_tokens, page_shift, dim;  // page_tokens = 1 << page_shift >= 16; dim a multiple of 32, at most 256
+};
+struct KvBatch {  // vdb_kv_batch
+    const int32_t* table;    // [count][table_width] page numbers
+    const int32_t* lengths;  // [count] tokens held, the new ones included
+    const int32_t* offsets;  // [count + 1], or nullptr: one new token per sequence
+    uint64_t tokens;         // rows of the new tokens' arrays
+    uint32_t count, table_width;
+};
+struct KvAppendArgs {
+    KvMemory mem;
+    KvBatch batch;
+    const void *k, *v;
+    uint64_t k_token, k_head, v_token, v_head;  // strides in elements
+    const float *cos, *sin;                     // [positions][rot / 2]
+    uint64_t positions;
+    uint32_t rot;  // rotated dimensions (0: none), a multiple of 16
+    bool interleaved;
+    const void* q;  // nullptr: no queries
+    uint64_t q_token, q_head;
+    uint32_t q_heads;
+    void* q_out;  // [tokens][q_heads][dim]
+};
+int launch_kv_append(const KvAppendArgs& a, int dtype, uint32_t max_new, hipStream_t stream, std::string* err);
+
+struct KvAttendArgs {
+    KvMemory mem;
+    KvBatch batch;
+    const void* q;
+    uint64_t q_token, q_head;
+    uint32_t q_heads;
+    float scale;
+    int64_t window;         // 0: all
+    const int64_t* select;  // [count][heads][n_select] token numbers, nullptr: every token
+    uint32_t n_select;
+    void* out;   // [tokens][q_heads][dim]
+    float* lse;  // [tokens][q_heads], or nullptr
+};
+size_t kv_attend_workspace_bytes(const KvAttendArgs& a, uint32_t max_new);
+int launch_kv_attend(const KvAttendArgs& a, int dtype, uint32_t max_new, void* workspace, hipStream_t stream, std::string* err);
+
 }  // namespace vdb

@@ -1,0 +1,173 @@
+"""Keys and values of language-model contexts in 8 bits, in pages: the store that attention reads, over everything or over
+the tokens that an index found.
+
+An index over a context's keys (``HierarchicalNSW`` or ``BruteforceSearch`` with the inner-product space, labels = token
+numbers) answers which tokens matter for a query; ``KeyValueMemory.attend(select=labels)`` reads those, without ``select``
+it reads all of them.  Everything runs on CUDA tensors and on torch's current stream of their device
+(include/vdb_index.h, vdb_kv_*)."""
+from __future__ import annotations
+
+import ctypes as C
+
+from . import _lib
+from ._lib import KvBatchStruct, KvMemoryStruct, check
+from .rows4 import dtype_code, on_device
+
+
+def _rows(x, what: str):
+    """x [tokens, heads, dim], or a copy of it, as the kernels read it: heads of contiguous numbers, 16-byte steps."""
+    s = x.stride()
+    if s[2] != 1 or s[0] % 8 or s[1] % 8 or s[0] < 0 or s[1] < 0 or x.data_ptr() % 16:
+        x = x.contiguous()
+        if x.data_ptr() % 16:
+            x = x.clone()
+    return x
+
+
+class KeyValueMemory:
+    """``pages`` pages of ``page_tokens`` tokens of ``kv_heads`` keys and values of ``head_dim`` numbers.
+
+    ``k``, ``v``: float8_e4m3fn [pages, kv_heads, page_tokens, head_dim]; ``k_scale``, ``v_scale``: float32
+    [pages, kv_heads].  A stored number is code * scale.  Which page holds what is the caller's: ``table`` [sequences, width]
+    int32, token t of sequence b lies in page table[b, t // page_tokens].  ``lengths`` [sequences] int32 counts a sequence's
+    tokens, the new ones of the call included, for ``append`` and ``attend`` alike."""
+
+    def __init__(self, pages: int, page_tokens: int, kv_heads: int, head_dim: int, device="cuda"):
+        import torch
+
+        code = lambda: torch.zeros((pages, kv_heads, page_tokens, head_dim), dtype=torch.uint8, device=device).view(torch.float8_e4m3fn)  # noqa: E731
+        scale = lambda: torch.ones((pages, kv_heads), dtype=torch.float32, device=device)  # noqa: E731
+        self._take(code(), code(), scale(), scale())
+
+    @classmethod
+    def from_tensors(cls, k, v, k_scale, v_scale) -> "KeyValueMemory":
+        """A memory that is these tensors (shared, not copied)."""
+        self = cls.__new__(cls)
+        self._take(k, v, k_scale, v_scale)
+        return self
+
+    def _take(self, k, v, k_scale, v_scale):
+        import torch
+
+        if k.dim() != 4 or k.shape != v.shape or k_scale.shape != k.shape[:2] or v_scale.shape != k.shape[:2]:
+            raise ValueError("expected k, v [pages, kv_heads, page_tokens, head_dim] and k_scale, v_scale [pages, kv_heads]")
+        if k.dtype != torch.float8_e4m3fn or v.dtype != torch.float8_e4m3fn or k_scale.dtype != torch.float32 or v_scale.dtype != torch.float32:
+            raise ValueError("k, v: float8_e4m3fn; k_scale, v_scale: float32")
+        tensors = (k, v, k_scale, v_scale)
+        if not all(t.is_cuda and t.device == k.device for t in tensors):
+            raise ValueError("k, v, k_scale, v_scale: CUDA tensors on one device")
+        if not all(t.is_contiguous() for t in tensors):
+            raise ValueError("k, v, k_scale, v_scale must be contiguous")
+        pages, heads, page_tokens, dim = k.shape
+        if page_tokens < 16 or page_tokens > 1024 or page_tokens & (page_tokens - 1):
+            raise ValueError("page_tokens must be a power of two in 16..1024")
+        if dim < 32 or dim > 256 or dim % 32:
+            raise ValueError("head_dim must be a multiple of 32 in 32..256")
+        self._l = _lib.lib()
+        self.k, self.v, self.k_scale, self.v_scale = tensors
+        self.device = k.device
+        self.kv_heads, self.page_tokens, self.head_dim = heads, page_tokens, dim
+        self._m = KvMemoryStruct(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), pages, heads, page_tokens, dim)
+
+    def _batch(self, table, lengths, offsets, max_new, tokens):
+        import torch
+
+        n = lengths.shape[0]
+        if table.dtype != torch.int32 or lengths.dtype != torch.int32 or table.dim() != 2 or lengths.dim() != 1 or table.shape[0] != n:
+            raise ValueError("table [sequences, width] and lengths [sequences]: int32")
+        if table.device != self.device or lengths.device != self.device or not (table.is_contiguous() and lengths.is_contiguous()):
+            raise ValueError(f"table and lengths: contiguous, on {self.device}")
+        if offsets is None:
+            if tokens != n:
+                raise ValueError(f"without offsets every sequence has one new token: {tokens} rows for {n} sequences")
+        elif offsets.dtype != torch.int32 or tuple(offsets.shape) != (n + 1,) or offsets.device != self.device or not offsets.is_contiguous():
+            raise ValueError(f"offsets: contiguous int32 [{n + 1}] on {self.device}")
+        return KvBatchStruct(table.data_ptr(), lengths.data_ptr(), None if offsets is None else offsets.data_ptr(), n, max(table.shape[1], 1), tokens, max_new)
+
+    def _check_rows(self, x, heads, what):
+        if x.dim() != 3 or x.shape[2] != self.head_dim or (heads and x.shape[1] != heads) or x.device != self.device:
+            raise ValueError(f"{what}: expected [tokens, {heads or 'heads'}, {self.head_dim}] on {self.device}, got {tuple(x.shape)} on {x.device}")
+
+    def append(self, k, v, table, lengths, *, offsets=None, max_new=None, queries=None, cos=None, sin=None, interleaved: bool = False):
+        """Stores the keys and values k, v [tokens, kv_heads, head_dim] of new tokens.
+
+        Row b is the last token of sequence b, or with ``offsets`` [sequences + 1] int32 rows offsets[b] .. offsets[b + 1] - 1
+        are its last ones (at most ``max_new`` of any sequence; by default all rows).  ``cos``, ``sin`` [positions, half]
+        float32 turn the first 2 * half numbers of each key by its position's angles, in pairs (d, d + half), or (2 i, 2 i + 1)
+        if ``interleaved``.  Returns ``queries`` [tokens, q_heads, head_dim], turned likewise (rows of no sequence: copied; None without queries)."""
+        import torch
+
+        self._check_rows(k, self.kv_heads, "k")
+        t = dtype_code(k, "k")
+        if v.shape != k.shape or v.dtype != k.dtype or v.device != k.device:
+            raise ValueError("k and v: one shape, type and device")
+        tokens = k.shape[0]
+        batch = self._batch(table, lengths, offsets, tokens if max_new is None else max_new, tokens)
+        rot = positions = 0
+        if (cos is None) != (sin is None):
+            raise ValueError("cos and sin go together")
+        if cos is not None:
+            if cos.dim() != 2 or cos.shape != sin.shape or cos.dtype != torch.float32 or sin.dtype != torch.float32:
+                raise ValueError("cos and sin: float32 [positions, half]")
+            if cos.device != self.device or sin.device != self.device or not (cos.is_contiguous() and sin.is_contiguous()):
+                raise ValueError(f"cos and sin: contiguous, on {self.device}")
+            positions, rot = cos.shape[0], 2 * cos.shape[1]
+        k, v = _rows(k, "k"), _rows(v, "v")
+        q = out = None
+        if queries is not None:
+            self._check_rows(queries, None, "queries")
+            if queries.shape[0] != tokens or queries.dtype != k.dtype:
+                raise ValueError(f"queries: [{tokens}, q_heads, {self.head_dim}] {k.dtype}")
+            out = queries
+            if rot:
+                q = _rows(queries, "queries")
+                out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        with on_device(self.device) as stream:
+            check(self._l.vdb_kv_append_device(self._m, batch, t, k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1),
+                                               None if cos is None else cos.data_ptr(), None if sin is None else sin.data_ptr(), positions, rot,
+                                               interleaved, None if q is None else q.data_ptr(), 0 if q is None else q.stride(0),
+                                               0 if q is None else q.stride(1), 0 if q is None else q.shape[1],
+                                               None if q is None else out.data_ptr(), stream))
+        return out
+
+    def attend(self, q, table, lengths, *, offsets=None, max_new=None, scale=None, window: int = 0, select=None, return_lse: bool = False):
+        """Attention of queries q [tokens, q_heads, head_dim] over the memory: [tokens, q_heads, head_dim] in q's type, and
+        with ``return_lse`` the logarithm of the softmax's sum, [tokens, q_heads] float32.
+
+        Rows as in ``append``.  A query sees its own token and those before it, with ``window`` only the last ``window`` of
+        them; with ``select`` [sequences, kv_heads, n] int64 (one new token per sequence) it sees the tokens with these
+        numbers, each as often as listed; numbers outside the sequence are skipped, as a search's padding is.
+        ``scale`` is 1 / sqrt(head_dim) unless given."""
+        import torch
+
+        self._check_rows(q, None, "q")
+        t = dtype_code(q, "q")
+        tokens, q_heads, dim = q.shape
+        if q_heads == 0 or q_heads % self.kv_heads:
+            raise ValueError(f"q: a multiple of {self.kv_heads} heads")
+        if window < 0:
+            raise ValueError("window must not be negative")
+        batch = self._batch(table, lengths, offsets, tokens if max_new is None else max_new, tokens)
+        n_select = 0
+        if select is not None:
+            if offsets is not None or window:
+                raise ValueError("select goes with one new token per sequence and no window")
+            if select.dtype != torch.int64 or select.dim() != 3 or tuple(select.shape[:2]) != (tokens, self.kv_heads) or select.device != self.device:
+                raise ValueError(f"select: int64 [{tokens}, {self.kv_heads}, n] on {self.device}")
+            select = select.contiguous()
+            n_select = select.shape[2]
+            if n_select == 0:  # nothing to see: a list of one number that no sequence has
+                select, n_select = torch.full((tokens, self.kv_heads, 1), -1, dtype=torch.int64, device=self.device), 1
+        q = _rows(q, "q")
+        # rows of no sequence are zeros
+        make = torch.empty if offsets is None else torch.zeros
+        out = make((tokens, q_heads, dim), dtype=q.dtype, device=self.device)
+        lse = make((tokens, q_heads), dtype=torch.float32, device=self.device) if return_lse else None
+        need = self._l.vdb_kv_attend_workspace(self._m, batch, q_heads, n_select)
+        work = torch.empty(need, dtype=torch.uint8, device=self.device) if need else None
+        with on_device(self.device) as stream:
+            check(self._l.vdb_kv_attend_device(self._m, batch, t, q.data_ptr(), q.stride(0), q.stride(1), q_heads,
+                                               float(dim) ** -0.5 if scale is None else float(scale), window,
+                                               None if select is None else select.data_ptr(), n_select, out.data_ptr(),
+                                               None if lse is None else lse.data_ptr(), None if work is None else work.data_ptr(), need, stream))
+        return (out, lse) if return_lse else out

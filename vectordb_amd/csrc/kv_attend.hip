@@ -86,201 +86,349 @@ struct Chunks {
     static constexpr int tile(int c) { return offset(c) / 16; }
 };
 
+// Work of one launch.  The tokens of a row tile are cut into `splits` ranges of `chunk` (a multiple of 128), one block each;
+// where more than one range holds tokens, the blocks leave (maximum, sum, output) in the workspace and kv_join adds them up
+// in the order of the ranges.
+struct Plan {
+    uint32_t tiles;   // row tiles of 16 that have blocks of their own (more than that are walked by the blocks of range 0)
+    uint32_t splits;
+    uint32_t chunk;
+    float* part;      // [sequence][head][tile][split][16][D + 2]
+};
+
+typedef const __attribute__((address_space(4))) int32_t* UniformI32;  // read through scalar registers
+typedef const __attribute__((address_space(4))) float* UniformF32;
+
+struct Sequence {
+    int64_t first, n_new, start, len;
+};
+
+__device__ __forceinline__ bool sequence_of(const KvAttendArgs& a, uint32_t b, Sequence& s) {
+    s.first = a.batch.offsets ? a.batch.offsets[b] : b;
+    s.n_new = a.batch.offsets ? (int64_t)a.batch.offsets[b + 1] - s.first : 1;
+    s.start = (int64_t)a.batch.lengths[b] - s.n_new;
+    s.len = min((int64_t)a.batch.lengths[b], (int64_t)a.batch.table_width << a.mem.page_shift);
+    return s.n_new > 0 && s.first >= 0 && s.first + s.n_new <= (int64_t)a.batch.tokens;
+}
+
+// Tokens (or places of the list of selected ones) [lo, hi) that rows row0 .. row1 see; lo is rounded down to the tiles of 32.
+template <bool SEL>
+__device__ __forceinline__ void range_of(const KvAttendArgs& a, const Sequence& s, int64_t pos0, int64_t pos1, int64_t& lo, int64_t& hi) {
+    hi = SEL ? (int64_t)a.n_select : max((int64_t)0, min(pos1 + 1, s.len));
+    lo = SEL || a.window == 0 ? 0 : max((int64_t)0, pos0 - a.window + 1);
+}
+
+__device__ __forceinline__ float max_of_quarters(float x) {  // over the lanes m, m + 16, m + 32, m + 48
+    auto r = __builtin_amdgcn_permlane16_swap(bits_of(x), bits_of(x), false, false);
+    x = __builtin_fmaxf(float_of(r[0]), float_of(r[1]));
+    r = __builtin_amdgcn_permlane32_swap(bits_of(x), bits_of(x), false, false);
+    return __builtin_fmaxf(float_of(r[0]), float_of(r[1]));
+}
+
+// One tile of 32 tokens as a lane holds it: of its two score rows 8 * DS code bytes each, of its 8 tokens 2 * DS each.
+template <int DS>
+struct Tile {
+    static constexpr int VW = DS / 4 * 2 + (DS >> 1 & 1) + (DS & 1);
+    u32x2 k[2][DS];
+    uint32_t v[8][VW];
+    float ks[8], vs[8];  // one value (in [0]) unless tokens are selected
+    uint32_t have;       // bit t: token t of the lane's 8 is there (all ones where every token of the tile is)
+    bool full;           // every row sees every token of the tile
+};
+
 template <int T, int DS, bool SEL>
-__global__ __launch_bounds__(256) void kv_attend(KvAttendArgs a) {
+__global__ __launch_bounds__(256) void kv_attend(KvAttendArgs a, Plan plan) {
     constexpr bool HALF = T == kF16;
     constexpr int NQ = T == kF32 ? 3 : 1, NP = Parts<T>::value, D = DS * 32, ND = DS * 2, LDO = Shape<T, DS>::LDO;
     extern __shared__ float smem[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int m = lane & 15, q4 = lane >> 4;
     const uint32_t b = blockIdx.z, head = blockIdx.y, H = a.mem.heads, P = a.mem.page_tokens, G = a.q_heads / H;
-    const int64_t first = a.batch.offsets ? a.batch.offsets[b] : b;
-    const int64_t n_new = a.batch.offsets ? (int64_t)a.batch.offsets[b + 1] - first : 1;
-    if (n_new <= 0 || first < 0 || first + n_new > (int64_t)a.batch.tokens) return;
-    const int64_t len = min((int64_t)a.batch.lengths[b], (int64_t)a.batch.table_width * P);
-    const int64_t start = (int64_t)a.batch.lengths[b] - n_new;
-    const int32_t* table = a.batch.table + (uint64_t)b * a.batch.table_width;
+    const uint32_t split = blockIdx.x % plan.splits;
+    Sequence s;
+    if (!sequence_of(a, b, s)) return;
+    const UniformI32 table = (UniformI32)(a.batch.table + (uint64_t)b * a.batch.table_width);
     const int64_t* select = SEL ? a.select + ((uint64_t)b * H + head) * a.n_select : nullptr;
-    const int64_t rows = n_new * G;
+    const int64_t rows = s.n_new * G;
     const uint8_t* kc = (const uint8_t*)a.mem.k;
     const uint8_t* vc = (const uint8_t*)a.mem.v;
+    const float to_log2 = a.scale * kLog2e;
 
-    for (int64_t row0 = (int64_t)blockIdx.x * 16; row0 < rows; row0 += (int64_t)gridDim.x * 16) {
+    for (int64_t rt = blockIdx.x / plan.splits; rt * 16 < rows; rt += plan.tiles) {
+        const int64_t row0 = rt * 16, row1 = min(row0 + 15, rows - 1);
+        // positions of the tile's first and last row; tokens [lo, hi) are seen by some row, [lo_all, hi_all) by every row
+        const int64_t pos0 = s.start + row0 / G, pos1 = s.start + row1 / G;
+        int64_t lo, hi;
+        range_of<SEL>(a, s, pos0, pos1, lo, hi);
+        const bool same = SEL || pos0 == pos1;
+        const int64_t lo_all = a.window == 0 ? 0 : max((int64_t)0, pos1 - a.window + 1), hi_all = SEL ? hi : min(pos0 + 1, hi);
+        int64_t kb0 = lo & ~31ll, kb1 = hi;
+        bool whole = true;  // this block sees all of the tile's tokens
+        if (plan.splits > 1) {
+            if (rt < plan.tiles) {
+                whole = kb1 - kb0 <= (int64_t)plan.chunk;
+                kb0 += (int64_t)split * plan.chunk;
+                kb1 = min(kb1, kb0 + (int64_t)plan.chunk);
+                if (split && kb0 >= kb1) continue;
+            } else if (split) {
+                continue;
+            }
+        }
         const int64_t r = row0 + m;
         const bool live = r < rows;
         const int64_t tok = live ? r / G : 0;
         const uint32_t qh = head * G + (live ? (uint32_t)(r - tok * G) : 0);
-        const int64_t pos = live ? start + tok : -1;
+        const int64_t pos = live ? s.start + tok : -1;
         u32x4 qf[NQ][DS];
         {
-            const E<T>* q = (const E<T>*)a.q + (uint64_t)(first + tok) * a.q_token + (uint64_t)qh * a.q_head + q4 * 8 * DS;
+            const E<T>* q = (const E<T>*)a.q + (uint64_t)(s.first + tok) * a.q_token + (uint64_t)qh * a.q_head + q4 * 8 * DS;
 #pragma unroll
             for (int j = 0; j < DS; ++j) {
                 if constexpr (T == kF32) {
                     const f32x4 x = live ? *(const f32x4*)(q + j * 8) : f32x4{0, 0, 0, 0};
                     const f32x4 y = live ? *(const f32x4*)(q + j * 8 + 4) : f32x4{0, 0, 0, 0};
 #pragma unroll
-                    for (int s = 0; s < NQ; ++s)
-                        qf[s][j] = u32x4{pack_hi16(bf16_part(x[0], s), bf16_part(x[1], s)), pack_hi16(bf16_part(x[2], s), bf16_part(x[3], s)),
-                                         pack_hi16(bf16_part(y[0], s), bf16_part(y[1], s)), pack_hi16(bf16_part(y[2], s), bf16_part(y[3], s))};
+                    for (int n = 0; n < NQ; ++n)
+                        qf[n][j] = u32x4{pack_hi16(bf16_part(x[0], n), bf16_part(x[1], n)), pack_hi16(bf16_part(x[2], n), bf16_part(x[3], n)),
+                                         pack_hi16(bf16_part(y[0], n), bf16_part(y[1], n)), pack_hi16(bf16_part(y[2], n), bf16_part(y[3], n))};
                 } else {
                     qf[0][j] = live ? *(const u32x4*)(q + j * 8) : u32x4{0, 0, 0, 0};
                 }
             }
         }
-        // positions of the tile's first and last row; tokens [lo, hi) are seen by some row, [lo_all, hi_all) by every row
-        const int64_t pos0 = start + row0 / G, pos1 = start + min(row0 + 15, rows - 1) / G;
-        const int64_t hi = SEL ? (int64_t)a.n_select : max((int64_t)0, min(pos1 + 1, len));
-        const int64_t lo = SEL || a.window == 0 ? 0 : max((int64_t)0, pos0 - a.window + 1);
-        const bool same = SEL || pos0 == pos1;
-        const int64_t lo_all = a.window == 0 ? 0 : max((int64_t)0, pos1 - a.window + 1), hi_all = pos0 + 1;
 
         f32x4 o[ND];
 #pragma unroll
         for (int d = 0; d < ND; ++d) o[d] = f32x4{0, 0, 0, 0};
         float top = kNone, sum = 0.0f;
 
-        for (int64_t kb = (lo & ~31ll) + wave * 32; kb < hi; kb += 128) {
-            // ---- where the tokens lie: two for the scores (row m of either tile), eight for the values
-            float ks[8], vs[8];
-            bool have[8];
-            int64_t koff[2];
-            int64_t voff[8];
-            auto place = [&](int64_t t) -> int64_t {  // row number of token t, or -1
-                if (t < 0 || t >= len) return -1;
-                const int32_t pid = table[t >> a.mem.page_shift];
-                if (pid < 0 || (uint64_t)pid >= a.mem.pages) return -1;
-                return (((int64_t)pid * H + head) << a.mem.page_shift) + (t & (P - 1));
-            };
+        // Fetches the tile at kb.  Tokens that are not there are never read from: their addresses are those of a page that is.
+        // Returns false (on all lanes) if no token of the tile is.
+        auto fetch = [&](int64_t kb, Tile<DS>& x) -> bool {
+            int64_t krow[2], vrow[8];
+            if constexpr (!SEL) {
+                int64_t page[2];
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const int64_t t = kb + 16 * h;
+                    page[h] = t < s.len ? (int64_t)table[t >> a.mem.page_shift] : -1;
+                    if (page[h] >= (int64_t)a.mem.pages) page[h] = -1;
+                }
+                if (page[0] < 0 && page[1] < 0) return false;
+                x.full = kb >= lo_all && kb + 32 <= hi_all && page[0] >= 0 && page[1] >= 0;
+                const int64_t p0 = (page[0] < 0 ? page[1] : page[0]) * H + head, p1 = (page[1] < 0 ? page[0] : page[1]) * H + head;
+                const float ks0 = ((UniformF32)a.mem.k_scale)[p0], ks1 = ((UniformF32)a.mem.k_scale)[p1];
+                const float vs0 = ((UniformF32)a.mem.v_scale)[p0], vs1 = ((UniformF32)a.mem.v_scale)[p1];
+                x.ks[0] = q4 < 2 ? ks0 : ks1;
+                x.vs[0] = q4 < 2 ? vs0 : vs1;
+                const int64_t r0 = (p0 << a.mem.page_shift) + (kb & (P - 1)), r1 = (p1 << a.mem.page_shift) + ((kb + 16) & (P - 1)) - 16;
+                krow[0] = (m < 8 ? r0 : r1) + (m >> 2) * 8 + (m & 3);
+                krow[1] = krow[0] + 4;
+                vrow[0] = (q4 < 2 ? r0 : r1) + q4 * 8;
+#pragma unroll
+                for (int t = 1; t < 8; ++t) vrow[t] = vrow[0] + t;
+                x.have = ~0u;
+                if (!x.full) {
+                    x.have = 0;
+#pragma unroll
+                    for (int t = 0; t < 8; ++t) {
+                        const int64_t i = kb + q4 * 8 + t;
+                        x.have |= (i >= lo && i < hi && page[q4 >> 1] >= 0 ? 1u : 0u) << t;
+                    }
+                }
+            } else {
+                // lanes 0-31 look the 32 places of the list up (and the keys' scales), lanes 32-63 likewise with the values' scales
+                int64_t* row_s = (int64_t*)(smem) + wave * 64;  // [32] row numbers, then [64] scales
+                float* scale_s = (float*)(row_s + 32);
+                const int64_t i = kb + (lane & 31);
+                const int64_t t = i < hi ? select[i] : -1;
+                int64_t page = -1;
+                if (t >= 0 && t < s.len) page = a.batch.table[(uint64_t)b * a.batch.table_width + (t >> a.mem.page_shift)];
+                const bool there = page >= 0 && page < (int64_t)a.mem.pages;
+                const uint64_t any = __ballot(there);
+                if (!any) return false;
+                const int64_t ph = page * H + head;
+                const float sc = there ? (lane < 32 ? a.mem.k_scale : a.mem.v_scale)[ph] : 0.0f;
+                int64_t row = there ? (ph << a.mem.page_shift) + (t & (P - 1)) : -1;
+                if (lane < 32) row_s[lane] = row;
+                scale_s[lane] = sc;
+                __builtin_amdgcn_wave_barrier();
+                krow[0] = row_s[(m >> 2) * 8 + (m & 3)];
+                krow[1] = row_s[(m >> 2) * 8 + 4 + (m & 3)];
+                x.have = 0;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    vrow[e] = row_s[q4 * 8 + e];
+                    x.have |= (vrow[e] >= 0 ? 1u : 0u) << e;
+                    x.ks[e] = scale_s[q4 * 8 + e];
+                    x.vs[e] = scale_s[32 + q4 * 8 + e];
+                }
+                __builtin_amdgcn_wave_barrier();
+                x.full = (uint32_t)any == ~0u;
+                if (!x.full) {  // row 0 of the memory exists, as some row does
+                    krow[0] = max(krow[0], (int64_t)0);
+                    krow[1] = max(krow[1], (int64_t)0);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) vrow[e] = max(vrow[e], (int64_t)0);
+                }
+            }
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
-                const int64_t i = kb + (m >> 2) * 8 + t * 4 + (m & 3);
-                koff[t] = i >= lo && i < hi ? place(SEL ? select[i] : i) : -1;
+                const uint8_t* p = kc + krow[t] * D + q4 * 8 * DS;
+#pragma unroll
+                for (int j = 0; j < DS; ++j) x.k[t][j] = *(const u32x2*)(p + j * 8);
             }
 #pragma unroll
             for (int t = 0; t < 8; ++t) {
-                const int64_t i = kb + q4 * 8 + t;
-                voff[t] = i >= lo && i < hi ? place(SEL ? select[i] : i) : -1;
-                have[t] = voff[t] >= 0;
-                const uint64_t page = have[t] ? (uint64_t)voff[t] >> a.mem.page_shift : 0;
-                ks[t] = have[t] ? a.mem.k_scale[page] : 0.0f;
-                vs[t] = have[t] ? a.mem.v_scale[page] : 0.0f;
+                const uint8_t* p = vc + vrow[t] * D;
+#pragma unroll
+                for (int c = 0; c < DS / 4; ++c) {
+                    const u32x2 y = *(const u32x2*)(p + c * 128 + m * 8);
+                    x.v[t][2 * c] = y[0];
+                    x.v[t][2 * c + 1] = y[1];
+                }
+                if constexpr (DS & 2) x.v[t][DS / 4 * 2] = *(const uint32_t*)(p + DS / 4 * 128 + m * 4);
+                if constexpr (DS & 1) x.v[t][Tile<DS>::VW - 1] = *(const uint16_t*)(p + DS / 2 * 64 + m * 2);
             }
+            return true;
+        };
+
+        auto work = [&](int64_t kb, Tile<DS>& x) {
             f32x4 sc[2];
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
                 sc[t] = f32x4{0, 0, 0, 0};
-                const uint8_t* kp = kc + (koff[t] < 0 ? 0 : koff[t]) * D + q4 * 8 * DS;
 #pragma unroll
                 for (int j = 0; j < DS; ++j) {
-                    const u32x2 w = koff[t] >= 0 ? *(const u32x2*)(kp + j * 8) : u32x2{0, 0};
-                    const u32x4 kf = widen<HALF>(w[0], w[1]);
+                    const u32x4 kf = widen<HALF>(x.k[t][j][0], x.k[t][j][1]);
 #pragma unroll
-                    for (int s = 0; s < NQ; ++s) sc[t] = mfma<HALF>(kf, qf[s][j], sc[t]);
+                    for (int n = 0; n < NQ; ++n) sc[t] = mfma<HALF>(kf, qf[n][j], sc[t]);
                 }
             }
             // ---- softmax over what the lane's row sees of its 8 tokens
             float p[8];
-            bool seen[8];
-            float now = top;
 #pragma unroll
-            for (int t = 0; t < 8; ++t) {
-                const int64_t i = kb + q4 * 8 + t;
-                seen[t] = live && have[t] && (SEL || (i <= pos && (a.window == 0 || i > pos - a.window)));
-                p[t] = sc[t >> 2][t & 3] * (ks[t] * (a.scale * kLog2e));
-                if (seen[t] && !(p[t] <= now)) now = p[t];
+            for (int t = 0; t < 8; ++t) p[t] = sc[t >> 2][t & 3] * (x.ks[SEL ? t : 0] * to_log2);
+            uint32_t seen = 255;
+            if (!x.full) {
+                seen = live ? x.have : 0;
+                if constexpr (!SEL) {
+#pragma unroll
+                    for (int t = 0; t < 8; ++t) {
+                        const int64_t i = kb + q4 * 8 + t;
+                        if (!(i <= pos && (a.window == 0 || i > pos - a.window))) seen &= ~(1u << t);
+                    }
+                }
+#pragma unroll
+                for (int t = 0; t < 8; ++t) p[t] = seen >> t & 1 ? p[t] : -__builtin_inff();
+                // what no row sees may hold anything: it is taken for zeros
+#pragma unroll
+                for (int t = 0; t < 8; ++t)
+#pragma unroll
+                    for (int w = 0; w < Tile<DS>::VW; ++w) x.v[t][w] = x.have >> t & 1 ? x.v[t][w] : 0;
             }
-            now = __builtin_fmaxf(now, __shfl_xor(now, 16));
-            now = __builtin_fmaxf(now, __shfl_xor(now, 32));
-            const float shrink = exp2f(top - now);
-            top = now;
-            sum *= shrink;
+            float now = __builtin_fmaxf(__builtin_fmaxf(__builtin_fmaxf(p[0], p[1]), __builtin_fmaxf(p[2], p[3])),
+                                        __builtin_fmaxf(__builtin_fmaxf(p[4], p[5]), __builtin_fmaxf(p[6], p[7])));
+            now = max_of_quarters(now);
+            if (__any(now > top)) {
+                now = __builtin_fmaxf(now, top);
+                const float shrink = __builtin_amdgcn_exp2f(top - now);
+                top = now;
+                sum *= shrink;
+#pragma unroll
+                for (int d = 0; d < ND; ++d) o[d] *= shrink;
+            }
 #pragma unroll
             for (int t = 0; t < 8; ++t) {
-                p[t] = seen[t] ? exp2f(p[t] - now) : 0.0f;
+                p[t] = __builtin_amdgcn_exp2f(p[t] - top);
                 sum += p[t];
-                p[t] *= vs[t];
+                p[t] *= x.vs[SEL ? t : 0];
+            }
+            if (!x.full) {  // (a scale that belongs to no token may hold anything)
+#pragma unroll
+                for (int t = 0; t < 8; ++t) p[t] = seen >> t & 1 ? p[t] : 0.0f;
             }
             u32x4 pf[NP];
 #pragma unroll
-            for (int s = 0; s < NP; ++s) {
+            for (int n = 0; n < NP; ++n) {
 #pragma unroll
                 for (int t = 0; t < 4; ++t) {
                     if constexpr (NP == 1) {
                         bf16x2 w = {(__bf16)p[2 * t], (__bf16)p[2 * t + 1]};
-                        pf[s][t] = __builtin_bit_cast(uint32_t, w);
+                        pf[n][t] = __builtin_bit_cast(uint32_t, w);
                     } else {
-                        pf[s][t] = pack_hi16(bf16_part(p[2 * t], s), bf16_part(p[2 * t + 1], s));
+                        pf[n][t] = pack_hi16(bf16_part(p[2 * t], n), bf16_part(p[2 * t + 1], n));
                     }
                 }
             }
+            // a NaN among values that some rows of the tile do not see must not reach those (0 * NaN)
+            bool mixed = false;
+            if (!SEL && !x.full && !same) {
+                uint32_t odd = 0;
 #pragma unroll
-            for (int d = 0; d < ND; ++d) o[d] *= shrink;
+                for (int t = 0; t < 8; ++t)
+#pragma unroll
+                    for (int w = 0; w < Tile<DS>::VW; ++w) odd |= nan_bytes(x.v[t][w]);
+                mixed = __any(odd != 0);
+            }
             // ---- values: chunks of w dimensions a lane
 #pragma unroll
             for (int c = 0; c < Chunks<DS>::count; ++c) {
-                const int w = Chunks<DS>::width(c), off = Chunks<DS>::offset(c) + m * w;
+                const int w = Chunks<DS>::width(c), word = c <= DS / 4 ? 2 * c : 2 * (DS / 4) + 1;
                 uint32_t col[8][2];  // [dimension][tokens 0-3, 4-7]
-                uint32_t odd = 0;
 #pragma unroll
                 for (int hf = 0; hf < 2; ++hf) {
-                    uint32_t x[4][2];
-#pragma unroll
-                    for (int t = 0; t < 4; ++t) {
-                        const uint8_t* vp = vc + (have[hf * 4 + t] ? voff[hf * 4 + t] : 0) * D + off;
-                        x[t][0] = x[t][1] = 0;
-                        if (have[hf * 4 + t]) {
-                            if (w == 8) {
-                                const u32x2 y = *(const u32x2*)vp;
-                                x[t][0] = y[0], x[t][1] = y[1];
-                            } else if (w == 4) {
-                                x[t][0] = *(const uint32_t*)vp;
-                            } else {
-                                x[t][0] = *(const uint16_t*)vp;
-                            }
-                        }
-                        odd |= nan_bytes(x[t][0]) | nan_bytes(x[t][1]);
-                    }
 #pragma unroll
                     for (int g = 0; g < (w + 3) / 4; ++g) {
-                        const uint32_t in[4] = {x[0][g], x[1][g], x[2][g], x[3][g]};
+                        const uint32_t in[4] = {x.v[hf * 4][word + g], x.v[hf * 4 + 1][word + g], x.v[hf * 4 + 2][word + g], x.v[hf * 4 + 3][word + g]};
                         uint32_t out[4];
                         transpose4(in, out);
 #pragma unroll
                         for (int e = 0; e < 4 && g * 4 + e < w; ++e) col[g * 4 + e][hf] = out[e];
                     }
                 }
-                // a NaN among values that some rows of the tile do not see must not reach those (0 * NaN)
-                const bool mixed = !same && (kb < lo_all || kb + 32 > hi_all) && __any(odd != 0);
 #pragma unroll
                 for (int e = 0; e < w; ++e) {
                     const int d = Chunks<DS>::tile(c) + e;
-                    uint32_t x = col[e][0], y = col[e][1];
+                    uint32_t y = col[e][0], z = col[e][1];
                     if (mixed) {
-                        const uint32_t nx = nan_bytes(x) >> 7, ny = nan_bytes(y) >> 7;  // 1 in the bytes that are NaN
-                        x &= ~(nx * 255u);
+                        const uint32_t ny = nan_bytes(y) >> 7, nz = nan_bytes(z) >> 7;  // 1 in the bytes that are NaN
                         y &= ~(ny * 255u);
-                        const u32x4 is_nan = widen<false>(nx * 0x38u, ny * 0x38u);  // 0x38 = 1.0
+                        z &= ~(nz * 255u);
+                        const u32x4 is_nan = widen<false>(ny * 0x38u, nz * 0x38u);  // 0x38 = 1.0
                         u32x4 sees;
 #pragma unroll
-                        for (int t = 0; t < 4; ++t) sees[t] = (seen[2 * t] ? 0x3F80u : 0u) | (seen[2 * t + 1] ? 0x3F800000u : 0u);
+                        for (int t = 0; t < 4; ++t) sees[t] = (seen >> (2 * t) & 1 ? 0x3F80u : 0u) | (seen >> (2 * t + 1) & 1 ? 0x3F800000u : 0u);
                         const f32x4 n = mfma<false>(is_nan, sees, f32x4{0, 0, 0, 0});
 #pragma unroll
                         for (int i = 0; i < 4; ++i)
                             if (n[i] > 0.0f) o[d][i] = float_of(0x7FC00000u);
                     }
-                    const u32x4 vf = widen<false>(x, y);
+                    const u32x4 vf = widen<false>(y, z);
 #pragma unroll
-                    for (int s = 0; s < NP; ++s) o[d] = mfma<false>(vf, pf[s], o[d]);
+                    for (int n = 0; n < NP; ++n) o[d] = mfma<false>(vf, pf[n], o[d]);
                 }
             }
+        };
+
+        // the next tile is on its way while one is worked on
+        Tile<DS> ta, tb;
+        int64_t kb = kb0 + wave * 32;
+        bool fa = kb < kb1 && fetch(kb, ta), fb;
+        for (; kb < kb1; kb += 256) {
+            fb = kb + 128 < kb1 && fetch(kb + 128, tb);
+            if (fa) work(kb, ta);
+            fa = kb + 256 < kb1 && fetch(kb + 256, ta);
+            if (fb) work(kb + 128, tb);
         }
+
         // ---- join the four waves: each row's maximum, then sums and outputs in wave order
-        float* so = smem;                    // [4][16][LDO]
-        float* st = smem + 4 * 16 * LDO;     // [4][16] maxima
-        float* ss = st + 64;                 // [4][16] sums
+        float* so = smem;                 // [4][16][LDO]
+        float* st = smem + 4 * 16 * LDO;  // [4][16] maxima
+        float* ss = st + 64;              // [4][16] sums
         sum += __shfl_xor(sum, 16);
         sum += __shfl_xor(sum, 32);
+        if (SEL) __syncthreads();  // the look-up tables of the waves lie there as well
         if (q4 == 0) st[wave * 16 + m] = top, ss[wave * 16 + m] = sum;
 #pragma unroll
         for (int c = 0; c < Chunks<DS>::count; ++c) {
@@ -295,40 +443,131 @@ __global__ __launch_bounds__(256) void kv_attend(KvAttendArgs a) {
         const int row = threadIdx.x >> 4, part = threadIdx.x & 15;
         float best = kNone;
 #pragma unroll
-        for (int w = 0; w < 4; ++w) best = fmaxf(best, st[w * 16 + row]);
+        for (int w = 0; w < 4; ++w) best = __builtin_fmaxf(best, st[w * 16 + row]);
         float f[4], total = 0.0f;
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
-            f[w] = exp2f(st[w * 16 + row] - best);
+            f[w] = __builtin_amdgcn_exp2f(st[w * 16 + row] - best);
             total += f[w] * ss[w * 16 + row];
         }
         if (row0 + row < rows) {
-            const int64_t ot = (row0 + row) / G;
-            const uint64_t orow = (uint64_t)(first + ot) * a.q_heads + head * G + (uint32_t)(row0 + row - ot * G);
-            const bool none = total == 0.0f;  // (a NaN is something)
-            const float inv = none ? 0.0f : 1.0f / total;
-            E<T>* out = (E<T>*)a.out + orow * D + part * ND;
+            float v[ND];
 #pragma unroll
             for (int d = 0; d < ND; ++d) {
-                float v = 0.0f;
+                v[d] = 0.0f;
 #pragma unroll
-                for (int w = 0; w < 4; ++w) v += f[w] * so[(w * 16 + row) * LDO + part * ND + d];
-                out[d] = (E<T>)(none ? 0.0f : v * inv);
+                for (int w = 0; w < 4; ++w) v[d] += f[w] * so[(w * 16 + row) * LDO + part * ND + d];
             }
-            if (a.lse && part == 0) a.lse[orow] = none ? -__builtin_inff() : (best + log2f(total)) * kLn2;
+            if (whole) {
+                const int64_t ot = (row0 + row) / G;
+                const uint64_t orow = (uint64_t)(s.first + ot) * a.q_heads + head * G + (uint32_t)(row0 + row - ot * G);
+                const bool none = total == 0.0f;  // (a NaN is something)
+                const float inv = none ? 0.0f : 1.0f / total;
+                E<T>* out = (E<T>*)a.out + orow * D + part * ND;
+#pragma unroll
+                for (int d = 0; d < ND; ++d) out[d] = (E<T>)(none ? 0.0f : v[d] * inv);
+                if (a.lse && part == 0) a.lse[orow] = none ? -__builtin_inff() : (best + __builtin_amdgcn_logf(total)) * kLn2;
+            } else {
+                float* w = plan.part + (((((uint64_t)b * H + head) * plan.tiles + rt) * plan.splits + split) * 16 + row) * (D + 2);
+#pragma unroll
+                for (int d = 0; d < ND; d += 2) *(f32x2*)(w + part * ND + d) = f32x2{v[d], v[d + 1]};
+                if (part == 0) *(f32x2*)(w + D) = f32x2{best, total};
+            }
         }
         __syncthreads();
     }
 }
 
+// Adds up the ranges of one row: block (row, head, sequence).
+template <int T, bool SEL>
+__global__ __launch_bounds__(256) void kv_join(KvAttendArgs a, Plan plan) {
+    __shared__ float red[256 * 4];
+    __shared__ float mx[4], sums[32];
+    const uint32_t b = blockIdx.z, head = blockIdx.y, H = a.mem.heads, G = a.q_heads / H, D = a.mem.dim;
+    Sequence s;
+    if (!sequence_of(a, b, s)) return;
+    const int64_t row = blockIdx.x, rows = s.n_new * G, rt = row / 16;
+    if (row >= rows) return;
+    int64_t lo, hi;
+    range_of<SEL>(a, s, s.start + rt * 16 / G, s.start + min(rt * 16 + 15, rows - 1) / G, lo, hi);
+    const int64_t used64 = (hi - (lo & ~31ll) + plan.chunk - 1) / plan.chunk;
+    if (used64 <= 1) return;  // written by kv_attend
+    const uint32_t used = (uint32_t)min(used64, (int64_t)plan.splits);
+    const uint64_t step = 16 * (D + 2);
+    const float* part = plan.part + ((((uint64_t)b * H + head) * plan.tiles + rt) * plan.splits * 16 + row % 16) * (D + 2);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    float best = kNone;
+    for (uint32_t i = threadIdx.x; i < used; i += 256) best = __builtin_fmaxf(best, part[i * step + D]);
+#pragma unroll
+    for (int o = 32; o; o >>= 1) best = __builtin_fmaxf(best, __shfl_xor(best, o));
+    if (lane == 0) mx[wave] = best;
+    __syncthreads();
+    best = __builtin_fmaxf(__builtin_fmaxf(mx[0], mx[1]), __builtin_fmaxf(mx[2], mx[3]));
+    // groups of D / 4 threads, each thread four dimensions of every groups-th range
+    const uint32_t width = D / 4, groups = 256 / width, g = threadIdx.x / width, d = threadIdx.x % width * 4;
+    f32x4 acc = {0, 0, 0, 0};
+    float total = 0.0f;
+    if (g < groups) {
+        for (uint32_t i = g; i < used; i += groups) {
+            const float* w = part + i * step;
+            const f32x2 x = *(const f32x2*)(w + d), y = *(const f32x2*)(w + d + 2), z = *(const f32x2*)(w + D);
+            const float f = __builtin_amdgcn_exp2f(z[0] - best);
+            total += f * z[1];
+            acc += f32x4{x[0], x[1], y[0], y[1]} * f;
+        }
+    }
+    *(f32x4*)(red + threadIdx.x * 4) = acc;
+    if (g < groups && d == 0) sums[g] = total;
+    __syncthreads();
+    if (threadIdx.x < width) {
+        float sum = 0.0f;
+        f32x4 v = {0, 0, 0, 0};
+        for (uint32_t i = 0; i < groups; ++i) {
+            sum += sums[i];
+            v += *(const f32x4*)(red + (i * width + threadIdx.x) * 4);
+        }
+        const int64_t ot = row / G;
+        const uint64_t orow = (uint64_t)(s.first + ot) * a.q_heads + head * G + (uint32_t)(row - ot * G);
+        const bool none = sum == 0.0f;
+        const float inv = none ? 0.0f : 1.0f / sum;
+        E<T>* out = (E<T>*)a.out + orow * D + threadIdx.x * 4;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) out[i] = (E<T>)(none ? 0.0f : v[i] * inv);
+        if (a.lse && threadIdx.x == 0) a.lse[orow] = none ? -__builtin_inff() : (best + __builtin_amdgcn_logf(sum)) * kLn2;
+    }
+}
+
 template <int T, int DS>
-hipError_t launch_one(const KvAttendArgs& a, uint32_t max_new, hipStream_t stream) {
-    const uint32_t G = a.q_heads / a.mem.heads;
-    const uint32_t tiles = (uint32_t)std::min<uint64_t>(((uint64_t)max_new * G + 15) / 16, 65535);
-    const dim3 grid(tiles, a.mem.heads, a.batch.count);
-    if (a.select) hipLaunchKernelGGL((kv_attend<T, DS, true>), grid, dim3(256), (Shape<T, DS>::lds), stream, a);
-    else hipLaunchKernelGGL((kv_attend<T, DS, false>), grid, dim3(256), (Shape<T, DS>::lds), stream, a);
+hipError_t launch_one(const KvAttendArgs& a, const Plan& plan, hipStream_t stream) {
+    const dim3 grid(plan.tiles * plan.splits, a.mem.heads, a.batch.count);
+    if (a.select) hipLaunchKernelGGL((kv_attend<T, DS, true>), grid, dim3(256), (Shape<T, DS>::lds), stream, a, plan);
+    else hipLaunchKernelGGL((kv_attend<T, DS, false>), grid, dim3(256), (Shape<T, DS>::lds), stream, a, plan);
     return hipGetLastError();
+}
+
+template <int T>
+hipError_t launch_join(const KvAttendArgs& a, const Plan& plan, uint32_t rows, hipStream_t stream) {
+    const dim3 grid(std::min(rows, plan.tiles * 16), a.mem.heads, a.batch.count);
+    if (a.select) hipLaunchKernelGGL((kv_join<T, true>), grid, dim3(256), 0, stream, a, plan);
+    else hipLaunchKernelGGL((kv_join<T, false>), grid, dim3(256), 0, stream, a, plan);
+    return hipGetLastError();
+}
+
+// How a launch is cut, from what the host knows: the table's width (or the list's length, or the window) bounds the tokens.
+Plan plan_of(const KvAttendArgs& a, uint32_t max_new) {
+    const uint32_t G = a.q_heads / a.mem.heads;
+    Plan p{};
+    p.tiles = (uint32_t)std::min<uint64_t>(((uint64_t)max_new * G + 15) / 16, 65535);
+    uint64_t tokens = a.select ? a.n_select : (uint64_t)a.batch.table_width << a.mem.page_shift;
+    if (!a.select && a.window) tokens = std::min<uint64_t>(tokens, (uint64_t)a.window + max_new + 31);
+    const uint64_t blocks = (uint64_t)p.tiles * a.mem.heads * a.batch.count;
+    // as many ranges as give some 4096 blocks, none shorter than 512 tokens
+    const uint64_t want = std::max<uint64_t>(1, 4096 / blocks);
+    uint64_t chunk = std::max<uint64_t>(512, (tokens + want - 1) / want);
+    chunk = (chunk + 127) / 128 * 128;
+    p.chunk = (uint32_t)std::min<uint64_t>(chunk, 1u << 30);
+    p.splits = (uint32_t)((tokens + p.chunk - 1) / p.chunk);
+    return p;
 }
 
 }  // namespace
@@ -340,30 +579,37 @@ hipError_t launch_one(const KvAttendArgs& a, uint32_t max_new, hipStream_t strea
 #define VDB_CAT(a, b) VDB_CAT2(a, b)
 
 // compiled once per element type (-DVDB_PART = vdb_dtype)
-hipError_t VDB_CAT(kv_attend_launch_, VDB_PART)(const KvAttendArgs& a, uint32_t max_new, hipStream_t stream) {
+hipError_t VDB_CAT(kv_attend_launch_, VDB_PART)(const KvAttendArgs& a, uint32_t max_new, void* workspace, hipStream_t stream) {
+    Plan plan = plan_of(a, max_new);
+    plan.part = (float*)workspace;
+    hipError_t e = hipErrorInvalidValue;
     switch (a.mem.dim / 32) {
-        case 1: return launch_one<VDB_PART, 1>(a, max_new, stream);
-        case 2: return launch_one<VDB_PART, 2>(a, max_new, stream);
-        case 3: return launch_one<VDB_PART, 3>(a, max_new, stream);
-        case 4: return launch_one<VDB_PART, 4>(a, max_new, stream);
-        case 5: return launch_one<VDB_PART, 5>(a, max_new, stream);
-        case 6: return launch_one<VDB_PART, 6>(a, max_new, stream);
-        case 7: return launch_one<VDB_PART, 7>(a, max_new, stream);
-        case 8: return launch_one<VDB_PART, 8>(a, max_new, stream);
+        case 1: e = launch_one<VDB_PART, 1>(a, plan, stream); break;
+        case 2: e = launch_one<VDB_PART, 2>(a, plan, stream); break;
+        case 3: e = launch_one<VDB_PART, 3>(a, plan, stream); break;
+        case 4: e = launch_one<VDB_PART, 4>(a, plan, stream); break;
+        case 5: e = launch_one<VDB_PART, 5>(a, plan, stream); break;
+        case 6: e = launch_one<VDB_PART, 6>(a, plan, stream); break;
+        case 7: e = launch_one<VDB_PART, 7>(a, plan, stream); break;
+        case 8: e = launch_one<VDB_PART, 8>(a, plan, stream); break;
     }
-    return hipErrorInvalidValue;
+    if (e == hipSuccess && plan.splits > 1) e = launch_join<VDB_PART>(a, plan, (uint32_t)std::min<uint64_t>((uint64_t)max_new * (a.q_heads / a.mem.heads), 1u << 30), stream);
+    return e;
 }
 
 #if VDB_PART == 0
-hipError_t kv_attend_launch_1(const KvAttendArgs&, uint32_t, hipStream_t);
-hipError_t kv_attend_launch_2(const KvAttendArgs&, uint32_t, hipStream_t);
+hipError_t kv_attend_launch_1(const KvAttendArgs&, uint32_t, void*, hipStream_t);
+hipError_t kv_attend_launch_2(const KvAttendArgs&, uint32_t, void*, hipStream_t);
 
-size_t kv_attend_workspace_bytes(const KvAttendArgs&, uint32_t) { return 0; }
+size_t kv_attend_workspace_bytes(const KvAttendArgs& a, uint32_t max_new) {
+    const Plan p = plan_of(a, max_new);
+    return p.splits > 1 ? (size_t)a.batch.count * a.mem.heads * p.tiles * p.splits * 16 * (a.mem.dim + 2) * 4 : 0;
+}
 
-int launch_kv_attend(const KvAttendArgs& a, int dtype, uint32_t max_new, void*, hipStream_t stream, std::string* err) {
-    const hipError_t e = dtype == kF32 ? kv_attend_launch_0(a, max_new, stream)
-                         : dtype == kF16 ? kv_attend_launch_1(a, max_new, stream)
-                                         : kv_attend_launch_2(a, max_new, stream);
+int launch_kv_attend(const KvAttendArgs& a, int dtype, uint32_t max_new, void* workspace, hipStream_t stream, std::string* err) {
+    const hipError_t e = dtype == kF32 ? kv_attend_launch_0(a, max_new, workspace, stream)
+                         : dtype == kF16 ? kv_attend_launch_1(a, max_new, workspace, stream)
+                                         : kv_attend_launch_2(a, max_new, workspace, stream);
     if (e == hipSuccess) return 0;
     if (err) *err = std::string("kv_attend: ") + hipGetErrorString(e);
     return 3;

@@ -293,7 +293,7 @@ typedef struct vdb_kv_memory {
     void* v;         /* likewise */
     float* k_scale;  /* [pages][heads], positive and finite where a page holds tokens */
     float* v_scale;
-    size_t pages;        /* < 2^31 */
+    size_t pages;        /* 1..2^31-1 */
     size_t heads;        /* key / value heads, 1..32767 */
     size_t page_tokens;  /* a power of two, 16..1024 */
     size_t dim;          /* a multiple of 32, 32..256 */
@@ -305,7 +305,7 @@ typedef struct vdb_kv_batch {
                               * last tokens of sequence b (rows of no sequence are left alone; a sequence whose rows do not lie
                               * in 0..tokens-1 has none).  NULL: row b is sequence b's last token, and tokens = count */
     size_t count;            /* sequences, at most 65535 */
-    size_t table_width;      /* pages a row of the table has room for, >= 1 */
+    size_t table_width;      /* pages a row of the table has room for, >= 1; for attention table_width * page_tokens < 2^31 - 1024 */
     size_t tokens;           /* rows of the new tokens' arrays, < 2^31 */
     size_t max_new;          /* most new tokens of any sequence (a size for launches: a wrong one costs time, not correctness) */
 } vdb_kv_batch;

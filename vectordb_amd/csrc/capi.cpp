@@ -1824,7 +1824,7 @@ KvMemory kv_memory(const vdb_kv_memory* m) {
         throw std::invalid_argument("kv memory: page_tokens must be a power of two in 16..1024");
     if (m->dim < 32 || m->dim > 256 || m->dim % 32) throw std::invalid_argument("kv memory: dim must be a multiple of 32 in 32..256");
     if (m->heads < 1 || m->heads > 32767) throw std::invalid_argument("kv memory: heads must be in 1..32767");
-    if (m->pages >= (1ull << 31)) throw std::invalid_argument("kv memory: pages must be below 2^31");
+    if (m->pages < 1 || m->pages >= (1ull << 31)) throw std::invalid_argument("kv memory: pages must be in 1..2^31-1");
     uint32_t shift = 4;
     while ((1u << shift) < m->page_tokens) ++shift;
     return KvMemory{m->k, m->v, m->k_scale, m->v_scale, m->pages, (uint32_t)m->heads, (uint32_t)m->page_tokens, shift, (uint32_t)m->dim};
@@ -1864,9 +1864,11 @@ KvAttendArgs kv_attend_args(const vdb_kv_memory* memory, const vdb_kv_batch* bat
     KvAttendArgs a{};
     a.mem = kv_memory(memory);
     a.batch = kv_batch(batch);
+    if (((uint64_t)a.batch.table_width << a.mem.page_shift) >= (1ull << 31) - 1024)
+        throw std::invalid_argument("kv attend: table_width * page_tokens must be below 2^31 - 1024");
     if (q_heads < 1 || q_heads % a.mem.heads || q_heads / a.mem.heads > 65535)
         throw std::invalid_argument("kv attend: q_heads must be a multiple of the memory's heads");
-    if (n_select >= (1ull << 31)) throw std::invalid_argument("kv attend: n_select must be below 2^31");
+    if (n_select >= (1ull << 31) - 1024) throw std::invalid_argument("kv attend: n_select must be below 2^31 - 1024");
     a.q_heads = (uint32_t)q_heads;
     a.n_select = (uint32_t)n_select;
     return a;

@@ -99,23 +99,28 @@ struct Plan {
 typedef const __attribute__((address_space(4))) int32_t* UniformI32;  // read through scalar registers
 typedef const __attribute__((address_space(4))) float* UniformF32;
 
+// Token numbers fit 32 bits with room to step past the end (the host checks the table's width and the list's length).
 struct Sequence {
-    int64_t first, n_new, start, len;
+    int64_t first;
+    int32_t n_new, start, len;  // start: position of the first new token, negative if the length counts fewer tokens
 };
 
 __device__ __forceinline__ bool sequence_of(const KvAttendArgs& a, uint32_t b, Sequence& s) {
     s.first = a.batch.offsets ? a.batch.offsets[b] : b;
-    s.n_new = a.batch.offsets ? (int64_t)a.batch.offsets[b + 1] - s.first : 1;
-    s.start = (int64_t)a.batch.lengths[b] - s.n_new;
-    s.len = min((int64_t)a.batch.lengths[b], (int64_t)a.batch.table_width << a.mem.page_shift);
-    return s.n_new > 0 && s.first >= 0 && s.first + s.n_new <= (int64_t)a.batch.tokens;
+    const int64_t n = a.batch.offsets ? (int64_t)a.batch.offsets[b + 1] - s.first : 1;
+    if (n <= 0 || s.first < 0 || s.first + n > (int64_t)a.batch.tokens) return false;
+    const int32_t held = max(a.batch.lengths[b], 0);
+    s.n_new = (int32_t)n;
+    s.start = held - s.n_new;
+    s.len = (int32_t)min((int64_t)held, (int64_t)a.batch.table_width << a.mem.page_shift);
+    return true;
 }
 
 // Tokens (or places of the list of selected ones) [lo, hi) that rows row0 .. row1 see; lo is rounded down to the tiles of 32.
 template <bool SEL>
-__device__ __forceinline__ void range_of(const KvAttendArgs& a, const Sequence& s, int64_t pos0, int64_t pos1, int64_t& lo, int64_t& hi) {
-    hi = SEL ? (int64_t)a.n_select : max((int64_t)0, min(pos1 + 1, s.len));
-    lo = SEL || a.window == 0 ? 0 : max((int64_t)0, pos0 - a.window + 1);
+__device__ __forceinline__ void range_of(const KvAttendArgs& a, const Sequence& s, int32_t pos0, int32_t pos1, int32_t& lo, int32_t& hi) {
+    hi = SEL ? (int32_t)a.n_select : max(0, min(pos1, s.len - 1) + 1);
+    lo = SEL || a.window == 0 ? 0 : (int32_t)max((int64_t)0, pos0 - a.window + 1);
 }
 
 __device__ __forceinline__ float max_of_quarters(float x) {  // over the lanes m, m + 16, m + 32, m + 48
@@ -125,31 +130,31 @@ __device__ __forceinline__ float max_of_quarters(float x) {  // over the lanes m
     return __builtin_fmaxf(float_of(r[0]), float_of(r[1]));
 }
 
-// One tile of 32 tokens as a lane holds it: of its two score rows 8 * DS code bytes each, of its 8 tokens 2 * DS each.
+// The bytes of a key that a lane holds for matrix step j (8 of them) start at this place of the row: pairs of steps lie side by
+// side, so that four lanes read 64 contiguous bytes at once.
 template <int DS>
-struct Tile {
-    static constexpr int VW = DS / 4 * 2 + (DS >> 1 & 1) + (DS & 1);
-    u32x2 k[2][DS];
-    uint32_t v[8][VW];
-    float ks[8], vs[8];  // one value (in [0]) unless tokens are selected
-    uint32_t have;       // bit t: token t of the lane's 8 is there (all ones where every token of the tile is)
-    bool full;           // every row sees every token of the tile
-};
+__device__ __forceinline__ constexpr int key_byte(int q4, int j) {
+    return j == DS - 1 && (DS & 1) ? (DS - 1) * 32 + q4 * 8 : (j >> 1) * 64 + q4 * 16 + (j & 1) * 8;
+}
 
 template <int T, int DS, bool SEL>
-__global__ __launch_bounds__(256) void kv_attend(KvAttendArgs a, Plan plan) {
+__global__ __launch_bounds__(256, T == kF32 ? (DS <= 2 ? 3 : DS <= 5 ? 2 : 1) : DS <= 2 ? 4 : DS <= 4 ? 3 : 2) void kv_attend(KvAttendArgs a, Plan plan) {
     constexpr bool HALF = T == kF16;
     constexpr int NQ = T == kF32 ? 3 : 1, NP = Parts<T>::value, D = DS * 32, ND = DS * 2, LDO = Shape<T, DS>::LDO;
+    constexpr int VW = DS / 4 * 2 + (DS >> 1 & 1) + (DS & 1);  // words of a value that a lane holds
     extern __shared__ float smem[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int m = lane & 15, q4 = lane >> 4;
     const uint32_t b = blockIdx.z, head = blockIdx.y, H = a.mem.heads, P = a.mem.page_tokens, G = a.q_heads / H;
-    const uint32_t split = blockIdx.x % plan.splits;
+    // Blocks go to the eight dies in turn, so with four or eight ranges a die would get one and the same range of every sequence,
+    // the last one of which only the long sequences have: the ranges rotate from head to head (64 sequences of 1 000 to
+    // 8 192 tokens: 147 us without, 125 with).
+    const uint32_t split = (blockIdx.x + blockIdx.y + blockIdx.z * gridDim.y) % plan.splits;
     Sequence s;
     if (!sequence_of(a, b, s)) return;
     const UniformI32 table = (UniformI32)(a.batch.table + (uint64_t)b * a.batch.table_width);
     const int64_t* select = SEL ? a.select + ((uint64_t)b * H + head) * a.n_select : nullptr;
-    const int64_t rows = s.n_new * G;
+    const int64_t rows = (int64_t)s.n_new * G;
     const uint8_t* kc = (const uint8_t*)a.mem.k;
     const uint8_t* vc = (const uint8_t*)a.mem.v;
     const float to_log2 = a.scale * kLog2e;
@@ -157,42 +162,114 @@ __global__ __launch_bounds__(256) void kv_attend(KvAttendArgs a, Plan plan) {
     for (int64_t rt = blockIdx.x / plan.splits; rt * 16 < rows; rt += plan.tiles) {
         const int64_t row0 = rt * 16, row1 = min(row0 + 15, rows - 1);
         // positions of the tile's first and last row; tokens [lo, hi) are seen by some row, [lo_all, hi_all) by every row
-        const int64_t pos0 = s.start + row0 / G, pos1 = s.start + row1 / G;
-        int64_t lo, hi;
+        const int32_t pos0 = s.start + (int32_t)(row0 / G), pos1 = s.start + (int32_t)(row1 / G);
+        int32_t lo, hi;
         range_of<SEL>(a, s, pos0, pos1, lo, hi);
         const bool same = SEL || pos0 == pos1;
-        const int64_t lo_all = a.window == 0 ? 0 : max((int64_t)0, pos1 - a.window + 1), hi_all = SEL ? hi : min(pos0 + 1, hi);
-        int64_t kb0 = lo & ~31ll, kb1 = hi;
+        const int32_t lo_all = a.window == 0 ? 0 : (int32_t)max((int64_t)0, pos1 - a.window + 1), hi_all = SEL ? hi : min(max(pos0, -1) + 1, hi);
+        int32_t kb0 = lo & ~31, kb1 = hi;
         bool whole = true;  // this block sees all of the tile's tokens
         if (plan.splits > 1) {
             if (rt < plan.tiles) {
-                whole = kb1 - kb0 <= (int64_t)plan.chunk;
-                kb0 += (int64_t)split * plan.chunk;
-                kb1 = min(kb1, kb0 + (int64_t)plan.chunk);
-                if (split && kb0 >= kb1) continue;
+                whole = kb1 - kb0 <= (int32_t)plan.chunk;
+                const int64_t at = kb0 + (int64_t)split * plan.chunk;
+                if (split && at >= kb1) continue;
+                kb0 = (int32_t)at;
+                kb1 = (int32_t)min((int64_t)kb1, at + plan.chunk);
             } else if (split) {
                 continue;
             }
         }
         const int64_t r = row0 + m;
         const bool live = r < rows;
-        const int64_t tok = live ? r / G : 0;
-        const uint32_t qh = head * G + (live ? (uint32_t)(r - tok * G) : 0);
-        const int64_t pos = live ? s.start + tok : -1;
+        const int32_t tok = live ? (int32_t)(r / G) : 0;
+        const uint32_t qh = head * G + (live ? (uint32_t)(r - (int64_t)tok * G) : 0);
+        const int32_t pos = live ? s.start + tok : -1;
+
+        // ---- where tokens lie
+        // Not selected: a tile of 32 lies in one page or two, whose numbers are the same for the whole wave.  Pages that are
+        // not there count as page 0 for the loads, and their tokens are masked.
+        auto page_of = [&](int32_t t) -> int32_t {  // -1: none
+            int32_t page = t < s.len ? table[t >> a.mem.page_shift] : -1;
+            return (uint32_t)page < (uint32_t)a.mem.pages ? page : -1;
+        };
+        // Selected: lane l (and l + 32) looks place kb + (l & 31) of the list up, in three steps one tile apart, so that none
+        // of the loads is waited for: token number, page number, then row and scales into the wave's table (two, in turn).
+        int64_t* rows_s = (int64_t*)smem + wave * 128;       // [2][32] row numbers, -1: none
+        float* scales_s = (float*)smem + wave * 256 + 128;   // [2][64] key scales, value scales
+        auto listed = [&](int32_t kb) -> int64_t {
+            const int32_t i = kb + (lane & 31);
+            return i < kb1 ? select[i] : -1;
+        };
+        auto paged = [&](int64_t t) -> int32_t { return t >= 0 && t < s.len ? a.batch.table[(uint64_t)b * a.batch.table_width + (t >> a.mem.page_shift)] : -1; };
+        auto placed = [&](int64_t t, int32_t page, int slot) {
+            const bool there = (uint32_t)page < (uint32_t)a.mem.pages;
+            const int64_t ph = (int64_t)page * H + head;
+            if (lane < 32) rows_s[slot * 32 + lane] = there ? (ph << a.mem.page_shift) + (t & (P - 1)) : -1;
+            scales_s[slot * 64 + lane] = there ? (lane < 32 ? a.mem.k_scale : a.mem.v_scale)[ph] : 0.0f;
+        };
+
+        u32x2 kw[2][DS];
+        uint32_t vw[8][VW];
+        auto load_keys = [&](int32_t kb, int32_t p0, int32_t p1, int slot) {
+            int64_t row[2];
+            if constexpr (SEL) {
+                row[0] = max(rows_s[slot * 32 + (m >> 2) * 8 + (m & 3)], (int64_t)0);
+                row[1] = max(rows_s[slot * 32 + (m >> 2) * 8 + 4 + (m & 3)], (int64_t)0);
+            } else {
+                const int64_t r0 = (((int64_t)max(p0, 0) * H + head) << a.mem.page_shift) + (kb & (P - 1));
+                const int64_t r1 = (((int64_t)max(p1, 0) * H + head) << a.mem.page_shift) + ((kb + 16) & (P - 1)) - 16;
+                row[0] = (m < 8 ? r0 : r1) + (m >> 2) * 8 + (m & 3);
+                row[1] = row[0] + 4;
+            }
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                const uint8_t* p = kc + row[t] * D + (DS > 1 ? q4 * 16 : 0);
+#pragma unroll
+                for (int j = 0; j + 1 < DS; j += 2) {
+                    const u32x4 w = *(const u32x4*)(p + j * 32);
+                    kw[t][j] = u32x2{w[0], w[1]};
+                    kw[t][j + 1] = u32x2{w[2], w[3]};
+                }
+                if constexpr (DS & 1) kw[t][DS - 1] = *(const u32x2*)(kc + row[t] * D + key_byte<DS>(q4, DS - 1));
+            }
+        };
+        auto load_values = [&](int32_t kb, int32_t p0, int32_t p1, int slot) {
+            int64_t first = 0;
+            if constexpr (!SEL) {
+                const int64_t r0 = (((int64_t)max(p0, 0) * H + head) << a.mem.page_shift) + (kb & (P - 1));
+                const int64_t r1 = (((int64_t)max(p1, 0) * H + head) << a.mem.page_shift) + ((kb + 16) & (P - 1)) - 16;
+                first = (q4 < 2 ? r0 : r1) + q4 * 8;
+            }
+#pragma unroll
+            for (int t = 0; t < 8; ++t) {
+                const uint8_t* p = vc + (SEL ? max(rows_s[slot * 32 + q4 * 8 + t], (int64_t)0) : first + t) * D;
+#pragma unroll
+                for (int c = 0; c < DS / 4; ++c) {
+                    const u32x2 y = *(const u32x2*)(p + c * 128 + m * 8);
+                    vw[t][2 * c] = y[0];
+                    vw[t][2 * c + 1] = y[1];
+                }
+                if constexpr (DS & 2) vw[t][DS / 4 * 2] = *(const uint32_t*)(p + DS / 4 * 128 + m * 4);
+                if constexpr (DS & 1) vw[t][VW - 1] = *(const uint16_t*)(p + DS / 2 * 64 + m * 2);
+            }
+        };
+
         u32x4 qf[NQ][DS];
         {
-            const E<T>* q = (const E<T>*)a.q + (uint64_t)(s.first + tok) * a.q_token + (uint64_t)qh * a.q_head + q4 * 8 * DS;
+            const E<T>* q = (const E<T>*)a.q + (uint64_t)(s.first + tok) * a.q_token + (uint64_t)qh * a.q_head;
 #pragma unroll
             for (int j = 0; j < DS; ++j) {
+                const E<T>* qj = q + key_byte<DS>(q4, j);
                 if constexpr (T == kF32) {
-                    const f32x4 x = live ? *(const f32x4*)(q + j * 8) : f32x4{0, 0, 0, 0};
-                    const f32x4 y = live ? *(const f32x4*)(q + j * 8 + 4) : f32x4{0, 0, 0, 0};
+                    const f32x4 x = live ? *(const f32x4*)qj : f32x4{0, 0, 0, 0};
+                    const f32x4 y = live ? *(const f32x4*)(qj + 4) : f32x4{0, 0, 0, 0};
 #pragma unroll
                     for (int n = 0; n < NQ; ++n)
                         qf[n][j] = u32x4{pack_hi16(bf16_part(x[0], n), bf16_part(x[1], n)), pack_hi16(bf16_part(x[2], n), bf16_part(x[3], n)),
                                          pack_hi16(bf16_part(y[0], n), bf16_part(y[1], n)), pack_hi16(bf16_part(y[2], n), bf16_part(y[3], n))};
                 } else {
-                    qf[0][j] = live ? *(const u32x4*)(q + j * 8) : u32x4{0, 0, 0, 0};
+                    qf[0][j] = live ? *(const u32x4*)qj : u32x4{0, 0, 0, 0};
                 }
             }
         }
@@ -202,121 +279,87 @@ __global__ __launch_bounds__(256) void kv_attend(KvAttendArgs a, Plan plan) {
         for (int d = 0; d < ND; ++d) o[d] = f32x4{0, 0, 0, 0};
         float top = kNone, sum = 0.0f;
 
-        // Fetches the tile at kb.  Tokens that are not there are never read from: their addresses are those of a page that is.
-        // Returns false (on all lanes) if no token of the tile is.
-        auto fetch = [&](int64_t kb, Tile<DS>& x) -> bool {
-            int64_t krow[2], vrow[8];
-            if constexpr (!SEL) {
-                int64_t page[2];
+        int32_t kb = kb0 + wave * 32;
+        int32_t p0 = -1, p1 = -1, n0 = -1, n1 = -1;  // pages of this tile and of the next
+        int64_t t1 = -1, t2 = -1;                    // selected: tokens of the next tile and of the one after it
+        int32_t g1 = -1;                             // page of the next tile's token
+        int slot = 0;
+        if (kb < kb1) {
+            if constexpr (SEL) {
+                const int64_t t0 = listed(kb);
+                t1 = listed(kb + 128);
+                t2 = listed(kb + 256);
+                const int32_t g0 = paged(t0);
+                g1 = paged(t1);
+                placed(t0, g0, 0);
+                __builtin_amdgcn_wave_barrier();
+            } else {
+                p0 = page_of(kb), p1 = page_of(kb + 16);
+                n0 = page_of(kb + 128), n1 = page_of(kb + 144);
+            }
+            load_keys(kb, p0, p1, 0);
+        }
+        for (; kb < kb1; kb += 128) {
+            const bool more = kb + 128 < kb1;
+            load_values(kb, p0, p1, slot);
+            float ks[SEL ? 8 : 1], vs[SEL ? 8 : 1];
+            uint32_t have = 0;  // bit t: token t of the lane's 8 is there, and in the range that some row sees
+            bool full;          // every row sees every token of the tile
+            if constexpr (SEL) {
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const int64_t t = kb + 16 * h;
-                    page[h] = t < s.len ? (int64_t)table[t >> a.mem.page_shift] : -1;
-                    if (page[h] >= (int64_t)a.mem.pages) page[h] = -1;
+                for (int t = 0; t < 8; ++t) {
+                    have |= (rows_s[slot * 32 + q4 * 8 + t] >= 0 ? 1u : 0u) << t;
+                    ks[t] = scales_s[slot * 64 + q4 * 8 + t];
+                    vs[t] = scales_s[slot * 64 + 32 + q4 * 8 + t];
                 }
-                if (page[0] < 0 && page[1] < 0) return false;
-                x.full = kb >= lo_all && kb + 32 <= hi_all && page[0] >= 0 && page[1] >= 0;
-                const int64_t p0 = (page[0] < 0 ? page[1] : page[0]) * H + head, p1 = (page[1] < 0 ? page[0] : page[1]) * H + head;
-                const float ks0 = ((UniformF32)a.mem.k_scale)[p0], ks1 = ((UniformF32)a.mem.k_scale)[p1];
-                const float vs0 = ((UniformF32)a.mem.v_scale)[p0], vs1 = ((UniformF32)a.mem.v_scale)[p1];
-                x.ks[0] = q4 < 2 ? ks0 : ks1;
-                x.vs[0] = q4 < 2 ? vs0 : vs1;
-                const int64_t r0 = (p0 << a.mem.page_shift) + (kb & (P - 1)), r1 = (p1 << a.mem.page_shift) + ((kb + 16) & (P - 1)) - 16;
-                krow[0] = (m < 8 ? r0 : r1) + (m >> 2) * 8 + (m & 3);
-                krow[1] = krow[0] + 4;
-                vrow[0] = (q4 < 2 ? r0 : r1) + q4 * 8;
-#pragma unroll
-                for (int t = 1; t < 8; ++t) vrow[t] = vrow[0] + t;
-                x.have = ~0u;
-                if (!x.full) {
-                    x.have = 0;
+                full = __all(have == 255);
+                if (more) {
+                    placed(t1, g1, slot ^ 1);
+                    g1 = paged(t2);
+                    t1 = t2;
+                    t2 = listed(kb + 384);
+                }
+                __builtin_amdgcn_wave_barrier();
+            } else {
+                const int64_t x0 = (int64_t)max(p0, 0) * H + head, x1 = (int64_t)max(p1, 0) * H + head;
+                const float ks0 = ((UniformF32)a.mem.k_scale)[x0], ks1 = ((UniformF32)a.mem.k_scale)[x1];
+                const float vs0 = ((UniformF32)a.mem.v_scale)[x0], vs1 = ((UniformF32)a.mem.v_scale)[x1];
+                ks[0] = q4 < 2 ? ks0 : ks1;
+                vs[0] = q4 < 2 ? vs0 : vs1;
+                full = kb >= lo_all && kb + 32 <= hi_all && p0 >= 0 && p1 >= 0;
+                if (!full) {
 #pragma unroll
                     for (int t = 0; t < 8; ++t) {
-                        const int64_t i = kb + q4 * 8 + t;
-                        x.have |= (i >= lo && i < hi && page[q4 >> 1] >= 0 ? 1u : 0u) << t;
+                        const int32_t i = kb + q4 * 8 + t;
+                        have |= (i >= lo && i < hi && (q4 < 2 ? p0 : p1) >= 0 ? 1u : 0u) << t;
                     }
                 }
-            } else {
-                // lanes 0-31 look the 32 places of the list up (and the keys' scales), lanes 32-63 likewise with the values' scales
-                int64_t* row_s = (int64_t*)(smem) + wave * 64;  // [32] row numbers, then [64] scales
-                float* scale_s = (float*)(row_s + 32);
-                const int64_t i = kb + (lane & 31);
-                const int64_t t = i < hi ? select[i] : -1;
-                int64_t page = -1;
-                if (t >= 0 && t < s.len) page = a.batch.table[(uint64_t)b * a.batch.table_width + (t >> a.mem.page_shift)];
-                const bool there = page >= 0 && page < (int64_t)a.mem.pages;
-                const uint64_t any = __ballot(there);
-                if (!any) return false;
-                const int64_t ph = page * H + head;
-                const float sc = there ? (lane < 32 ? a.mem.k_scale : a.mem.v_scale)[ph] : 0.0f;
-                int64_t row = there ? (ph << a.mem.page_shift) + (t & (P - 1)) : -1;
-                if (lane < 32) row_s[lane] = row;
-                scale_s[lane] = sc;
-                __builtin_amdgcn_wave_barrier();
-                krow[0] = row_s[(m >> 2) * 8 + (m & 3)];
-                krow[1] = row_s[(m >> 2) * 8 + 4 + (m & 3)];
-                x.have = 0;
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    vrow[e] = row_s[q4 * 8 + e];
-                    x.have |= (vrow[e] >= 0 ? 1u : 0u) << e;
-                    x.ks[e] = scale_s[q4 * 8 + e];
-                    x.vs[e] = scale_s[32 + q4 * 8 + e];
-                }
-                __builtin_amdgcn_wave_barrier();
-                x.full = (uint32_t)any == ~0u;
-                if (!x.full) {  // row 0 of the memory exists, as some row does
-                    krow[0] = max(krow[0], (int64_t)0);
-                    krow[1] = max(krow[1], (int64_t)0);
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) vrow[e] = max(vrow[e], (int64_t)0);
-                }
             }
-#pragma unroll
-            for (int t = 0; t < 2; ++t) {
-                const uint8_t* p = kc + krow[t] * D + q4 * 8 * DS;
-#pragma unroll
-                for (int j = 0; j < DS; ++j) x.k[t][j] = *(const u32x2*)(p + j * 8);
-            }
-#pragma unroll
-            for (int t = 0; t < 8; ++t) {
-                const uint8_t* p = vc + vrow[t] * D;
-#pragma unroll
-                for (int c = 0; c < DS / 4; ++c) {
-                    const u32x2 y = *(const u32x2*)(p + c * 128 + m * 8);
-                    x.v[t][2 * c] = y[0];
-                    x.v[t][2 * c + 1] = y[1];
-                }
-                if constexpr (DS & 2) x.v[t][DS / 4 * 2] = *(const uint32_t*)(p + DS / 4 * 128 + m * 4);
-                if constexpr (DS & 1) x.v[t][Tile<DS>::VW - 1] = *(const uint16_t*)(p + DS / 2 * 64 + m * 2);
-            }
-            return true;
-        };
-
-        auto work = [&](int64_t kb, Tile<DS>& x) {
             f32x4 sc[2];
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
                 sc[t] = f32x4{0, 0, 0, 0};
 #pragma unroll
                 for (int j = 0; j < DS; ++j) {
-                    const u32x4 kf = widen<HALF>(x.k[t][j][0], x.k[t][j][1]);
+                    const u32x4 kf = widen<HALF>(kw[t][j][0], kw[t][j][1]);
 #pragma unroll
                     for (int n = 0; n < NQ; ++n) sc[t] = mfma<HALF>(kf, qf[n][j], sc[t]);
                 }
             }
+            // the keys of the next tile travel while the values of this one are worked on
+            if (more) load_keys(kb + 128, n0, n1, slot ^ 1);
             // ---- softmax over what the lane's row sees of its 8 tokens
             float p[8];
 #pragma unroll
-            for (int t = 0; t < 8; ++t) p[t] = sc[t >> 2][t & 3] * (x.ks[SEL ? t : 0] * to_log2);
+            for (int t = 0; t < 8; ++t) p[t] = sc[t >> 2][t & 3] * (ks[SEL ? t : 0] * to_log2);
             uint32_t seen = 255;
-            if (!x.full) {
-                seen = live ? x.have : 0;
+            if (!full) {
+                seen = live ? have : 0;
                 if constexpr (!SEL) {
 #pragma unroll
                     for (int t = 0; t < 8; ++t) {
-                        const int64_t i = kb + q4 * 8 + t;
-                        if (!(i <= pos && (a.window == 0 || i > pos - a.window))) seen &= ~(1u << t);
+                        const int32_t i = kb + q4 * 8 + t;
+                        if (!(i <= pos && (a.window == 0 || i > (int64_t)pos - a.window))) seen &= ~(1u << t);
                     }
                 }
 #pragma unroll
@@ -325,7 +368,7 @@ __global__ __launch_bounds__(256) void kv_attend(KvAttendArgs a, Plan plan) {
 #pragma unroll
                 for (int t = 0; t < 8; ++t)
 #pragma unroll
-                    for (int w = 0; w < Tile<DS>::VW; ++w) x.v[t][w] = x.have >> t & 1 ? x.v[t][w] : 0;
+                    for (int w = 0; w < VW; ++w) vw[t][w] = have >> t & 1 ? vw[t][w] : 0;
             }
             float now = __builtin_fmaxf(__builtin_fmaxf(__builtin_fmaxf(p[0], p[1]), __builtin_fmaxf(p[2], p[3])),
                                         __builtin_fmaxf(__builtin_fmaxf(p[4], p[5]), __builtin_fmaxf(p[6], p[7])));
@@ -342,9 +385,9 @@ __global__ __launch_bounds__(256) void kv_attend(KvAttendArgs a, Plan plan) {
             for (int t = 0; t < 8; ++t) {
                 p[t] = __builtin_amdgcn_exp2f(p[t] - top);
                 sum += p[t];
-                p[t] *= x.vs[SEL ? t : 0];
+                p[t] *= vs[SEL ? t : 0];
             }
-            if (!x.full) {  // (a scale that belongs to no token may hold anything)
+            if (!full) {  // (a scale that belongs to no token may hold anything)
 #pragma unroll
                 for (int t = 0; t < 8; ++t) p[t] = seen >> t & 1 ? p[t] : 0.0f;
             }
@@ -363,12 +406,12 @@ __global__ __launch_bounds__(256) void kv_attend(KvAttendArgs a, Plan plan) {
             }
             // a NaN among values that some rows of the tile do not see must not reach those (0 * NaN)
             bool mixed = false;
-            if (!SEL && !x.full && !same) {
+            if (!SEL && !full && !same) {
                 uint32_t odd = 0;
 #pragma unroll
                 for (int t = 0; t < 8; ++t)
 #pragma unroll
-                    for (int w = 0; w < Tile<DS>::VW; ++w) odd |= nan_bytes(x.v[t][w]);
+                    for (int w = 0; w < VW; ++w) odd |= nan_bytes(vw[t][w]);
                 mixed = __any(odd != 0);
             }
             // ---- values: chunks of w dimensions a lane
@@ -380,7 +423,7 @@ __global__ __launch_bounds__(256) void kv_attend(KvAttendArgs a, Plan plan) {
                 for (int hf = 0; hf < 2; ++hf) {
 #pragma unroll
                     for (int g = 0; g < (w + 3) / 4; ++g) {
-                        const uint32_t in[4] = {x.v[hf * 4][word + g], x.v[hf * 4 + 1][word + g], x.v[hf * 4 + 2][word + g], x.v[hf * 4 + 3][word + g]};
+                        const uint32_t in[4] = {vw[hf * 4][word + g], vw[hf * 4 + 1][word + g], vw[hf * 4 + 2][word + g], vw[hf * 4 + 3][word + g]};
                         uint32_t out[4];
                         transpose4(in, out);
 #pragma unroll
@@ -409,17 +452,9 @@ __global__ __launch_bounds__(256) void kv_attend(KvAttendArgs a, Plan plan) {
                     for (int n = 0; n < NP; ++n) o[d] = mfma<false>(vf, pf[n], o[d]);
                 }
             }
-        };
-
-        // the next tile is on its way while one is worked on
-        Tile<DS> ta, tb;
-        int64_t kb = kb0 + wave * 32;
-        bool fa = kb < kb1 && fetch(kb, ta), fb;
-        for (; kb < kb1; kb += 256) {
-            fb = kb + 128 < kb1 && fetch(kb + 128, tb);
-            if (fa) work(kb, ta);
-            fa = kb + 256 < kb1 && fetch(kb + 256, ta);
-            if (fb) work(kb + 128, tb);
+            p0 = n0, p1 = n1;
+            if constexpr (!SEL) n0 = page_of(kb + 256), n1 = page_of(kb + 272);
+            slot ^= 1;
         }
 
         // ---- join the four waves: each row's maximum, then sums and outputs in wave order
@@ -478,46 +513,55 @@ __global__ __launch_bounds__(256) void kv_attend(KvAttendArgs a, Plan plan) {
     }
 }
 
-// Adds up the ranges of one row: block (row, head, sequence).
-template <int T, bool SEL>
-__global__ __launch_bounds__(256) void kv_join(KvAttendArgs a, Plan plan) {
-    __shared__ float red[256 * 4];
-    __shared__ float mx[4], sums[32];
+// Adds up the ranges of one row: block (row, head, sequence).  Every thread has four of its loads in flight.
+template <int T, bool SEL, int kJoinThreads>
+__global__ __launch_bounds__(kJoinThreads) void kv_join(KvAttendArgs a, Plan plan) {
+    __shared__ float red[kJoinThreads * 4], mx[kJoinThreads / 64], sums[64];
     const uint32_t b = blockIdx.z, head = blockIdx.y, H = a.mem.heads, G = a.q_heads / H, D = a.mem.dim;
     Sequence s;
     if (!sequence_of(a, b, s)) return;
-    const int64_t row = blockIdx.x, rows = s.n_new * G, rt = row / 16;
+    const int64_t row = blockIdx.x, rows = (int64_t)s.n_new * G, rt = row / 16;
     if (row >= rows) return;
-    int64_t lo, hi;
-    range_of<SEL>(a, s, s.start + rt * 16 / G, s.start + min(rt * 16 + 15, rows - 1) / G, lo, hi);
-    const int64_t used64 = (hi - (lo & ~31ll) + plan.chunk - 1) / plan.chunk;
-    if (used64 <= 1) return;  // written by kv_attend
-    const uint32_t used = (uint32_t)min(used64, (int64_t)plan.splits);
+    int32_t lo, hi;
+    range_of<SEL>(a, s, s.start + (int32_t)(rt * 16 / G), s.start + (int32_t)(min(rt * 16 + 15, rows - 1) / G), lo, hi);
+    lo &= ~31;
+    if (hi - lo <= (int32_t)plan.chunk) return;  // written by kv_attend
+    const uint32_t used = min(((uint32_t)(hi - lo) + plan.chunk - 1) / plan.chunk, plan.splits);
     const uint64_t step = 16 * (D + 2);
     const float* part = plan.part + ((((uint64_t)b * H + head) * plan.tiles + rt) * plan.splits * 16 + row % 16) * (D + 2);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     float best = kNone;
-    for (uint32_t i = threadIdx.x; i < used; i += 256) best = __builtin_fmaxf(best, part[i * step + D]);
+    for (uint32_t i = threadIdx.x; i < used; i += kJoinThreads) best = __builtin_fmaxf(best, part[i * step + D]);
 #pragma unroll
     for (int o = 32; o; o >>= 1) best = __builtin_fmaxf(best, __shfl_xor(best, o));
     if (lane == 0) mx[wave] = best;
     __syncthreads();
-    best = __builtin_fmaxf(__builtin_fmaxf(mx[0], mx[1]), __builtin_fmaxf(mx[2], mx[3]));
+#pragma unroll
+    for (int w = 0; w < kJoinThreads / 64; ++w) best = __builtin_fmaxf(best, mx[w]);
     // groups of D / 4 threads, each thread four dimensions of every groups-th range
-    const uint32_t width = D / 4, groups = 256 / width, g = threadIdx.x / width, d = threadIdx.x % width * 4;
+    const uint32_t width = D / 4, groups = kJoinThreads / width, g = threadIdx.x / width, d = threadIdx.x % width * 4;
     f32x4 acc = {0, 0, 0, 0};
     float total = 0.0f;
     if (g < groups) {
-        for (uint32_t i = g; i < used; i += groups) {
-            const float* w = part + i * step;
-            const f32x2 x = *(const f32x2*)(w + d), y = *(const f32x2*)(w + d + 2), z = *(const f32x2*)(w + D);
-            const float f = __builtin_amdgcn_exp2f(z[0] - best);
-            total += f * z[1];
-            acc += f32x4{x[0], x[1], y[0], y[1]} * f;
+        for (uint32_t i = g; i < used; i += 4 * groups) {
+            f32x2 x[4], y[4], z[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const float* w = part + (uint64_t)min(i + u * groups, used - 1) * step;
+                x[u] = *(const f32x2*)(w + d), y[u] = *(const f32x2*)(w + d + 2), z[u] = *(const f32x2*)(w + D);
+            }
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                if (i + u * groups < used) {
+                    const float f = __builtin_amdgcn_exp2f(z[u][0] - best);
+                    total += f * z[u][1];
+                    acc += f32x4{x[u][0], x[u][1], y[u][0], y[u][1]} * f;
+                }
+            }
         }
+        if (d == 0) sums[g] = total;
     }
     *(f32x4*)(red + threadIdx.x * 4) = acc;
-    if (g < groups && d == 0) sums[g] = total;
     __syncthreads();
     if (threadIdx.x < width) {
         float sum = 0.0f;
@@ -545,11 +589,18 @@ hipError_t launch_one(const KvAttendArgs& a, const Plan& plan, hipStream_t strea
     return hipGetLastError();
 }
 
+template <int T, bool SEL>
+void launch_join_of(const KvAttendArgs& a, const Plan& plan, const dim3& grid, hipStream_t stream) {
+    // 512 threads a row where there are many ranges (384: 10 us against 17), 256 where there are few (6: 6.3 us against 9.5)
+    if (plan.splits > 64) hipLaunchKernelGGL((kv_join<T, SEL, 512>), grid, dim3(512), 0, stream, a, plan);
+    else hipLaunchKernelGGL((kv_join<T, SEL, 256>), grid, dim3(256), 0, stream, a, plan);
+}
+
 template <int T>
 hipError_t launch_join(const KvAttendArgs& a, const Plan& plan, uint32_t rows, hipStream_t stream) {
     const dim3 grid(std::min(rows, plan.tiles * 16), a.mem.heads, a.batch.count);
-    if (a.select) hipLaunchKernelGGL((kv_join<T, true>), grid, dim3(256), 0, stream, a, plan);
-    else hipLaunchKernelGGL((kv_join<T, false>), grid, dim3(256), 0, stream, a, plan);
+    if (a.select) launch_join_of<T, true>(a, plan, grid, stream);
+    else launch_join_of<T, false>(a, plan, grid, stream);
     return hipGetLastError();
 }
 
@@ -561,9 +612,13 @@ Plan plan_of(const KvAttendArgs& a, uint32_t max_new) {
     uint64_t tokens = a.select ? a.n_select : (uint64_t)a.batch.table_width << a.mem.page_shift;
     if (!a.select && a.window) tokens = std::min<uint64_t>(tokens, (uint64_t)a.window + max_new + 31);
     const uint64_t blocks = (uint64_t)p.tiles * a.mem.heads * a.batch.count;
-    // as many ranges as give some 4096 blocks, none shorter than 512 tokens
-    const uint64_t want = std::max<uint64_t>(1, 4096 / blocks);
-    uint64_t chunk = std::max<uint64_t>(512, (tokens + want - 1) / want);
+    // As many ranges as give some 3072 blocks, four times what the chip holds at once: sequences of different lengths even out
+    // (64 of 1 000 to 8 192 tokens, 8 heads: 147 us at 1024 blocks, 130 at 1536, 121 at 3072, 125 at 4096).  But no range
+    // shorter than 512 tokens (selected ones: 1024), where a block's start and end begin to count (500 tokens in one block 9.4 us,
+    // in four 6.0 and 4.4 for the join; 2048 selected ones in two ranges 40 us, in four 46), and at most 384 of one row, or the
+    // join counts (two sequences of 500 003: 384 ranges 103 + 10 us, 768 104 + 17, 256 109 + 8).
+    const uint64_t want = std::min<uint64_t>(384, std::max<uint64_t>(1, 3072 / blocks));
+    uint64_t chunk = std::max<uint64_t>(a.select ? 1024 : 512, (tokens + want - 1) / want);
     chunk = (chunk + 127) / 128 * 128;
     p.chunk = (uint32_t)std::min<uint64_t>(chunk, 1u << 30);
     p.splits = (uint32_t)((tokens + p.chunk - 1) / p.chunk);

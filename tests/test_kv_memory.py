@@ -81,29 +81,33 @@ def attend_ref(q, k, v, ks, vs, table, lengths, offsets, page, scale, window=0, 
     mass, size, count = torch.zeros(T, hq, D, dtype=torch.float64), torch.zeros(T, hq, dtype=torch.float64), 1
     for b, n_held in enumerate(lengths):
         lo, hi = offsets[b], offsets[b + 1]
-        if hi <= lo or lo < 0 or hi > T:
+        if hi <= lo or lo < 0 or hi > T or n_held == 0:
             continue
-        for t in range(lo, hi):
-            pos = n_held - (hi - t)
-            for h in range(H):
-                if select is not None:
-                    at = [int(i) for i in select[b, h] if 0 <= int(i) < n_held]
-                else:
-                    at = range(max(0, pos - window + 1) if window else 0, pos + 1)
-                at = torch.tensor([i for i in at if i // page < table.shape[1] and 0 <= int(table[b, i // page]) < pages], dtype=torch.long)
-                if not len(at):
-                    continue
-                pid = table[b].long()[at // page]
-                kk = k.view(torch.uint8)[pid, h, at % page].view(E4M3).double() * ks[pid, h].double()[:, None]
-                vv = v.view(torch.uint8)[pid, h, at % page].view(E4M3).double() * vs[pid, h].double()[:, None]
-                qq = q[t, h * G:(h + 1) * G].double()
-                s = qq @ kk.t() * scale
-                p = torch.softmax(s, 1)
-                out[t, h * G:(h + 1) * G] = p @ vv
-                mass[t, h * G:(h + 1) * G] = p @ vv.abs()
-                lse[t, h * G:(h + 1) * G] = torch.logsumexp(s, 1)
-                size[t, h * G:(h + 1) * G] = (qq.abs() @ kk.abs().t() * abs(scale)).max(1).values
-                count = max(count, len(at))
+        pos = torch.arange(n_held - (hi - lo), n_held)
+        for h in range(H):
+            at = select[b, h] if select is not None else torch.arange(n_held)
+            at = at[(at >= 0) & (at < min(n_held, page * table.shape[1]))]
+            pid = table[b].long()[at // page]
+            at, pid = at[(pid >= 0) & (pid < pages)], pid[(pid >= 0) & (pid < pages)]
+            if not len(at):
+                continue
+            hidden = torch.zeros(hi - lo, len(at), dtype=torch.bool)
+            if select is None:
+                hidden |= at[None, :] > pos[:, None]
+                if window:
+                    hidden |= at[None, :] <= pos[:, None] - window
+            kk = k.view(torch.uint8)[pid, h, at % page].view(E4M3).double() * ks[pid, h].double()[:, None]
+            vv = v.view(torch.uint8)[pid, h, at % page].view(E4M3).double() * vs[pid, h].double()[:, None]
+            qq = q[lo:hi, h * G:(h + 1) * G].double()
+            s = (qq @ kk.t() * scale).masked_fill(hidden[:, None, :], -math.inf)  # [new, G, tokens]
+            p = torch.softmax(s, 2).masked_fill((hidden.all(1))[:, None, None], 0.0)
+            lost = ~hidden[:, None, :, None] & torch.isnan(vv)[None, None]  # a NaN that is seen; one that is not has no effect
+            o = p @ vv.nan_to_num() if not torch.isnan(vv).any() else torch.where(lost.any(2), torch.nan, p @ vv.nan_to_num())
+            out[lo:hi, h * G:(h + 1) * G] = o
+            mass[lo:hi, h * G:(h + 1) * G] = p @ vv.nan_to_num().abs()
+            lse[lo:hi, h * G:(h + 1) * G] = torch.logsumexp(s, 2)
+            size[lo:hi, h * G:(h + 1) * G] = (qq.abs() @ kk.abs().t() * abs(scale)).masked_fill(hidden[:, None, :], 0.0).amax(2)
+            count = max(count, int((~hidden).sum(1).max()))
     return out, lse, mass, size, count
 
 
@@ -627,3 +631,49 @@ def test_decoding_in_a_graph_and_on_a_stream():
             torch.cuda.synchronize()
         assert torch.equal(out, want) and torch.equal(lse, want_lse)
         assert torch.equal(a.k.view(torch.uint8), b.k.view(torch.uint8)) and torch.equal(a.v_scale, b.v_scale)
+
+
+MANY = [
+    # sequences, longest, most new, page, heads, q heads, dim, window: enough rows for the kernel that shares widened tokens
+    (16, 150, 110, 16, 8, 16, 32, 0),
+    (9, 300, 128, 64, 4, 24, 64, 0),
+    (16, 140, 60, 16, 8, 32, 96, 33),
+    (10, 260, 130, 32, 8, 16, 128, 0),
+    (10, 200, 130, 128, 8, 16, 160, 70),
+    (10, 130, 120, 16, 8, 16, 224, 0),
+    (10, 150, 100, 64, 8, 16, 256, 0),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("case", MANY, ids=lambda c: "-".join(map(str, c)))
+def test_attend_many_rows(dtype, case):
+    """Chunks of many sequences: of all lengths, some with no new token, an absent page, a table that is too short, NaN codes
+    that only later queries see, and garbage behind the last tokens."""
+    count, longest, most, page, heads, hq, dim, window = case
+    t = TYPES[dtype]
+    r = np.random.default_rng(dim)
+    held = [longest] + [int(x) for x in r.integers(1, longest, count - 1)]
+    new = [most] + [min(h, int(x)) for h, x in zip(held[1:], r.integers(0, most, count - 1))]
+    s = Setup(held, page, heads, dim, seed=dim, width=-(-longest // page) - (1 if page == 16 else 0))
+    s.table[1, 0] = -1
+    for c in (s.k.view(torch.uint8), s.v.view(torch.uint8)):
+        for b, n in enumerate(held):
+            if n % page and n // page < s.table.shape[1]:
+                c[s.table[b, n // page].long(), :, n % page:] = 0x7F
+    for b, tok in ((0, longest - 20), (0, longest // 2), (2, held[2] - 1)):
+        if tok // page < s.table.shape[1] and s.table[b, tok // page] >= 0:
+            s.v.view(torch.uint8)[s.table[b, tok // page].long(), 1, tok % page, dim - 3] = 0xFF
+            s.k.view(torch.uint8)[s.table[b, tok // page].long(), 2, tok % page, 1] = 0x7F
+    off = offsets_of(new)
+    q = s.randn(off[-1] + 2, hq, dim, dtype=t)
+    mem = s.memory()
+    table, lengths = s.on_gpu()
+    out, lse = mem.attend(q.cuda(), table, lengths, offsets=ints(off), max_new=most, window=window, return_lse=True)
+    ref = attend_ref(q, s.k, s.v, s.ks, s.vs, s.table, held, off, page, dim ** -0.5, window)
+    check_attend(out[:off[-1]], lse[:off[-1]], [x[:off[-1]] if torch.is_tensor(x) else x for x in ref], t)
+    assert not out[off[-1]:].any()
+    out = mem.attend(q.cuda(), table, lengths, offsets=ints(off), max_new=most, window=window, scale=-0.3)
+    ref = attend_ref(q, s.k, s.v, s.ks, s.vs, s.table, held, off, page, -0.3, window)
+    check_attend(out[:off[-1]], None, [x[:off[-1]] if torch.is_tensor(x) else x for x in ref], t)

@@ -94,6 +94,8 @@ struct Plan {
     uint32_t splits;
     uint32_t chunk;
     float* part;      // [sequence][head][tile][split][16][D + 2]
+    uint32_t max_new;
+    bool many;        // kv_attend_many, which needs none of the above
 };
 
 typedef const __attribute__((address_space(4))) int32_t* UniformI32;  // read through scalar registers
@@ -138,7 +140,7 @@ __device__ __forceinline__ constexpr int key_byte(int q4, int j) {
 }
 
 template <int T, int DS, bool SEL>
-__global__ __launch_bounds__(256, T == kF32 ? (DS <= 2 ? 3 : DS <= 5 ? 2 : 1) : DS <= 2 ? 4 : DS <= 4 ? 3 : 2) void kv_attend(KvAttendArgs a, Plan plan) {
+__global__ __launch_bounds__(256, T == kF32 ? (DS <= 2 ? 3 : DS <= 5 ? 2 : 1) : DS <= 2 ? 4 : DS <= 4 ? 3 : DS <= 6 ? 2 : 1) void kv_attend(KvAttendArgs a, Plan plan) {
     constexpr bool HALF = T == kF16;
     constexpr int NQ = T == kF32 ? 3 : 1, NP = Parts<T>::value, D = DS * 32, ND = DS * 2, LDO = Shape<T, DS>::LDO;
     constexpr int VW = DS / 4 * 2 + (DS >> 1 & 1) + (DS & 1);  // words of a value that a lane holds
@@ -415,6 +417,8 @@ __global__ __launch_bounds__(256, T == kF32 ? (DS <= 2 ? 3 : DS <= 5 ? 2 : 1) : 
                 mixed = __any(odd != 0);
             }
             // ---- values: chunks of w dimensions a lane
+            auto values = [&](auto is_mixed) {
+            constexpr bool MIXED = decltype(is_mixed)::value;
 #pragma unroll
             for (int c = 0; c < Chunks<DS>::count; ++c) {
                 const int w = Chunks<DS>::width(c), word = c <= DS / 4 ? 2 * c : 2 * (DS / 4) + 1;
@@ -434,7 +438,7 @@ __global__ __launch_bounds__(256, T == kF32 ? (DS <= 2 ? 3 : DS <= 5 ? 2 : 1) : 
                 for (int e = 0; e < w; ++e) {
                     const int d = Chunks<DS>::tile(c) + e;
                     uint32_t y = col[e][0], z = col[e][1];
-                    if (mixed) {
+                    if constexpr (MIXED) {
                         const uint32_t ny = nan_bytes(y) >> 7, nz = nan_bytes(z) >> 7;  // 1 in the bytes that are NaN
                         y &= ~(ny * 255u);
                         z &= ~(nz * 255u);
@@ -452,6 +456,9 @@ __global__ __launch_bounds__(256, T == kF32 ? (DS <= 2 ? 3 : DS <= 5 ? 2 : 1) : 
                     for (int n = 0; n < NP; ++n) o[d] = mfma<false>(vf, pf[n], o[d]);
                 }
             }
+            };
+            if (mixed) values(std::true_type());
+            else values(std::false_type());
             p0 = n0, p1 = n1;
             if constexpr (!SEL) n0 = page_of(kb + 256), n1 = page_of(kb + 272);
             slot ^= 1;
@@ -510,6 +517,423 @@ __global__ __launch_bounds__(256, T == kF32 ? (DS <= 2 ? 3 : DS <= 5 ? 2 : 1) : 
             }
         }
         __syncthreads();
+    }
+}
+
+// ---- many rows: chunks of prompts ---------------------------------------------------------------------
+//
+// Four waves of NT tiles of 16 rows go through the tokens together, 64 at a time.  What bounds this is, next to the matrix
+// units (256 cycles for 32 tokens x 16 rows at 128 dimensions), the softmax on the vector units (about as long: an exp2 costs
+// four instructions) and the reads of LDS; so
+//   - codes are widened to bf16 (f16) once per block, into LDS in the order in which lanes hold matrix operands; a wave uses
+//     each operand it reads for its NT row tiles;
+//   - the scale of a page's values is folded into the exponent: w = exp2(score + log2 v_scale - M) with M the running
+//     maximum of just that, and the softmax's sum takes w / v_scale; so a score costs one fma, one exp2, one add;
+//   - the loads of the tile after next are under way while one is computed and the next is being widened.
+template <int T, int DS>
+struct Many {
+    static constexpr int NT = T == kF32 || DS > 6 ? 1 : 2;
+    static constexpr int rows = 4 * NT * 16;
+    static constexpr int D = DS * 32, ND = DS * 2;
+    static constexpr int side = 64 * D * 2;                // bytes of 64 keys (or values) in bf16
+    static constexpr size_t lds = 4 * side + 64;           // two buffers of both, and of the scales of four pages each
+    static constexpr int units = (D * 2 + 255) / 256;      // (8 tokens x 4 dimensions) of values a thread widens; D * 2 units in all
+    static constexpr int pieces = (D * 4 + 255) / 256;     // 16-byte pieces of keys a thread widens; D * 4 in all
+};
+
+template <int T, int DS>
+__global__ __launch_bounds__(256, DS <= 4 ? 2 : 1) void kv_attend_many(KvAttendArgs a) {
+    typedef Many<T, DS> M;
+    constexpr bool HALF = T == kF16;
+    constexpr int NQ = T == kF32 ? 3 : 1, NP = Parts<T>::value, D = M::D, ND = M::ND, NT = M::NT, side = M::side;
+    extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int m = lane & 15, q4 = lane >> 4;
+    const uint32_t H = a.mem.heads, b = blockIdx.z, head = blockIdx.x % H, P = a.mem.page_tokens, G = a.q_heads / H;
+    Sequence s;
+    if (!sequence_of(a, b, s)) return;
+    const int32_t* table = a.batch.table + (uint64_t)b * a.batch.table_width;
+    float* scales_s = (float*)(lds + 4 * side);  // [2][8]: of keys, of values
+    const int64_t rows = (int64_t)s.n_new * G;
+    const uint8_t* kc = (const uint8_t*)a.mem.k;
+    const uint8_t* vc = (const uint8_t*)a.mem.v;
+    const float to_log2 = __builtin_fabsf(a.scale) * kLog2e;
+    const uint32_t flip = a.scale < 0.0f ? (T == kF32 ? 0x80000000u : 0x80008000u) : 0u;  // the scale's sign goes into the queries
+    // Page numbers: 64 of them in a register of the wave, refilled every 64 pages.  (Scalar loads would do, but a wait for LDS is
+    // a wait for them as well.)
+    int32_t held = -1, held_from = 0;
+    auto page_of = [&](int32_t t) -> int32_t {  // -1: none
+        return t < s.len ? __builtin_amdgcn_readlane(held, (t >> a.mem.page_shift) - held_from) : -1;
+    };
+    auto pages = [&](int32_t kb) {  // of a tile, one for every 16 tokens
+        if (kb < s.len && ((kb + 63) >> a.mem.page_shift) - held_from > 63) {
+            held_from = kb >> a.mem.page_shift;
+            const uint32_t at = held_from + lane;
+            const int32_t page = at < a.batch.table_width ? table[at] : -1;
+            held = (uint32_t)page < (uint32_t)a.mem.pages ? page : -1;
+        }
+        return i32x4{page_of(kb), page_of(kb + 16), page_of(kb + 32), page_of(kb + 48)};
+    };
+
+    // The last rows see the most tokens: they go first.  (All sequences' last rows before the others would even out better on paper,
+    // but neighbouring blocks go to other parts of the chip in turn, and four sequences then have one each: 785 us instead of 394;
+    // with the sequences rotated, 410.)
+    const int64_t nblocks = (rows + M::rows - 1) / M::rows;
+    for (int64_t rb = nblocks - 1 - blockIdx.x / H; rb >= 0; rb -= gridDim.x / H) {
+        const int64_t row0 = rb * M::rows, row1 = min(row0 + M::rows - 1, rows - 1);
+        const int32_t pos0 = s.start + (int32_t)(row0 / G), pos1 = s.start + (int32_t)(row1 / G);
+        int32_t lo, hi;
+        range_of<false>(a, s, pos0, pos1, lo, hi);
+        // this wave's rows
+        const int64_t wrow0 = row0 + wave * NT * 16, wrow1 = min(wrow0 + NT * 16 - 1, rows - 1);
+        const bool idle = wrow0 >= rows;
+        const int32_t wpos0 = s.start + (int32_t)(min(wrow0, rows - 1) / G), wpos1 = s.start + (int32_t)(wrow1 / G);
+        const int32_t w_lo = a.window == 0 ? 0 : (int32_t)max((int64_t)0, wpos0 - a.window + 1);
+        // the tokens [lo_all, hi_all) are seen by all rows of the block
+        const int32_t lo_all = a.window == 0 ? 0 : (int32_t)max((int64_t)0, pos1 - a.window + 1), hi_all = min(max(pos0, -1) + 1, hi);
+        u32x4 qf[NT][NQ][DS];
+        int32_t pos[NT];
+#pragma unroll
+        for (int ct = 0; ct < NT; ++ct) {
+            const int64_t r = wrow0 + ct * 16 + m;
+            const bool live = r < rows;
+            const int32_t tok = live ? (int32_t)(r / G) : 0;
+            const uint32_t qh = head * G + (live ? (uint32_t)(r - (int64_t)tok * G) : 0);
+            pos[ct] = live ? s.start + tok : -1;
+            const E<T>* q = (const E<T>*)a.q + (uint64_t)(s.first + tok) * a.q_token + (uint64_t)qh * a.q_head + q4 * 8;
+#pragma unroll
+            for (int j = 0; j < DS; ++j) {
+                if constexpr (T == kF32) {
+                    u32x4 x = live ? *(const u32x4*)(q + j * 32) : u32x4{0, 0, 0, 0};
+                    u32x4 y = live ? *(const u32x4*)(q + j * 32 + 4) : u32x4{0, 0, 0, 0};
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) x[i] ^= flip, y[i] ^= flip;
+#pragma unroll
+                    for (int n = 0; n < NQ; ++n)
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            qf[ct][n][j][i] = pack_hi16(bf16_part(float_of(x[2 * i]), n), bf16_part(float_of(x[2 * i + 1]), n));
+                            qf[ct][n][j][2 + i] = pack_hi16(bf16_part(float_of(y[2 * i]), n), bf16_part(float_of(y[2 * i + 1]), n));
+                        }
+                } else {
+                    qf[ct][0][j] = live ? *(const u32x4*)(q + j * 32) : u32x4{0, 0, 0, 0};
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) qf[ct][0][j][i] ^= flip;
+                }
+            }
+        }
+        f32x4 o[NT][ND];
+        float top[NT], sum[NT];
+#pragma unroll
+        for (int ct = 0; ct < NT; ++ct) {
+            top[ct] = wrow0 + ct * 16 + m < rows ? kNone : -kNone, sum[ct] = 0.0f;  // (a row that does not exist has no weights)
+#pragma unroll
+            for (int d = 0; d < ND; ++d) o[ct][d] = f32x4{0, 0, 0, 0};
+        }
+
+        // Places in LDS, in bytes, apart from multiples of 1 KB (a matrix operand) that go into the instructions.  Operand rows are
+        // exchanged by j (keys) and d (values), so that the pieces that neighbouring threads write lie in different banks.
+        uint32_t key_at[4], value_at[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            key_at[j] = (q4 * 16 + (m ^ ((j * 2 + (q4 >> 1)) & 7))) * 16;
+            value_at[j] = side + (q4 * 16 + (m ^ j)) * 16;
+        }
+        // ---- staging: a thread widens `pieces` 16-byte pieces of keys, and `units` of 8 tokens x 4 dimensions of values
+        float scale_r = 1.0f;  // of threads 0-7
+        u32x4 kr[M::pieces];
+        uint32_t vr[M::units][8];
+        const uint64_t page_bytes = (uint64_t)H * P * D;
+        const uint8_t* const kh = kc + (uint64_t)head * P * D;
+        const uint8_t* const vh = vc + (uint64_t)head * P * D;
+        auto pick = [&](i32x4 pg, int i) { return i < 2 ? (i == 0 ? pg[0] : pg[1]) : (i == 2 ? pg[2] : pg[3]); };
+        auto load = [&](int32_t kb, i32x4 pg) {
+            if (tid < 8) {
+                const int32_t page = pick(pg, tid & 3);
+                scale_r = page >= 0 ? (tid < 4 ? a.mem.k_scale : a.mem.v_scale)[(int64_t)page * H + head] : 1.0f;
+            }
+#pragma unroll
+            for (int i = 0; i < M::pieces; ++i) {
+                const int piece = tid + i * 256;
+                if (D * 4 % 256 == 0 || piece < D * 4) {
+                    const int tok = piece / (D / 16), c = piece % (D / 16);
+                    const uint32_t page = (uint32_t)max(pick(pg, tok >> 4), 0);
+                    kr[i] = *(const u32x4*)(kh + page * page_bytes + ((kb + tok) & (P - 1)) * (uint32_t)D + c * 16);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < M::units; ++i) {
+                const int unit = tid + i * 256;
+                if (D * 2 % 256 == 0 || unit < D * 2) {
+                    const int grp = unit / (D / 4), c = unit % (D / 4);
+                    const uint32_t page = (uint32_t)max(pick(pg, grp >> 1), 0);
+                    const uint8_t* p = vh + page * page_bytes + ((kb + grp * 8) & (P - 1)) * (uint32_t)D + c * 4;
+#pragma unroll
+                    for (int t = 0; t < 8; ++t) vr[i][t] = *(const uint32_t*)(p + t * D);
+                }
+            }
+        };
+        // every row of the block sees every token of the tile
+        auto plain = [&](int32_t kb, i32x4 pg) {
+            return kb >= lo_all && kb + 64 <= hi_all && (pg[0] | pg[1] | pg[2] | pg[3]) >= 0;
+        };
+        auto hide = [&](int32_t kb, i32x4 pg) {
+            if (!plain(kb, pg)) {  // what no row sees may hold anything: it is taken for zeros
+#pragma unroll
+                for (int i = 0; i < M::units; ++i) {
+                    const int grp = (tid + i * 256) / (D / 4), t0 = kb + grp * 8;
+                    const bool there = pick(pg, (grp >> 1) & 3) >= 0;
+#pragma unroll
+                    for (int t = 0; t < 8; ++t) {
+                        vr[i][t] = there && t0 + t >= lo && t0 + t < hi ? vr[i][t] : 0;
+                    }
+                }
+            }
+        };
+        auto store_keys = [&](int buf) {
+            unsigned char* ks = lds + buf * 2 * side;
+            if (tid < 8) scales_s[buf * 8 + tid] = scale_r;
+#pragma unroll
+            for (int i = 0; i < M::pieces; ++i) {
+                const int piece = tid + i * 256;
+                if (D * 4 % 256 == 0 || piece < D * 4) {
+                    // token x of 32: row (x >> 3) * 4 + (x & 3) of score tile (x >> 2) & 1.  Bytes 16 c .. + 15: quarters
+                    // 2 (c & 1), 2 (c & 1) + 1 of step c / 2.  Rows are exchanged by c, so that pieces of one token go to other banks.
+                    const int tok = piece / (D / 16), c = piece % (D / 16), x = tok & 31;
+                    const int tile = (tok >> 5) * 2 + (x >> 2 & 1), row = ((x >> 3) * 4 + (x & 3)) ^ (c & 7);
+                    unsigned char* w = ks + ((tile * DS + (c >> 1)) * 64 + (c & 1) * 32 + row) * 16;
+                    *(u32x4*)w = widen<HALF>(kr[i][0], kr[i][1]);
+                    *(u32x4*)(w + 256) = widen<HALF>(kr[i][2], kr[i][3]);
+                }
+            }
+        };
+        auto store_values = [&](int buf) {
+            unsigned char* vs = lds + buf * 2 * side + side;
+#pragma unroll
+            for (int i = 0; i < M::units; ++i) {
+                const int unit = tid + i * 256;
+                if (D * 2 % 256 == 0 || unit < D * 2) {
+                    const int grp = unit / (D / 4), c = unit % (D / 4);
+                    uint32_t x[4], y[4];
+                    transpose4(vr[i], x);
+                    transpose4(vr[i] + 4, y);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int d = c * 4 + e, dt = d >> 4;
+                        *(u32x4*)(vs + ((dt * 2 + (grp >> 2)) * 64 + (grp & 3) * 16 + ((d & 15) ^ (dt & 3))) * 16) = widen<false>(x[e], y[e]);
+                    }
+                }
+            }
+        };
+
+        const int32_t kb0 = lo & ~63;
+        i32x4 pa, pb, pc;  // pages of this tile, of the next, of the one after it
+        __syncthreads();
+        if (kb0 < hi) {
+            held_from = -64;
+            pa = pages(kb0);
+            pb = pages(kb0 + 64);
+            pc = pages(kb0 + 128);
+            load(kb0, pa);
+            hide(kb0, pa);
+            store_keys(0);
+            store_values(0);
+            if (kb0 + 64 < hi) load(kb0 + 64, pb);
+        }
+        __syncthreads();
+        int32_t kb = kb0;
+        int buf = 0;
+        // One tile.  FULL: every row of the block sees every token of it, and the running reference of the softmax stays what it
+        // is.  That need not be the maximum: no score is compared with another while the sums of the weights stay below 2^11.
+        // Where one does not (rarely: in the first tiles) the answer is false, nothing has been added up, and the tile is done
+        // again with FULL = false, which looks at every score and scales what there is.  (One loop that does both holds every
+        // output twice: 500 spilled bytes a lane and twice the time.)
+        auto compute = [&](auto is_full) -> bool {
+            constexpr bool FULL = decltype(is_full)::value;
+            const unsigned char* here = lds + buf * 2 * side;
+                float c[2], lv[2], inv[2];
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    c[h] = scales_s[buf * 8 + 2 * h + (q4 >> 1)] * to_log2;
+                    const float vs = __builtin_fmaxf(scales_s[buf * 8 + 4 + 2 * h + (q4 >> 1)], 0x1p-120f);
+                    lv[h] = __builtin_amdgcn_logf(vs), inv[h] = __builtin_amdgcn_rcpf(vs);
+                }
+                    // scores: operands are read three products ahead; the next tile is widened beside them
+                    f32x4 sc[2][NT][2];
+                    u32x4 kf[4];
+                    auto read_key = [&](int e) { kf[e & 3] = *(const u32x4*)(here + key_at[e % DS & 3] + e * 1024); };
+#pragma unroll
+                    for (int e = 0; e < 3 && e < 4 * DS; ++e) read_key(e);
+#pragma unroll
+                    for (int e = 0; e < 4 * DS; ++e) {
+                        const int i = e / DS, j = e % DS;
+                        if (e + 3 < 4 * DS) read_key(e + 3);
+                        if (e == DS) store_keys(buf ^ 1);
+                        if (e == 2 * DS) store_values(buf ^ 1);
+#pragma unroll
+                        for (int ct = 0; ct < NT; ++ct) {
+                            if (j == 0) sc[i >> 1][ct][i & 1] = f32x4{0, 0, 0, 0};
+#pragma unroll
+                            for (int n = 0; n < NQ; ++n) sc[i >> 1][ct][i & 1] = mfma<HALF>(kf[e & 3], qf[ct][n][j], sc[i >> 1][ct][i & 1]);
+                        }
+                        if (j == DS - 1) __builtin_amdgcn_sched_barrier(0);
+                    }
+                    uint32_t seen[2][NT];
+                    if constexpr (!FULL) {
+                        const int32_t lowest = a.window == 0 ? -1 : (int32_t)min(a.window, (int64_t)0x7FFFFFFF);
+#pragma unroll
+                        for (int h = 0; h < 2; ++h)
+#pragma unroll
+                            for (int ct = 0; ct < NT; ++ct) {
+                                seen[h][ct] = 0;
+                                const int32_t first = kb + h * 32 + q4 * 8, end = min(pos[ct], s.len - 1);
+                                const bool there = (q4 < 2 ? pa[2 * h] : pa[2 * h + 1]) >= 0;
+#pragma unroll
+                                for (int t = 0; t < 8; ++t) {
+                                    // (a position is at least -2^31 + 1 and a token at least 0: their difference, taken only where the token is not after the position, fits)
+                                    const bool see = there && first + t <= end && (lowest < 0 || pos[ct] - (first + t) < lowest);
+                                    seen[h][ct] |= (see ? 1u : 0u) << t;
+                                    sc[h][ct][t >> 2][t & 3] = see ? __builtin_fmaf(sc[h][ct][t >> 2][t & 3], c[h], lv[h]) : -__builtin_inff();
+                                }
+                            }
+#pragma unroll
+                        for (int ct = 0; ct < NT; ++ct) {
+                            float now = top[ct];
+#pragma unroll
+                            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                                for (int t = 0; t < 8; ++t) now = __builtin_fmaxf(now, sc[h][ct][t >> 2][t & 3]);
+                            now = max_of_quarters(now);
+                            const float shrink = __builtin_amdgcn_exp2f(top[ct] - now);
+                            top[ct] = now;
+                            sum[ct] *= shrink;
+#pragma unroll
+                            for (int d = 0; d < ND; ++d) o[ct][d] *= shrink;
+                        }
+                    }
+                    u32x4 pf[2][NT][NP];
+                    float more[NT];
+                    bool over = false;
+#pragma unroll
+                    for (int ct = 0; ct < NT; ++ct) {
+                        more[ct] = 0.0f;
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            const float off = FULL ? lv[h] - top[ct] : -top[ct];
+                            float p[8];
+#pragma unroll
+                            for (int t = 0; t < 8; ++t) {
+                                const float x = sc[h][ct][t >> 2][t & 3];
+                                p[t] = __builtin_amdgcn_exp2f(FULL ? __builtin_fmaf(x, c[h], off) : x + off);
+                            }
+                            const float part = ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
+                            over |= part > 2048.0f;
+                            more[ct] = __builtin_fmaf(part, inv[h], more[ct]);
+#pragma unroll
+                            for (int n = 0; n < NP; ++n)
+#pragma unroll
+                                for (int t = 0; t < 4; ++t) {
+                                    if constexpr (NP == 1) {
+                                        bf16x2 w = {(__bf16)p[2 * t], (__bf16)p[2 * t + 1]};
+                                        pf[h][ct][n][t] = __builtin_bit_cast(uint32_t, w);
+                                    } else {
+                                        pf[h][ct][n][t] = pack_hi16(bf16_part(p[2 * t], n), bf16_part(p[2 * t + 1], n));
+                                    }
+                                }
+                            __builtin_amdgcn_sched_barrier(0);
+                        }
+                    }
+                    if (FULL && __any(over)) return false;
+#pragma unroll
+                    for (int ct = 0; ct < NT; ++ct) sum[ct] += more[ct];
+                    if (kb + 128 < hi) load(kb + 128, pc);
+                    // values: likewise
+                    u32x4 vf[4];
+                    auto read_value = [&](int e) { vf[e & 3] = *(const u32x4*)(here + value_at[e % ND & 3] + (e % ND * 2 + e / ND) * 1024); };
+#pragma unroll
+                    for (int e = 0; e < 3; ++e) read_value(e);
+#pragma unroll
+                    for (int e = 0; e < 2 * ND; ++e) {
+                        const int h = e / ND, d = e % ND;
+                        if (e + 3 < 2 * ND) read_value(e + 3);
+                        u32x4 x = vf[e & 3];
+                        if constexpr (!FULL) {
+                            // A NaN among values that some rows do not see must not reach those (0 * NaN): it is taken out,
+                            // and counted for each row by a product of its own.  Tiles at an edge are few.
+                            u32x4 is_nan;
+#pragma unroll
+                            for (int t = 0; t < 4; ++t) {
+                                const uint32_t n = ((x[t] & 0x7FFFu) > 0x7F80u ? 0xFFFFu : 0u) | ((x[t] & 0x7FFF0000u) > 0x7F800000u ? 0xFFFF0000u : 0u);
+                                is_nan[t] = n & 0x3F803F80u;
+                                x[t] &= ~n;
+                            }
+#pragma unroll
+                            for (int ct = 0; ct < NT; ++ct) {
+                                u32x4 sees;
+#pragma unroll
+                                for (int t = 0; t < 4; ++t)
+                                    sees[t] = (seen[h][ct] >> (2 * t) & 1 ? 0x3F80u : 0u) | (seen[h][ct] >> (2 * t + 1) & 1 ? 0x3F800000u : 0u);
+                                const f32x4 n = mfma<false>(is_nan, sees, f32x4{0, 0, 0, 0});
+#pragma unroll
+                                for (int i = 0; i < 4; ++i) o[ct][d][i] = n[i] > 0.0f ? float_of(0x7FC00000u) : o[ct][d][i];
+                            }
+                        }
+#pragma unroll
+                        for (int ct = 0; ct < NT; ++ct)
+#pragma unroll
+                            for (int n = 0; n < NP; ++n) o[ct][d] = mfma<false>(x, pf[h][ct][n], o[ct][d]);
+                        if (!FULL || e % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+                    }
+                    return true;
+        };
+        auto advance = [&] {
+            pa = pb, pb = pc, pc = pages(kb + 192);
+            kb += 64;
+            buf ^= 1;
+            __syncthreads();
+        };
+        // (behind the last tile the other buffer is filled with what the registers hold, and read by nobody)
+        // Every wave passes the same barriers, one a tile, from whichever of the two loops.
+        while (kb < hi) {
+            if (kb + 64 < hi) hide(kb + 64, pb);
+            if (idle || kb > wpos1 || kb + 63 < w_lo) {
+                store_keys(buf ^ 1);
+                store_values(buf ^ 1);
+                if (kb + 128 < hi) load(kb + 128, pc);
+            } else {
+                compute(std::false_type());
+            }
+            advance();
+            bool again = false;
+            while (kb < hi && plain(kb, pa) && !again) {
+                if (kb + 64 < hi) hide(kb + 64, pb);
+                again = !compute(std::true_type());
+                if (!again) advance();
+            }
+        }
+#pragma unroll
+        for (int ct = 0; ct < NT; ++ct) {
+            float total = sum[ct];
+            total += __shfl_xor(total, 16);
+            total += __shfl_xor(total, 32);
+            const int64_t r = wrow0 + ct * 16 + m;
+            if (r < rows) {
+                const int32_t tok = (int32_t)(r / G);
+                const uint64_t orow = (uint64_t)(s.first + tok) * a.q_heads + head * G + (uint32_t)(r - (int64_t)tok * G);
+                const bool none = total == 0.0f;
+                const float inv = none ? 0.0f : 1.0f / total;
+                E<T>* out = (E<T>*)a.out + orow * D + q4 * 4;
+#pragma unroll
+                for (int d = 0; d < ND; ++d) {
+                    typedef __attribute__((ext_vector_type(4))) E<T> vec;
+                    vec v;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) v[i] = (E<T>)(none ? 0.0f : o[ct][d][i] * inv);
+                    *(vec*)(out + d * 16) = v;
+                }
+                if (a.lse && q4 == 0) a.lse[orow] = none ? -__builtin_inff() : (top[ct] + __builtin_amdgcn_logf(total)) * kLn2;
+            }
+        }
     }
 }
 
@@ -583,6 +1007,12 @@ __global__ __launch_bounds__(kJoinThreads) void kv_join(KvAttendArgs a, Plan pla
 
 template <int T, int DS>
 hipError_t launch_one(const KvAttendArgs& a, const Plan& plan, hipStream_t stream) {
+    if (plan.many) {
+        const uint32_t G = a.q_heads / a.mem.heads, rows = Many<T, DS>::rows;
+        const uint64_t blocks = std::min<uint64_t>(((uint64_t)plan.max_new * G + rows - 1) / rows, (1u << 30) / a.mem.heads);
+        hipLaunchKernelGGL((kv_attend_many<T, DS>), dim3((uint32_t)blocks * a.mem.heads, 1, a.batch.count), dim3(256), (Many<T, DS>::lds), stream, a);
+        return hipGetLastError();
+    }
     const dim3 grid(plan.tiles * plan.splits, a.mem.heads, a.batch.count);
     if (a.select) hipLaunchKernelGGL((kv_attend<T, DS, true>), grid, dim3(256), (Shape<T, DS>::lds), stream, a, plan);
     else hipLaunchKernelGGL((kv_attend<T, DS, false>), grid, dim3(256), (Shape<T, DS>::lds), stream, a, plan);
@@ -608,6 +1038,10 @@ hipError_t launch_join(const KvAttendArgs& a, const Plan& plan, uint32_t rows, h
 Plan plan_of(const KvAttendArgs& a, uint32_t max_new) {
     const uint32_t G = a.q_heads / a.mem.heads;
     Plan p{};
+    p.max_new = max_new;
+    p.splits = 1;
+    p.many = !a.select && (uint64_t)max_new * G / 192 * a.mem.heads * a.batch.count >= 128;
+    if (p.many) return p;
     p.tiles = (uint32_t)std::min<uint64_t>(((uint64_t)max_new * G + 15) / 16, 65535);
     uint64_t tokens = a.select ? a.n_select : (uint64_t)a.batch.table_width << a.mem.page_shift;
     if (!a.select && a.window) tokens = std::min<uint64_t>(tokens, (uint64_t)a.window + max_new + 31);

@@ -53,10 +53,10 @@ class KeyValueMemory:
             raise ValueError("expected k, v [pages, kv_heads, page_tokens, head_dim] and k_scale, v_scale [pages, kv_heads]")
         if k.dtype != torch.float8_e4m3fn or v.dtype != torch.float8_e4m3fn or k_scale.dtype != torch.float32 or v_scale.dtype != torch.float32:
             raise ValueError("k, v: float8_e4m3fn; k_scale, v_scale: float32")
-        tensors = (k, v, k_scale, v_scale)
-        if not all(t.is_cuda and t.device == k.device for t in tensors):
+        device = k.device
+        if not k.is_cuda or v.device != device or k_scale.device != device or v_scale.device != device:
             raise ValueError("k, v, k_scale, v_scale: CUDA tensors on one device")
-        if not all(t.is_contiguous() for t in tensors):
+        if not (k.is_contiguous() and v.is_contiguous() and k_scale.is_contiguous() and v_scale.is_contiguous()):
             raise ValueError("k, v, k_scale, v_scale must be contiguous")
         pages, heads, page_tokens, dim = k.shape
         if page_tokens < 16 or page_tokens > 1024 or page_tokens & (page_tokens - 1):
@@ -64,8 +64,8 @@ class KeyValueMemory:
         if dim < 32 or dim > 256 or dim % 32:
             raise ValueError("head_dim must be a multiple of 32 in 32..256")
         self._l = _lib.lib()
-        self.k, self.v, self.k_scale, self.v_scale = tensors
-        self.device = k.device
+        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self.device = device
         self.kv_heads, self.page_tokens, self.head_dim = heads, page_tokens, dim
         self._m = KvMemoryStruct(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), pages, heads, page_tokens, dim)
 

@@ -9,17 +9,23 @@ from . import _lib
 from ._lib import BF16, F16, F32, check
 
 
-def dtype_code(t, what: str) -> int:
-    import torch
+_codes = {}
 
-    code = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}.get(t.dtype)
+
+def dtype_code(t, what: str) -> int:
+    if not _codes:
+        import torch
+
+        _codes.update({torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16})
+    code = _codes.get(t.dtype)
     if code is None:
         raise ValueError(f"{what}: float32, float16 or bfloat16, got {t.dtype}")
     return code
 
 
 class on_device:
-    """Makes a tensor's device current for the call, and gives its current stream."""
+    """Makes a tensor's device current for the call, and gives its current stream (as a number: torch.cuda.current_stream,
+    which makes an object of it, costs the host 7 us)."""
 
     __slots__ = ("index", "prev")
 
@@ -29,10 +35,10 @@ class on_device:
     def __enter__(self):
         import torch
 
-        self.prev = torch.cuda.current_device()
+        self.prev = torch._C._cuda_getDevice()
         if self.prev != self.index:
             torch.cuda.set_device(self.index)
-        return torch.cuda.current_stream().cuda_stream
+        return torch._C._cuda_getCurrentRawStream(self.index)
 
     def __exit__(self, *exc):
         if self.prev != self.index:

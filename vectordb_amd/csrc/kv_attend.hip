@@ -139,9 +139,20 @@ __device__ __forceinline__ constexpr int key_byte(int q4, int j) {
     return j == DS - 1 && (DS & 1) ? (DS - 1) * 32 + q4 * 8 : (j >> 1) * 64 + q4 * 16 + (j & 1) * 8;
 }
 
-template <int T, int DS, bool SEL>
-__global__ __launch_bounds__(256, T == kF32 ? (DS <= 2 ? 3 : DS <= 5 ? 2 : 1) : DS <= 2 ? 4 : DS <= 4 ? 3 : DS <= 6 ? 2 : 1) void kv_attend(KvAttendArgs a, Plan plan) {
-    constexpr bool HALF = T == kF16;
+// What a query sees: the tokens up to its own (chunks of several tokens), the same for all rows of a block (one new token per
+// sequence), or a list of tokens.
+enum { kChunks = 0, kSingle = 1, kSelected = 2 };
+
+// Waves a SIMD that the registers allow (512 / waves each, without spilling).
+constexpr int attend_waves(int t, int ds, int mode) {
+    if (t == kF32) return ds <= 2 ? 3 : ds <= 5 ? 2 : 1;
+    if (mode == kSingle) return ds <= 2 || (ds == 3 && t == kBF16) ? 4 : ds <= 4 ? 3 : 2;  // (bf16 at 128 would just fit four: 136 us instead of 120)
+    return ds <= 2 ? 4 : ds <= 4 ? 3 : ds <= 6 || mode == kSelected ? 2 : 1;
+}
+
+template <int T, int DS, int MODE>
+__global__ __launch_bounds__(256, attend_waves(T, DS, MODE)) void kv_attend(KvAttendArgs a, Plan plan) {
+    constexpr bool HALF = T == kF16, SEL = MODE == kSelected;
     constexpr int NQ = T == kF32 ? 3 : 1, NP = Parts<T>::value, D = DS * 32, ND = DS * 2, LDO = Shape<T, DS>::LDO;
     constexpr int VW = DS / 4 * 2 + (DS >> 1 & 1) + (DS & 1);  // words of a value that a lane holds
     extern __shared__ float smem[];
@@ -167,7 +178,7 @@ __global__ __launch_bounds__(256, T == kF32 ? (DS <= 2 ? 3 : DS <= 5 ? 2 : 1) : 
         const int32_t pos0 = s.start + (int32_t)(row0 / G), pos1 = s.start + (int32_t)(row1 / G);
         int32_t lo, hi;
         range_of<SEL>(a, s, pos0, pos1, lo, hi);
-        const bool same = SEL || pos0 == pos1;
+        const bool same = MODE != kChunks || pos0 == pos1;
         const int32_t lo_all = a.window == 0 ? 0 : (int32_t)max((int64_t)0, pos1 - a.window + 1), hi_all = SEL ? hi : min(max(pos0, -1) + 1, hi);
         int32_t kb0 = lo & ~31, kb1 = hi;
         bool whole = true;  // this block sees all of the tile's tokens
@@ -357,7 +368,7 @@ __global__ __launch_bounds__(256, T == kF32 ? (DS <= 2 ? 3 : DS <= 5 ? 2 : 1) : 
             uint32_t seen = 255;
             if (!full) {
                 seen = live ? have : 0;
-                if constexpr (!SEL) {
+                if constexpr (MODE == kChunks) {
 #pragma unroll
                     for (int t = 0; t < 8; ++t) {
                         const int32_t i = kb + q4 * 8 + t;
@@ -408,7 +419,7 @@ __global__ __launch_bounds__(256, T == kF32 ? (DS <= 2 ? 3 : DS <= 5 ? 2 : 1) : 
             }
             // a NaN among values that some rows of the tile do not see must not reach those (0 * NaN)
             bool mixed = false;
-            if (!SEL && !full && !same) {
+            if (MODE == kChunks && !full && !same) {
                 uint32_t odd = 0;
 #pragma unroll
                 for (int t = 0; t < 8; ++t)
@@ -457,8 +468,12 @@ __global__ __launch_bounds__(256, T == kF32 ? (DS <= 2 ? 3 : DS <= 5 ? 2 : 1) : 
                 }
             }
             };
-            if (mixed) values(std::true_type());
-            else values(std::false_type());
+            if constexpr (MODE == kChunks) {
+                if (mixed) values(std::true_type());
+                else values(std::false_type());
+            } else {
+                values(std::false_type());
+            }
             p0 = n0, p1 = n1;
             if constexpr (!SEL) n0 = page_of(kb + 256), n1 = page_of(kb + 272);
             slot ^= 1;
@@ -1014,8 +1029,9 @@ hipError_t launch_one(const KvAttendArgs& a, const Plan& plan, hipStream_t strea
         return hipGetLastError();
     }
     const dim3 grid(plan.tiles * plan.splits, a.mem.heads, a.batch.count);
-    if (a.select) hipLaunchKernelGGL((kv_attend<T, DS, true>), grid, dim3(256), (Shape<T, DS>::lds), stream, a, plan);
-    else hipLaunchKernelGGL((kv_attend<T, DS, false>), grid, dim3(256), (Shape<T, DS>::lds), stream, a, plan);
+    if (a.select) hipLaunchKernelGGL((kv_attend<T, DS, kSelected>), grid, dim3(256), (Shape<T, DS>::lds), stream, a, plan);
+    else if (!a.batch.offsets) hipLaunchKernelGGL((kv_attend<T, DS, kSingle>), grid, dim3(256), (Shape<T, DS>::lds), stream, a, plan);
+    else hipLaunchKernelGGL((kv_attend<T, DS, kChunks>), grid, dim3(256), (Shape<T, DS>::lds), stream, a, plan);
     return hipGetLastError();
 }
 

@@ -7,6 +7,7 @@
 // vector instruction per column.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <string>
 
 #include "launch.hpp"
@@ -23,73 +24,175 @@ struct ProductArgs {
     float* out;
     uint64_t x_stride;  // elements between two queries
     uint32_t n, dim, groups, nq;
+    uint32_t chunk;  // blocks of 128 columns whose queries are in LDS at once
 };
 
-// The columns [c0, c0 + 32) of a query as bf16 part `split`, zero beyond `dim`: four matrix operands of 8 columns.
-template <int T>
-__device__ __forceinline__ void load_parts(const typename Elem<T>::type* x, uint32_t c0, uint32_t dim, int split, uint32_t out[16]) {
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-        const uint32_t c = c0 + 2 * i;
-        const float a = c < dim ? to_f32(x[c]) : 0.0f;
-        const float b = c + 1 < dim ? to_f32(x[c + 1]) : 0.0f;
-        out[i] = pack_hi16(bf16_part(a, split), bf16_part(b, split));
-    }
-}
-
-// y[m][r] = sum_c x[m][c] * value[r][c] on the matrix units: 16 rows are the A operand; the 16 columns of B are (query, part)
-// pairs, a query in f32 being three bf16 parts (f16: two) that sum to it exactly.  So no bit of a query is lost, and the f32
-// accumulators see exact products.
-template <int T>
+// y[m][r] = sum_c x[m][c] * value[r][c] on the matrix units: 16 rows are the A operand, 16 queries the B operand.  A query in
+// f32 is three bf16 parts (f16: two) that sum to it exactly, one matrix instruction each into the same accumulator: no bit of a
+// query is lost, and the f32 accumulators see exact products.
+//
+// What bounds it is the rows' bytes.  The queries go to LDS once per block, as parts and in operand order; the blocks are
+// persistent, and a wave takes RT tiles of 16 rows by 128 columns at a time (16 bytes of codes and one scale a lane and tile),
+// the next ones on their way while these are multiplied.  A lane holds 32 consecutive columns of one row, and the four matrix
+// steps of a tile take 8 of them each, so that rows are read as they are stored, 64 bytes side by side.
+// Queries whose parts are too large for LDS are taken in ranges of columns, each added to the results of the one before.
+template <int T, int RT, int NCT, bool SPLIT>
 __global__ __launch_bounds__(256) void rows4_products(ProductArgs a) {
-    constexpr int S = Elem<T>::splits, Q = 16 / S;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    constexpr int S = Elem<T>::splits;
+    extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int m = lane & 15, q4 = lane >> 4;
-    const uint32_t row0 = (blockIdx.x * 4u + wave) * 16u;
-    if (row0 >= a.n) return;
-    const uint32_t row = min(row0 + m, a.n - 1);
-    const uint32_t query = blockIdx.y * Q + m / S;
-    const bool live = m < Q * S && query < a.nq;
-    const typename Elem<T>::type* x = (const typename Elem<T>::type*)a.x + (live ? query : 0) * a.x_stride;
-    const uint8_t* codes = a.codes + (uint64_t)row * a.groups * 16u;
-    const uint8_t* scales = a.scales + (uint64_t)row * a.groups;
-    f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (uint32_t g0 = 0; g0 < a.groups; g0 += 4) {
-        const uint32_t g = g0 + q4;
-        u32x4 w = {0, 0, 0, 0};
-        uint32_t e = 127;
-        if (g < a.groups) {
-            w = *(const u32x4*)(codes + (uint64_t)g * 16u);
-            e = scales[g];
+    const uint32_t q0 = blockIdx.y * (16 * NCT), nq = min(a.nq - q0, 16u * NCT);
+    const uint32_t nblk = (a.groups + 3) / 4, plane = a.chunk * nq * 256;  // bytes of one part of the queries
+    const uint32_t tiles = (a.n + 16 * RT - 1) / (16 * RT);
+    const uint32_t first = SPLIT ? blockIdx.x : blockIdx.x * 4 + wave, step = SPLIT ? gridDim.x : gridDim.x * 4;
+    // where a lane finds its query among nq of them (operands: [block][step][query][quarter] of 16 bytes)
+    uint32_t at[NCT];
+#pragma unroll
+    for (int ct = 0; ct < NCT; ++ct) at[ct] = (min((uint32_t)(ct * 16 + m), nq - 1) * 4 + q4) * 16;
+
+    for (uint32_t b0 = 0; b0 < nblk; b0 += a.chunk) {
+        const uint32_t b1 = min(b0 + a.chunk, nblk);
+        __syncthreads();
+        for (uint32_t u = threadIdx.x; u < (b1 - b0) * 16 * nq; u += 256) {  // 8 columns of one query
+            const uint32_t quarter = u & 3, query = (u >> 2) % nq, bs = (u >> 2) / nq;  // bs = block * 4 + step
+            const uint32_t c0 = (b0 + (bs >> 2)) * 128 + quarter * 32 + (bs & 3) * 8;
+            const typename Elem<T>::type* x = (const typename Elem<T>::type*)a.x + (uint64_t)(q0 + query) * a.x_stride;
+            float v[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = c0 + i < a.dim ? to_f32(x[c0 + i]) : 0.0f;
+#pragma unroll
+            for (int s = 0; s < S; ++s)
+                *(u32x4*)(lds + s * plane + u * 16) =
+                    u32x4{pack_hi16(bf16_part(v[0], s), bf16_part(v[1], s)), pack_hi16(bf16_part(v[2], s), bf16_part(v[3], s)),
+                          pack_hi16(bf16_part(v[4], s), bf16_part(v[5], s)), pack_hi16(bf16_part(v[6], s), bf16_part(v[7], s))};
         }
-        uint32_t b[16];
-        load_parts<T>(x, g * 32u, live ? a.dim : 0, m % S, b);
-        const float scale = float_of(e == 0 ? 0x00400000u : e << 23);
+        __syncthreads();
+
+        u32x4 w[2][RT];
+        uint32_t e[2][RT];
+        auto fetch = [&](uint32_t tile, uint32_t blk, u32x4 cw[RT], uint32_t ce[RT]) {
+            const uint32_t g = blk * 4 + q4;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            bf16x8 av;
-            uint32_t* ap = (uint32_t*)&av;
-            ap[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w[j], scale, 0));
-            ap[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w[j], scale, 1));
-            ap[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w[j], scale, 2));
-            ap[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w[j], scale, 3));
-            u32x4 bv = {b[4 * j], b[4 * j + 1], b[4 * j + 2], b[4 * j + 3]};
-            acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(av, __builtin_bit_cast(bf16x8, bv), acc, 0, 0, 0);
-        }
-    }
-    // lane (m, q4) holds rows row0 + 4 q4 + i of column m; the parts of a query sit in neighbouring columns
-    f32x4 y = {0.0f, 0.0f, 0.0f, 0.0f};
+            for (int r = 0; r < RT; ++r) {
+                const uint32_t row = min(tile * (16 * RT) + r * 16 + m, a.n - 1);
+                const uint64_t at = (uint64_t)row * a.groups + min(g, a.groups - 1);
+                cw[r] = *(const u32x4*)(a.codes + at * 16);
+                ce[r] = a.scales[at];
+                if (blk * 4 + 4 > a.groups && g >= a.groups) cw[r] = u32x4{0, 0, 0, 0}, ce[r] = 127;
+            }
+        };
+        f32x4 acc[RT][NCT];
+        auto multiply = [&](uint32_t blk, const u32x4 cw[RT], const uint32_t ce[RT]) {
+            const unsigned char* here = lds + (blk - b0) * nq * 256;
 #pragma unroll
-    for (int s = S - 1; s >= 0; --s) {
+            for (int j = 0; j < 4; ++j) {
+                u32x4 bv[NCT][S];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) y[i] += __shfl(acc[i], (lane & 48) | ((m * S + s) & 15));
-    }
-    const uint32_t oq = blockIdx.y * Q + m;
-    if (m < Q && oq < a.nq) {
+                for (int ct = 0; ct < NCT; ++ct)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const uint32_t r = row0 + 4 * q4 + i;
-            if (r < a.n) a.out[(uint64_t)oq * a.n + r] = y[i];
+                    for (int s = 0; s < S; ++s) bv[ct][s] = *(const u32x4*)(here + s * plane + j * nq * 64 + at[ct]);
+#pragma unroll
+                for (int r = 0; r < RT; ++r) {
+                    const float scale = float_of(ce[r] == 0 ? 0x00400000u : ce[r] << 23);
+                    const u32x4 av = {__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(cw[r][j], scale, 0)),
+                                      __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(cw[r][j], scale, 1)),
+                                      __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(cw[r][j], scale, 2)),
+                                      __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(cw[r][j], scale, 3))};
+#pragma unroll
+                    for (int ct = 0; ct < NCT; ++ct)
+#pragma unroll
+                        for (int s = S - 1; s >= 0; --s)
+                            acc[r][ct] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, av), __builtin_bit_cast(bf16x8, bv[ct][s]), acc[r][ct], 0, 0, 0);
+                }
+            }
+        };
+        // (tile, block) pairs of this wave in order; with SPLIT the block's waves share a tile and take every fourth block of it
+        const uint32_t start = b0 + (SPLIT ? wave : 0), stride = SPLIT ? 4 : 1;
+        uint32_t tile = first, blk = start, ntile = first, nblkk = start;
+        auto next = [&](uint32_t& t, uint32_t& b) {
+            b += stride;
+            if (b >= b1) b = start, t += step;
+        };
+        auto clear = [&] {
+#pragma unroll
+            for (int r = 0; r < RT; ++r)
+#pragma unroll
+                for (int ct = 0; ct < NCT; ++ct) acc[r][ct] = f32x4{0, 0, 0, 0};
+        };
+        // lane (m, q4) holds rows 4 q4 + i of query m
+        auto finish = [&](uint32_t t) {
+#pragma unroll
+            for (int ct = 0; ct < NCT; ++ct)
+                if (ct * 16 + m < nq) {
+#pragma unroll
+                    for (int r = 0; r < RT; ++r) {
+                        const uint32_t row = t * (16 * RT) + r * 16 + q4 * 4;
+                        float* o = a.out + (uint64_t)(q0 + ct * 16 + m) * a.n + row;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            if (row + i < a.n) o[i] = b0 ? o[i] + acc[r][ct][i] : acc[r][ct][i];
+                    }
+                }
+        };
+        if constexpr (!SPLIT) {
+            clear();
+            if (ntile < tiles) fetch(ntile, nblkk, w[0], e[0]);
+            while (tile < tiles) {
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    if (tile < tiles) {
+                        next(ntile, nblkk);
+                        if (ntile < tiles) fetch(ntile, nblkk, w[k ^ 1], e[k ^ 1]);
+                        multiply(blk, w[k], e[k]);
+                        const uint32_t t = tile;
+                        next(tile, blk);
+                        if (tile != t) {
+                            finish(t);
+                            clear();
+                        }
+                    }
+                }
+            }
+        } else {
+            float* red = (float*)(lds + S * plane);  // [4][RT * NCT * 4][64]
+            for (uint32_t t = first; t < tiles; t += step) {
+                clear();
+                uint32_t b = start;
+                if (b < b1) fetch(t, b, w[0], e[0]);
+                while (b < b1) {
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) {
+                        if (b < b1) {
+                            if (b + 4 < b1) fetch(t, b + 4, w[k ^ 1], e[k ^ 1]);
+                            multiply(b, w[k], e[k]);
+                            b += 4;
+                        }
+                    }
+                }
+#pragma unroll
+                for (int r = 0; r < RT; ++r)
+#pragma unroll
+                    for (int ct = 0; ct < NCT; ++ct)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) red[((wave * RT + r) * NCT + ct) * 256 + i * 64 + lane] = acc[r][ct][i];
+                __syncthreads();
+                if (wave == 0) {
+#pragma unroll
+                    for (int r = 0; r < RT; ++r)
+#pragma unroll
+                        for (int ct = 0; ct < NCT; ++ct)
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                float y = 0.0f;
+#pragma unroll
+                                for (int v = 0; v < 4; ++v) y += red[((v * RT + r) * NCT + ct) * 256 + i * 64 + lane];
+                                acc[r][ct][i] = y;
+                            }
+                    finish(t);
+                }
+                __syncthreads();
+            }
         }
     }
 }
@@ -172,11 +275,31 @@ int done(const char* what, std::string* err) {
 
 int launch_rows4_products(const uint8_t* d_codes, const uint8_t* d_scales, uint32_t n, uint32_t dim, const void* d_x, int dtype, uint32_t nq,
                           uint64_t x_stride, float* d_out, hipStream_t stream, std::string* err) {
-    const ProductArgs a{d_codes, d_scales, d_x, d_out, x_stride, n, dim, (dim + 31) / 32, nq};
-    const uint32_t bx = (n + 63) / 64;
+    ProductArgs a{d_codes, d_scales, d_x, d_out, x_stride, n, dim, (dim + 31) / 32, nq, 0};
     auto go = [&](auto t) {
-        constexpr int T = decltype(t)::value, Q = 16 / Elem<T>::splits;
-        hipLaunchKernelGGL((rows4_products<T>), dim3(bx, (nq + Q - 1) / Q), dim3(256), 0, stream, a);
+        constexpr int T = decltype(t)::value, S = Elem<T>::splits;
+        const uint32_t nblk = (a.groups + 3) / 4, tiles = (n + 15) / 16;
+        const bool two = nq > 16;  // two column tiles: 17 to 32 queries a pass over the rows
+        const uint32_t per = std::min(nq, two ? 32u : 16u), ys = (nq + (two ? 31 : 15)) / (two ? 32 : 16);
+        const uint32_t block = per * 256 * S;  // bytes of LDS for 128 columns
+        a.chunk = std::max(1u, std::min(nblk, (64u << 10) / block));
+        auto launch = [&](auto kernel, uint32_t rt, bool split) {
+            const uint32_t groups = (tiles + rt - 1) / rt;
+            const size_t lds = (size_t)a.chunk * block + (split ? 4 * rt * (two ? 2 : 1) * 1024 : 0);
+            const uint32_t fit = std::max<uint32_t>(1, std::min<uint32_t>(4, (uint32_t)((160u << 10) / lds)));
+            const uint32_t blocks = std::min(split ? groups : (groups + 3) / 4, 256 * fit);
+            hipLaunchKernelGGL(kernel, dim3(blocks, ys), dim3(256), lds, stream, a);
+        };
+        if (tiles <= 2048 && nblk >= 4) {
+            if (two) launch(rows4_products<T, 1, 2, true>, 1, true);
+            else launch(rows4_products<T, 1, 1, true>, 1, true);
+        } else if (tiles < 16384) {
+            if (two) launch(rows4_products<T, 1, 2, false>, 1, false);
+            else launch(rows4_products<T, 1, 1, false>, 1, false);
+        } else {
+            if (two) launch(rows4_products<T, 4, 2, false>, 4, false);
+            else launch(rows4_products<T, 4, 1, false>, 4, false);
+        }
     };
     if (dtype == kF32) go(std::integral_constant<int, kF32>());
     else if (dtype == kF16) go(std::integral_constant<int, kF16>());

@@ -221,3 +221,22 @@ def test_beside_the_exact_scan():
     tenth = score.topk(10, 1).values[:, 9:]
     keep = score >= tenth - 2.001 * off
     assert keep.gather(1, label).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("n,dim,nq", [(8200 * 16 + 3, 96, 3), (8200 * 16 + 5, 300, 2), (8192 * 16, 129, 20), (600 * 16 + 1, 600, 5),
+                                      (1500 * 16 + 7, 200, 18), (40, 30000, 2), (50, 9000, 16), (700, 2100, 32)])
+def test_products_every_variant(dtype, n, dim, nq):
+    """Sizes on both sides of every rule: many rows of one and of more blocks of columns, waves that share a tile, one and two
+    tiles of queries, queries too large for LDS."""
+    codes, scales = random_rows(n, dim, n % 1000 + dim)
+    rows = make(codes, scales, dim)
+    x = torch.from_numpy(np.random.default_rng(nq).standard_normal((nq, dim)).astype(np.float32)).to(TYPES[dtype])
+    y = rows.products(x.cuda())
+    rowsd = torch.from_numpy(values(codes, scales, dim))
+    ref, size = x.double() @ rowsd.t(), x.double().abs() @ rowsd.abs().t()
+    tol = (3 * -(-dim // 128) * 128 + 3) * 2.0 ** -24 * size + 1e-37
+    assert ((y.cpu().double() - ref).abs() <= tol).all()
+    again = rows.products(x.cuda())
+    assert torch.equal(y, again)

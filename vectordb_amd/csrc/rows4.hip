@@ -32,12 +32,17 @@ struct ProductArgs {
 // query is lost, and the f32 accumulators see exact products.
 //
 // What bounds it is the rows' bytes.  The queries go to LDS once per block, as parts and in operand order; the blocks are
-// persistent, and a wave takes RT tiles of 16 rows by 128 columns at a time (16 bytes of codes and one scale a lane and tile),
-// the next ones on their way while these are multiplied.  A lane holds 32 consecutive columns of one row, and the four matrix
-// steps of a tile take 8 of them each, so that rows are read as they are stored, 64 bytes side by side.
+// persistent, and a wave takes RT tiles of 16 rows by KB blocks of 128 columns at a time (16 bytes of codes and one scale a lane
+// for each), the next ones on their way while these are multiplied.  Four neighbouring lanes load 64 consecutive bytes of a row (a lane 32
+// columns, of which each of the four matrix steps takes 8) and the lanes then exchange what they hold for the order that the
+// matrix units want: loaded in that order, every lane touches a cache line of its own (1M x 128 x 16: 50 us instead of 30, with the stores).
+// The rows are the B operand, so that 16 lanes hold results of one query for neighbouring rows and store them side by side.
 // Queries whose parts are too large for LDS are taken in ranges of columns, each added to the results of the one before.
-template <int T, int RT, int NCT, bool SPLIT>
-__global__ __launch_bounds__(256) void rows4_products(ProductArgs a) {
+// Blocks that a compute unit holds, by registers.
+constexpr int products_blocks(int pieces, int nct) { return pieces == 1 ? 6 : nct == 1 ? 4 : 3; }
+
+template <int T, int RT, int KB, int NCT, bool SPLIT>
+__global__ __launch_bounds__(256, products_blocks(RT * KB, NCT)) void rows4_products(ProductArgs a) {
     constexpr int S = Elem<T>::splits;
     extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -59,8 +64,15 @@ __global__ __launch_bounds__(256) void rows4_products(ProductArgs a) {
             const uint32_t c0 = (b0 + (bs >> 2)) * 128 + quarter * 32 + (bs & 3) * 8;
             const typename Elem<T>::type* x = (const typename Elem<T>::type*)a.x + (uint64_t)(q0 + query) * a.x_stride;
             float v[8];
+            if (c0 + 8 <= a.dim) {
+                typedef __attribute__((ext_vector_type(8), aligned(sizeof(typename Elem<T>::type)))) typename Elem<T>::type vec;
+                const vec y = *(const vec*)(x + c0);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = c0 + i < a.dim ? to_f32(x[c0 + i]) : 0.0f;
+                for (int i = 0; i < 8; ++i) v[i] = to_f32((typename Elem<T>::type)y[i]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[i] = c0 + i < a.dim ? to_f32(x[c0 + i]) : 0.0f;
+            }
 #pragma unroll
             for (int s = 0; s < S; ++s)
                 *(u32x4*)(lds + s * plane + u * 16) =
@@ -69,46 +81,61 @@ __global__ __launch_bounds__(256) void rows4_products(ProductArgs a) {
         }
         __syncthreads();
 
-        u32x4 w[2][RT];
-        uint32_t e[2][RT];
-        auto fetch = [&](uint32_t tile, uint32_t blk, u32x4 cw[RT], uint32_t ce[RT]) {
-            const uint32_t g = blk * 4 + q4;
+        u32x4 w[2][RT * KB];
+        uint32_t e[2][RT * KB];
+        auto fetch = [&](uint32_t tile, uint32_t blk, u32x4 cw[RT * KB], uint32_t ce[RT * KB]) {
 #pragma unroll
             for (int r = 0; r < RT; ++r) {
-                const uint32_t row = min(tile * (16 * RT) + r * 16 + m, a.n - 1);
-                const uint64_t at = (uint64_t)row * a.groups + min(g, a.groups - 1);
-                cw[r] = *(const u32x4*)(a.codes + at * 16);
-                ce[r] = a.scales[at];
-                if (blk * 4 + 4 > a.groups && g >= a.groups) cw[r] = u32x4{0, 0, 0, 0}, ce[r] = 127;
+                const uint32_t row = min(tile * (16 * RT) + r * 16 + (lane >> 2), a.n - 1);
+#pragma unroll
+                for (int k = 0; k < KB; ++k) {
+                    const uint32_t g = (blk + k) * 4 + (lane & 3);
+                    const uint64_t at = (uint64_t)row * a.groups + min(g, a.groups - 1);
+                    cw[r * KB + k] = *(const u32x4*)(a.codes + at * 16);
+                    ce[r * KB + k] = a.scales[at];
+                    if ((blk + KB) * 4 > a.groups && g >= a.groups) cw[r * KB + k] = u32x4{0, 0, 0, 0}, ce[r * KB + k] = 127;
+                }
             }
         };
         f32x4 acc[RT][NCT];
-        auto multiply = [&](uint32_t blk, const u32x4 cw[RT], const uint32_t ce[RT]) {
-            const unsigned char* here = lds + (blk - b0) * nq * 256;
+        const int from = (m * 4 + q4) * 4;  // the lane that loaded this lane's piece
+        auto multiply = [&](uint32_t blk, u32x4 cw[RT * KB], uint32_t ce[RT * KB]) {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                u32x4 bv[NCT][S];
+            for (int p = 0; p < RT * KB; ++p) {
 #pragma unroll
-                for (int ct = 0; ct < NCT; ++ct)
+                for (int j = 0; j < 4; ++j) cw[p][j] = __builtin_amdgcn_ds_bpermute(from, cw[p][j]);
+                ce[p] = __builtin_amdgcn_ds_bpermute(from, ce[p]);
+            }
 #pragma unroll
-                    for (int s = 0; s < S; ++s) bv[ct][s] = *(const u32x4*)(here + s * plane + j * nq * 64 + at[ct]);
+            for (int k = 0; k < KB; ++k) {
+                if (KB > 1 && blk + k >= b1) break;
+                const unsigned char* here = lds + (blk + k - b0) * nq * 256;
 #pragma unroll
-                for (int r = 0; r < RT; ++r) {
-                    const float scale = float_of(ce[r] == 0 ? 0x00400000u : ce[r] << 23);
-                    const u32x4 av = {__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(cw[r][j], scale, 0)),
-                                      __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(cw[r][j], scale, 1)),
-                                      __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(cw[r][j], scale, 2)),
-                                      __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(cw[r][j], scale, 3))};
+                for (int j = 0; j < 4; ++j) {
+                    u32x4 bv[NCT][S];
 #pragma unroll
                     for (int ct = 0; ct < NCT; ++ct)
 #pragma unroll
-                        for (int s = S - 1; s >= 0; --s)
-                            acc[r][ct] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, av), __builtin_bit_cast(bf16x8, bv[ct][s]), acc[r][ct], 0, 0, 0);
+                        for (int s = 0; s < S; ++s) bv[ct][s] = *(const u32x4*)(here + s * plane + j * nq * 64 + at[ct]);
+#pragma unroll
+                    for (int r = 0; r < RT; ++r) {
+                        const uint32_t code = cw[r * KB + k][j], x = ce[r * KB + k];
+                        const float scale = float_of(x == 0 ? 0x00400000u : x << 23);
+                        const u32x4 av = {__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(code, scale, 0)),
+                                          __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(code, scale, 1)),
+                                          __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(code, scale, 2)),
+                                          __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(code, scale, 3))};
+#pragma unroll
+                        for (int ct = 0; ct < NCT; ++ct)
+#pragma unroll
+                            for (int s = S - 1; s >= 0; --s)
+                                acc[r][ct] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, bv[ct][s]), __builtin_bit_cast(bf16x8, av), acc[r][ct], 0, 0, 0);
+                    }
                 }
             }
         };
         // (tile, block) pairs of this wave in order; with SPLIT the block's waves share a tile and take every fourth block of it
-        const uint32_t start = b0 + (SPLIT ? wave : 0), stride = SPLIT ? 4 : 1;
+        const uint32_t start = b0 + (SPLIT ? wave * KB : 0), stride = SPLIT ? 4 * KB : KB;
         uint32_t tile = first, blk = start, ntile = first, nblkk = start;
         auto next = [&](uint32_t& t, uint32_t& b) {
             b += stride;
@@ -120,18 +147,20 @@ __global__ __launch_bounds__(256) void rows4_products(ProductArgs a) {
 #pragma unroll
                 for (int ct = 0; ct < NCT; ++ct) acc[r][ct] = f32x4{0, 0, 0, 0};
         };
-        // lane (m, q4) holds rows 4 q4 + i of query m
+        // lane (m, q4) holds row m of queries 4 q4 + i
         auto finish = [&](uint32_t t) {
 #pragma unroll
             for (int ct = 0; ct < NCT; ++ct)
-                if (ct * 16 + m < nq) {
 #pragma unroll
-                    for (int r = 0; r < RT; ++r) {
-                        const uint32_t row = t * (16 * RT) + r * 16 + q4 * 4;
-                        float* o = a.out + (uint64_t)(q0 + ct * 16 + m) * a.n + row;
+                for (int i = 0; i < 4; ++i) {
+                    const uint32_t query = ct * 16 + q4 * 4 + i;
+                    if (query < nq) {
 #pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                            if (row + i < a.n) o[i] = b0 ? o[i] + acc[r][ct][i] : acc[r][ct][i];
+                        for (int r = 0; r < RT; ++r) {
+                            const uint32_t row = t * (16 * RT) + r * 16 + m;
+                            float* o = a.out + (uint64_t)(q0 + query) * a.n + row;
+                            if (row < a.n) *o = b0 ? *o + acc[r][ct][i] : acc[r][ct][i];
+                        }
                     }
                 }
         };
@@ -164,9 +193,9 @@ __global__ __launch_bounds__(256) void rows4_products(ProductArgs a) {
 #pragma unroll
                     for (int k = 0; k < 2; ++k) {
                         if (b < b1) {
-                            if (b + 4 < b1) fetch(t, b + 4, w[k ^ 1], e[k ^ 1]);
+                            if (b + stride < b1) fetch(t, b + stride, w[k ^ 1], e[k ^ 1]);
                             multiply(b, w[k], e[k]);
-                            b += 4;
+                            b += stride;
                         }
                     }
                 }
@@ -283,23 +312,26 @@ int launch_rows4_products(const uint8_t* d_codes, const uint8_t* d_scales, uint3
         const uint32_t per = std::min(nq, two ? 32u : 16u), ys = (nq + (two ? 31 : 15)) / (two ? 32 : 16);
         const uint32_t block = per * 256 * S;  // bytes of LDS for 128 columns
         a.chunk = std::max(1u, std::min(nblk, (64u << 10) / block));
-        auto launch = [&](auto kernel, uint32_t rt, bool split) {
+        auto launch = [&](auto kernel, uint32_t rt, uint32_t kb, bool split) {
             const uint32_t groups = (tiles + rt - 1) / rt;
             const size_t lds = (size_t)a.chunk * block + (split ? 4 * rt * (two ? 2 : 1) * 1024 : 0);
-            const uint32_t fit = std::max<uint32_t>(1, std::min<uint32_t>(4, (uint32_t)((160u << 10) / lds)));
+            const uint32_t fit = std::max<uint32_t>(1, std::min<uint32_t>(products_blocks(rt * kb, two ? 2 : 1), (uint32_t)((160u << 10) / lds)));
             const uint32_t blocks = std::min(split ? groups : (groups + 3) / 4, 256 * fit);
             hipLaunchKernelGGL(kernel, dim3(blocks, ys), dim3(256), lds, stream, a);
         };
-        if (tiles <= 2048 && nblk >= 4) {
-            if (two) launch(rows4_products<T, 1, 2, true>, 1, true);
-            else launch(rows4_products<T, 1, 1, true>, 1, true);
-        } else if (tiles < 16384) {
-            if (two) launch(rows4_products<T, 1, 2, false>, 1, false);
-            else launch(rows4_products<T, 1, 1, false>, 1, false);
-        } else {
-            if (two) launch(rows4_products<T, 4, 2, false>, 4, false);
-            else launch(rows4_products<T, 4, 1, false>, 4, false);
-        }
+        auto pick = [&](auto n_ct) {
+            constexpr int NCT = decltype(n_ct)::value;
+            // Few rows: the waves of a block share the columns of a tile (4000 x 2000: 10.5 -> 6.0 us, 16 000 x 960: 7.9 -> 6.3), with
+            // more than a few queries only where there are very few (16 000 x 960 x 16: 9.6 -> 11.9 us: a block's LDS is filled for less).
+            // Many rows: 4 KB a wave at a time, of rows of more than 128 columns whole cache lines at once (1M x 960: four tiles by 128
+            // columns 169 us and 1.7 times the bytes, two by 256 119 us, one by 512 121, four by 256 138).
+            if (tiles <= (nq <= 4 ? 1024 : 512) && nblk >= 4) launch(rows4_products<T, 1, 1, NCT, true>, 1, 1, true);
+            else if (tiles < 8192) launch(rows4_products<T, 1, 1, NCT, false>, 1, 1, false);
+            else if (nblk == 1) launch(rows4_products<T, 4, 1, NCT, false>, 4, 1, false);
+            else launch(rows4_products<T, 2, 2, NCT, false>, 2, 2, false);
+        };
+        if (two) pick(std::integral_constant<int, 2>());
+        else pick(std::integral_constant<int, 1>());
     };
     if (dtype == kF32) go(std::integral_constant<int, kF32>());
     else if (dtype == kF16) go(std::integral_constant<int, kF16>());

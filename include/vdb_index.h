@@ -328,13 +328,13 @@ int vdb_kv_append_device(const vdb_kv_memory* memory, const vdb_kv_batch* batch,
  *   out = softmax(scale * q . k) v   over the tokens the query sees, [tokens][q_heads][dim] of `dtype`, 16-byte aligned
  *   lse nullable [tokens][q_heads] f32: the natural logarithm of the softmax's sum
  * Query head h reads key head h / (q_heads / heads).  The query at position t sees the present tokens 0..t, with window != 0
- * only the last `window` of them.  With select [count][heads][n_select] (needs offsets = NULL and window = 0) it sees those
+ * only the last `window` of them.  With select [count][heads][n_select >= 1] (needs offsets = NULL and window = 0) it sees those
  * token numbers instead, in any order, each as often as it is listed; numbers outside 0..lengths[b]-1 are skipped, so a
  * search's padding needs no care.  A query that sees nothing gives zeros and -infinity.
  * A token that a query does not see has no effect on its result, whatever it holds.
- * workspace: vdb_kv_attend_workspace() bytes of DEVICE memory, 16-byte aligned, free again once the stream has passed the
+ * workspace: vdb_kv_attend_workspace() bytes (same sizes; n_select 0 without select; 0 bytes may be needed) of DEVICE memory, 16-byte aligned, free again once the stream has passed the
  * call; any contents.  Calls that may overlap need workspaces of their own. */
-size_t vdb_kv_attend_workspace(const vdb_kv_memory* memory, const vdb_kv_batch* batch, size_t q_heads, size_t n_select);
+size_t vdb_kv_attend_workspace(const vdb_kv_memory* memory, const vdb_kv_batch* batch, size_t q_heads, size_t window, size_t n_select);
 int vdb_kv_attend_device(const vdb_kv_memory* memory, const vdb_kv_batch* batch, int dtype, const void* d_q, size_t q_token_stride,
                          size_t q_head_stride, size_t q_heads, float scale, size_t window, const int64_t* d_select, size_t n_select,
                          void* d_out, float* d_lse, void* d_workspace, size_t workspace_bytes, void* stream);

@@ -215,9 +215,11 @@ def test_attend_refusals_without_a_device():
         setattr(b, field, value)
         cases.append((l.vdb_kv_attend_device(m, b, 0, 16, 128, 64, 4, 1.0, 0, None, 0, 16, None, 16, 1 << 40, None), word))
     m, b = good()
+    b.table_width = 1000  # so many tokens that a workspace is needed
     for kw, word in [(dict(dtype=3), "type"), (dict(q=None), "queries"), (dict(q=8), "queries"), (dict(ts=4), "strides"), (dict(hs=65), "strides"),
                      (dict(qh=3), "q_heads"), (dict(qh=0), "q_heads"), (dict(window=1 << 31), "window"), (dict(out=None), "out"), (dict(out=8), "out"),
-                     (dict(select=16, n=4, window=3), "window"), (dict(select=4, n=4), "select"), (dict(select=16, n=1 << 31), "n_select")]:
+                     (dict(select=16, n=4, window=3), "window"), (dict(select=4, n=4), "select"), (dict(select=16, n=1 << 31), "n_select"), (dict(select=16, n=0), "n_select"),
+                     (dict(size=0), "workspace"), (dict(work=None), "workspace")]:
         cases.append((call(m, b, **kw), word))
         assert word in l.vdb_last_error().decode(), kw
     assert all(rc == _lib.VDB_ERR_INVALID for rc, _ in cases), cases
@@ -677,3 +679,48 @@ def test_attend_many_rows(dtype, case):
     out = mem.attend(q.cuda(), table, lengths, offsets=ints(off), max_new=most, window=window, scale=-0.3)
     ref = attend_ref(q, s.k, s.v, s.ks, s.vs, s.table, held, off, page, -0.3, window)
     check_attend(out[:off[-1]], None, [x[:off[-1]] if torch.is_tensor(x) else x for x in ref], t)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("held,window", [(199_000, 0), (199_000, 190_000), (150_000, 196_000), (199_680, 1000), (400, 180_000)])
+def test_attend_long_windows(held, window):
+    """A window cuts the work into other ranges than the whole table would: the workspace is the one of the call's own sizes."""
+    page, heads, dim = 64, 8, 32
+    s = Setup([held], page, heads, dim, seed=17, width=3120)
+    q = s.randn(1, heads, dim)
+    mem = s.memory()
+    table, lengths = s.on_gpu()
+    out, lse = mem.attend(q.cuda(), table, lengths, window=window, return_lse=True)
+    check_attend(out, lse, attend_ref(q, s.k, s.v, s.ks, s.vs, s.table, [held], [0, 1], page, dim ** -0.5, window), torch.float32)
+
+
+@pytest.mark.gpu
+def test_attend_long_lists():
+    """More listed tokens than the table has room for: every one counts."""
+    held, page, heads, dim, n = [60, 30], 16, 2, 64, 40_000
+    s = Setup(held, page, heads, dim, seed=18)
+    q = s.randn(2, 6, dim, dtype=torch.float16)
+    select = torch.randint(-5, 70, (2, heads, n), generator=s.g)
+    mem = s.memory()
+    table, lengths = s.on_gpu()
+    out, lse = mem.attend(q.cuda(), table, lengths, select=select.cuda(), return_lse=True)
+    check_attend(out, lse, attend_ref(q, s.k, s.v, s.ks, s.vs, s.table, held, [0, 1, 2], page, dim ** -0.5, 0, select), torch.float16)
+
+
+def test_workspace_covers_every_range():
+    """The workspace is a whole number of ranges, grows with the table and the list, and none is asked for where one range does."""
+    l = _lib.lib()
+    per = lambda dim: 16 * (dim + 2) * 4  # noqa: E731
+    for dim in (32, 128, 256):
+        for heads, group, count in ((1, 1, 1), (8, 4, 1), (8, 4, 64), (2, 20, 3)):
+            m = _lib.KvMemoryStruct(16, 16, 16, 16, 10, heads, 64, dim)
+            for tokens in (64, 512, 576, 4096, 200_000, 2_000_000):
+                b = _lib.KvBatchStruct(16, 16, None, count, tokens // 64, count, 1)
+                tiles = -(-group // 16)
+                for window, select in ((0, 0), (100, 0), (190_000, 0), (0, 1), (0, 5000), (0, 3_000_000)):
+                    need = l.vdb_kv_attend_workspace(m, b, heads * group, window, select)
+                    seen = select or (min(tokens, window + 32) if window else tokens)
+                    ranges, rest = divmod(need, count * heads * tiles * per(dim))
+                    assert rest == 0 and ranges <= 384
+                    if seen <= 512:
+                        assert need == 0

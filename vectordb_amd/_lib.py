@@ -102,7 +102,7 @@ SIGNATURES = {
     "vdb_rows4_unpack_device": (C.c_int, [_vp, _vp, C.c_size_t, C.c_size_t, _vp, _vp]),
     "vdb_rows4_products_device": (C.c_int, [_vp, _vp, C.c_size_t, C.c_size_t, _vp, C.c_int, C.c_size_t, C.c_size_t, _vp, _vp]),
     "vdb_kv_append_device": (C.c_int, _kvp + [C.c_int, _vp, _sz, _sz, _vp, _sz, _sz, _vp, _vp, _sz, _sz, C.c_int, _vp, _sz, _sz, _sz, _vp, _vp]),
-    "vdb_kv_attend_workspace": (C.c_size_t, _kvp + [_sz, _sz]),
+    "vdb_kv_attend_workspace": (C.c_size_t, _kvp + [_sz, _sz, _sz]),
     "vdb_kv_attend_device": (C.c_int, _kvp + [C.c_int, _vp, _sz, _sz, _sz, C.c_float, _sz, _vp, _sz, _vp, _vp, _vp, _sz, _vp]),
     "vdb_merge_topk_device": (C.c_int, [_vp, _vp, C.c_size_t, C.c_size_t, C.c_size_t, _vp, _vp, _vp]),
 }

@@ -1860,7 +1860,8 @@ void check_kv_dtype(int dtype) {
     if (dtype != VDB_F32 && dtype != VDB_F16 && dtype != VDB_BF16) throw std::invalid_argument("unknown element type");
 }
 
-KvAttendArgs kv_attend_args(const vdb_kv_memory* memory, const vdb_kv_batch* batch, size_t q_heads, size_t n_select) {
+// Everything that the division of the work, and so the workspace, depends on.  n_select 0: no selection.
+KvAttendArgs kv_attend_args(const vdb_kv_memory* memory, const vdb_kv_batch* batch, size_t q_heads, size_t window, size_t n_select) {
     KvAttendArgs a{};
     a.mem = kv_memory(memory);
     a.batch = kv_batch(batch);
@@ -1869,7 +1870,10 @@ KvAttendArgs kv_attend_args(const vdb_kv_memory* memory, const vdb_kv_batch* bat
     if (q_heads < 1 || q_heads % a.mem.heads || q_heads / a.mem.heads > 65535)
         throw std::invalid_argument("kv attend: q_heads must be a multiple of the memory's heads");
     if (n_select >= (1ull << 31) - 1024) throw std::invalid_argument("kv attend: n_select must be below 2^31 - 1024");
+    if (window >= (1ull << 31)) throw std::invalid_argument("kv attend: window must be below 2^31");
+    if (n_select && (a.batch.offsets || window)) throw std::invalid_argument("kv attend: selected tokens go with one new token per sequence and no window");
     a.q_heads = (uint32_t)q_heads;
+    a.window = (int64_t)window;
     a.n_select = (uint32_t)n_select;
     return a;
 }
@@ -1924,10 +1928,10 @@ int vdb_kv_append_device(const vdb_kv_memory* memory, const vdb_kv_batch* batch,
     });
 }
 
-size_t vdb_kv_attend_workspace(const vdb_kv_memory* memory, const vdb_kv_batch* batch, size_t q_heads, size_t n_select) {
+size_t vdb_kv_attend_workspace(const vdb_kv_memory* memory, const vdb_kv_batch* batch, size_t q_heads, size_t window, size_t n_select) {
     size_t bytes = 0;
     (void)guarded([&] {
-        const KvAttendArgs a = kv_attend_args(memory, batch, q_heads, n_select);
+        const KvAttendArgs a = kv_attend_args(memory, batch, q_heads, window, n_select);
         bytes = kv_attend_workspace_bytes(a, kv_max_new(batch));
         return (int)VDB_OK;
     });
@@ -1938,10 +1942,9 @@ int vdb_kv_attend_device(const vdb_kv_memory* memory, const vdb_kv_batch* batch,
                          size_t q_head_stride, size_t q_heads, float scale, size_t window, const int64_t* d_select, size_t n_select,
                          void* d_out, float* d_lse, void* d_workspace, size_t workspace_bytes, void* stream) {
     return guarded([&] {
-        KvAttendArgs a = kv_attend_args(memory, batch, q_heads, d_select ? n_select : 0);
+        if (d_select && !n_select) throw std::invalid_argument("kv attend: select needs n_select >= 1");
+        KvAttendArgs a = kv_attend_args(memory, batch, q_heads, window, d_select ? n_select : 0);
         check_kv_dtype(dtype);
-        if (window >= (1ull << 31)) throw std::invalid_argument("kv attend: window must be below 2^31");
-        if (d_select && (a.batch.offsets || window)) throw std::invalid_argument("kv attend: selected tokens go with one new token per sequence and no window");
         if (a.batch.count == 0 || a.batch.tokens == 0) return (int)VDB_OK;
         check_kv_pointers(a.mem, a.batch);
         check_kv_rows(d_q, q_token_stride, q_head_stride, "queries");
@@ -1955,7 +1958,6 @@ int vdb_kv_attend_device(const vdb_kv_memory* memory, const vdb_kv_batch* batch,
         a.q_token = q_token_stride;
         a.q_head = q_head_stride;
         a.scale = scale;
-        a.window = (int64_t)window;
         a.select = d_select;
         a.out = d_out;
         a.lse = d_lse;

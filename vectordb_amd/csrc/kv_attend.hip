@@ -1050,17 +1050,17 @@ hipError_t launch_join(const KvAttendArgs& a, const Plan& plan, uint32_t rows, h
     return hipGetLastError();
 }
 
-// How a launch is cut, from what the host knows: the table's width (or the list's length, or the window) bounds the tokens.
+// How a launch is cut, from what the host knows (sizes only, so that the workspace asked for is the one used): the table's width (or the list's length, or the window) bounds the tokens.
 Plan plan_of(const KvAttendArgs& a, uint32_t max_new) {
     const uint32_t G = a.q_heads / a.mem.heads;
     Plan p{};
     p.max_new = max_new;
     p.splits = 1;
-    p.many = !a.select && (uint64_t)max_new * G / 192 * a.mem.heads * a.batch.count >= 128;
+    p.many = !a.n_select && (uint64_t)max_new * G / 192 * a.mem.heads * a.batch.count >= 128;
     if (p.many) return p;
     p.tiles = (uint32_t)std::min<uint64_t>(((uint64_t)max_new * G + 15) / 16, 65535);
-    uint64_t tokens = a.select ? a.n_select : (uint64_t)a.batch.table_width << a.mem.page_shift;
-    if (!a.select && a.window) tokens = std::min<uint64_t>(tokens, (uint64_t)a.window + max_new + 31);
+    uint64_t tokens = a.n_select ? a.n_select : (uint64_t)a.batch.table_width << a.mem.page_shift;
+    if (!a.n_select && a.window) tokens = std::min<uint64_t>(tokens, (uint64_t)a.window + max_new + 31);
     const uint64_t blocks = (uint64_t)p.tiles * a.mem.heads * a.batch.count;
     // As many ranges as give some 3072 blocks, four times what the chip holds at once: sequences of different lengths even out
     // (64 of 1 000 to 8 192 tokens, 8 heads: 147 us at 1024 blocks, 130 at 1536, 121 at 3072, 125 at 4096).  But no range
@@ -1068,10 +1068,10 @@ Plan plan_of(const KvAttendArgs& a, uint32_t max_new) {
     // in four 6.0 and 4.4 for the join; 2048 selected ones in two ranges 40 us, in four 46), and at most 384 of one row, or the
     // join counts (two sequences of 500 003: 384 ranges 103 + 10 us, 768 104 + 17, 256 109 + 8).
     const uint64_t want = std::min<uint64_t>(384, std::max<uint64_t>(1, 3072 / blocks));
-    uint64_t chunk = std::max<uint64_t>(a.select ? 1024 : 512, (tokens + want - 1) / want);
+    uint64_t chunk = std::max<uint64_t>(a.n_select ? 1024 : 512, (tokens + want - 1) / want);
     chunk = (chunk + 127) / 128 * 128;
     p.chunk = (uint32_t)std::min<uint64_t>(chunk, 1u << 30);
-    p.splits = (uint32_t)((tokens + p.chunk - 1) / p.chunk);
+    p.splits = (uint32_t)std::max<uint64_t>(1, (tokens + p.chunk - 1) / p.chunk);
     return p;
 }
 

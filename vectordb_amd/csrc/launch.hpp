@@ -208,7 +208,7 @@ struct KvAttendArgs {
     float scale;
     int64_t window;         // 0: all
     const int64_t* select;  // [count][heads][n_select] token numbers, nullptr: every token
-    uint32_t n_select;
+    uint32_t n_select;      // 0 without select
     void* out;   // [tokens][q_heads][dim]
     float* lse;  // [tokens][q_heads], or nullptr
 };

@@ -7,14 +7,17 @@ it reads all of them.  Everything runs on CUDA tensors and on torch's current st
 (include/vdb_index.h, vdb_kv_*)."""
 from __future__ import annotations
 
-import ctypes as C
+import torch
 
 from . import _lib
-from ._lib import KvBatchStruct, KvMemoryStruct, check
+from ._lib import KvBatchStruct, KvMemoryStruct
 from .rows4 import dtype_code, on_device
 
 
-def _rows(x, what: str):
+_needs = {}  # bytes of workspace by the sizes of a call
+
+
+def _rows(x):
     """x [tokens, heads, dim], or a copy of it, as the kernels read it: heads of contiguous numbers, 16-byte steps."""
     s = x.stride()
     if s[2] != 1 or s[0] % 8 or s[1] % 8 or s[0] < 0 or s[1] < 0 or x.data_ptr() % 16:
@@ -33,8 +36,6 @@ class KeyValueMemory:
     tokens, the new ones of the call included, for ``append`` and ``attend`` alike."""
 
     def __init__(self, pages: int, page_tokens: int, kv_heads: int, head_dim: int, device="cuda"):
-        import torch
-
         code = lambda: torch.zeros((pages, kv_heads, page_tokens, head_dim), dtype=torch.uint8, device=device).view(torch.float8_e4m3fn)  # noqa: E731
         scale = lambda: torch.ones((pages, kv_heads), dtype=torch.float32, device=device)  # noqa: E731
         self._take(code(), code(), scale(), scale())
@@ -47,8 +48,6 @@ class KeyValueMemory:
         return self
 
     def _take(self, k, v, k_scale, v_scale):
-        import torch
-
         if k.dim() != 4 or k.shape != v.shape or k_scale.shape != k.shape[:2] or v_scale.shape != k.shape[:2]:
             raise ValueError("expected k, v [pages, kv_heads, page_tokens, head_dim] and k_scale, v_scale [pages, kv_heads]")
         if k.dtype != torch.float8_e4m3fn or v.dtype != torch.float8_e4m3fn or k_scale.dtype != torch.float32 or v_scale.dtype != torch.float32:
@@ -70,8 +69,6 @@ class KeyValueMemory:
         self._m = KvMemoryStruct(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), pages, heads, page_tokens, dim)
 
     def _batch(self, table, lengths, offsets, max_new, tokens):
-        import torch
-
         n = lengths.shape[0]
         if table.dtype != torch.int32 or lengths.dtype != torch.int32 or table.dim() != 2 or lengths.dim() != 1 or table.shape[0] != n:
             raise ValueError("table [sequences, width] and lengths [sequences]: int32")
@@ -95,8 +92,6 @@ class KeyValueMemory:
         are its last ones (at most ``max_new`` of any sequence; by default all rows).  ``cos``, ``sin`` [positions, half]
         float32 turn the first 2 * half numbers of each key by its position's angles, in pairs (d, d + half), or (2 i, 2 i + 1)
         if ``interleaved``.  Returns ``queries`` [tokens, q_heads, head_dim], turned likewise (rows of no sequence: copied; None without queries)."""
-        import torch
-
         self._check_rows(k, self.kv_heads, "k")
         t = dtype_code(k, "k")
         if v.shape != k.shape or v.dtype != k.dtype or v.device != k.device:
@@ -112,7 +107,7 @@ class KeyValueMemory:
             if cos.device != self.device or sin.device != self.device or not (cos.is_contiguous() and sin.is_contiguous()):
                 raise ValueError(f"cos and sin: contiguous, on {self.device}")
             positions, rot = cos.shape[0], 2 * cos.shape[1]
-        k, v = _rows(k, "k"), _rows(v, "v")
+        k, v = _rows(k), _rows(v)
         q = out = None
         if queries is not None:
             self._check_rows(queries, None, "queries")
@@ -120,14 +115,12 @@ class KeyValueMemory:
                 raise ValueError(f"queries: [{tokens}, q_heads, {self.head_dim}] {k.dtype}")
             out = queries
             if rot:
-                q = _rows(queries, "queries")
+                q = _rows(queries)
                 out = torch.empty_like(q, memory_format=torch.contiguous_format)
-        with on_device(self.device) as stream:
-            check(self._l.vdb_kv_append_device(self._m, batch, t, k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1),
-                                               None if cos is None else cos.data_ptr(), None if sin is None else sin.data_ptr(), positions, rot,
-                                               interleaved, None if q is None else q.data_ptr(), 0 if q is None else q.stride(0),
-                                               0 if q is None else q.stride(1), 0 if q is None else q.shape[1],
-                                               None if q is None else out.data_ptr(), stream))
+        ks, vs, qs = k.stride(), v.stride(), (0, 0) if q is None else q.stride()
+        on_device(self.device, self._l.vdb_kv_append_device, self._m, batch, t, k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1],
+                  cos.data_ptr() if rot else None, sin.data_ptr() if rot else None, positions, rot, interleaved,
+                  None if q is None else q.data_ptr(), qs[0], qs[1], 0 if q is None else q.shape[1], None if q is None else out.data_ptr())
         return out
 
     def attend(self, q, table, lengths, *, offsets=None, max_new=None, scale=None, window: int = 0, select=None, return_lse: bool = False):
@@ -138,8 +131,6 @@ class KeyValueMemory:
         them; with ``select`` [sequences, kv_heads, n] int64 (one new token per sequence) it sees the tokens with these
         numbers, each as often as listed; numbers outside the sequence are skipped, as a search's padding is.
         ``scale`` is 1 / sqrt(head_dim) unless given."""
-        import torch
-
         self._check_rows(q, None, "q")
         t = dtype_code(q, "q")
         tokens, q_heads, dim = q.shape
@@ -158,16 +149,20 @@ class KeyValueMemory:
             n_select = select.shape[2]
             if n_select == 0:  # nothing to see: a list of one number that no sequence has
                 select, n_select = torch.full((tokens, self.kv_heads, 1), -1, dtype=torch.int64, device=self.device), 1
-        q = _rows(q, "q")
+        q = _rows(q)
         # rows of no sequence are zeros
         make = torch.empty if offsets is None else torch.zeros
         out = make((tokens, q_heads, dim), dtype=q.dtype, device=self.device)
         lse = make((tokens, q_heads), dtype=torch.float32, device=self.device) if return_lse else None
-        need = self._l.vdb_kv_attend_workspace(self._m, batch, q_heads, n_select)
+        sizes = (self.kv_heads, self.page_tokens, dim, batch.count, batch.table_width, tokens, batch.max_new, offsets is None, q_heads, window, n_select)
+        need = _needs.get(sizes)
+        if need is None:
+            if len(_needs) > 10000:
+                _needs.clear()
+            need = _needs[sizes] = self._l.vdb_kv_attend_workspace(self._m, batch, q_heads, window, n_select)
         work = torch.empty(need, dtype=torch.uint8, device=self.device) if need else None
-        with on_device(self.device) as stream:
-            check(self._l.vdb_kv_attend_device(self._m, batch, t, q.data_ptr(), q.stride(0), q.stride(1), q_heads,
-                                               float(dim) ** -0.5 if scale is None else float(scale), window,
-                                               None if select is None else select.data_ptr(), n_select, out.data_ptr(),
-                                               None if lse is None else lse.data_ptr(), None if work is None else work.data_ptr(), need, stream))
+        qs = q.stride()
+        on_device(self.device, self._l.vdb_kv_attend_device, self._m, batch, t, q.data_ptr(), qs[0], qs[1], q_heads,
+                  float(dim) ** -0.5 if scale is None else float(scale), window, None if select is None else select.data_ptr(), n_select,
+                  out.data_ptr(), None if lse is None else lse.data_ptr(), None if work is None else work.data_ptr(), need)
         return (out, lse) if return_lse else out

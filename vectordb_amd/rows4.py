@@ -5,46 +5,33 @@ candidates by, or the scores themselves where that precision will do.  Everythin
 current stream of their device (include/vdb_index.h, vdb_rows4_*)."""
 from __future__ import annotations
 
+import torch
+
 from . import _lib
 from ._lib import BF16, F16, F32, check
 
-
-_codes = {}
+_codes = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
 
 
 def dtype_code(t, what: str) -> int:
-    if not _codes:
-        import torch
-
-        _codes.update({torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16})
     code = _codes.get(t.dtype)
     if code is None:
         raise ValueError(f"{what}: float32, float16 or bfloat16, got {t.dtype}")
     return code
 
 
-class on_device:
-    """Makes a tensor's device current for the call, and gives its current stream (as a number: torch.cuda.current_stream,
-    which makes an object of it, costs the host 7 us)."""
-
-    __slots__ = ("index", "prev")
-
-    def __init__(self, device):
-        self.index = device.index
-
-    def __enter__(self):
-        import torch
-
-        self.prev = torch._C._cuda_getDevice()
-        if self.prev != self.index:
-            torch.cuda.set_device(self.index)
-        return torch._C._cuda_getCurrentRawStream(self.index)
-
-    def __exit__(self, *exc):
-        if self.prev != self.index:
-            import torch
-
-            torch.cuda.set_device(self.prev)
+def on_device(device, call, *args) -> None:
+    """Calls ``call(*args, stream)`` with ``device`` current, on torch's current stream of it (as a number:
+    torch.cuda.current_stream, which makes an object of it, costs the host 7 us a call)."""
+    index, current = device.index, torch._C._cuda_getDevice()
+    if current == index:
+        check(call(*args, torch._C._cuda_getCurrentRawStream(index)))
+        return
+    torch.cuda.set_device(index)
+    try:
+        check(call(*args, torch._C._cuda_getCurrentRawStream(index)))
+    finally:
+        torch.cuda.set_device(current)
 
 
 class Rows4:
@@ -52,8 +39,6 @@ class Rows4:
     layout that include/vdb_index.h describes: e2m1 codes, a power-of-two scale for every 32 columns of a row."""
 
     def __init__(self, codes, scales, dim: int):
-        import torch
-
         groups = (int(dim) + 31) // 32
         if dim < 1:
             raise ValueError("dim must be positive")
@@ -69,8 +54,6 @@ class Rows4:
     @classmethod
     def pack(cls, rows) -> "Rows4":
         """Rounds rows [n, dim] (float32, float16 or bfloat16) to 4 bits."""
-        import torch
-
         if not rows.is_cuda or rows.dim() != 2:
             raise ValueError("rows: a CUDA tensor [n, dim]")
         t = dtype_code(rows, "rows")
@@ -80,8 +63,7 @@ class Rows4:
         groups = (dim + 31) // 32
         out = cls(torch.empty((n, groups * 16), dtype=torch.uint8, device=rows.device),
                   torch.empty((n, groups), dtype=torch.uint8, device=rows.device), dim)
-        with on_device(rows.device) as stream:
-            check(out._l.vdb_rows4_pack_device(rows.data_ptr(), t, n, dim, rows.stride(0), out.codes.data_ptr(), out.scales.data_ptr(), stream))
+        on_device(rows.device, out._l.vdb_rows4_pack_device, rows.data_ptr(), t, n, dim, rows.stride(0), out.codes.data_ptr(), out.scales.data_ptr())
         return out
 
     def __len__(self) -> int:
@@ -89,17 +71,12 @@ class Rows4:
 
     def unpack(self):
         """The values that the codes stand for, [n, dim] float32."""
-        import torch
-
         out = torch.empty((len(self), self.dim), dtype=torch.float32, device=self.codes.device)
-        with on_device(out.device) as stream:
-            check(self._l.vdb_rows4_unpack_device(self.codes.data_ptr(), self.scales.data_ptr(), len(self), self.dim, out.data_ptr(), stream))
+        on_device(out.device, self._l.vdb_rows4_unpack_device, self.codes.data_ptr(), self.scales.data_ptr(), len(self), self.dim, out.data_ptr())
         return out
 
     def products(self, queries, out=None):
         """Inner products of queries [nq, dim] (or [dim]) with every row: [nq, n] (or [n]) float32, into ``out`` if given."""
-        import torch
-
         x = queries if queries.dim() == 2 else queries.unsqueeze(0)
         if queries.dim() not in (1, 2) or x.shape[1] != self.dim or x.device != self.codes.device:
             raise ValueError(f"expected queries [nq, {self.dim}] on {self.codes.device}, got {tuple(queries.shape)} on {queries.device}")
@@ -111,7 +88,6 @@ class Rows4:
             out = torch.empty((nq, n) if queries.dim() == 2 else (n,), dtype=torch.float32, device=x.device)
         elif out.dtype != torch.float32 or out.device != x.device or out.numel() != nq * n or not out.is_contiguous():
             raise ValueError(f"out: a contiguous float32 tensor of {nq} x {n} on {x.device}")
-        with on_device(x.device) as stream:
-            check(self._l.vdb_rows4_products_device(self.codes.data_ptr(), self.scales.data_ptr(), n, self.dim, x.data_ptr(), t, nq, x.stride(0),
-                                                    out.data_ptr(), stream))
+        on_device(x.device, self._l.vdb_rows4_products_device, self.codes.data_ptr(), self.scales.data_ptr(), n, self.dim, x.data_ptr(), t, nq, x.stride(0),
+                  out.data_ptr())
         return out

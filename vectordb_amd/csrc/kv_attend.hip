@@ -35,6 +35,19 @@ struct Parts {
 
 // 8 codes (two words) -> 8 elements of the type that scores are computed in
 template <bool HALF>
+__device__ __forceinline__ u32x2 widen4(uint32_t x) {
+    u32x2 r;
+    if constexpr (HALF) {
+        r[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(x, 1.0f, false));
+        r[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(x, 1.0f, true));
+    } else {
+        r[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x, 1.0f, false));
+        r[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x, 1.0f, true));
+    }
+    return r;
+}
+
+template <bool HALF>
 __device__ __forceinline__ u32x4 widen(uint32_t lo, uint32_t hi) {
     u32x4 r;
     if constexpr (HALF) {
@@ -537,43 +550,114 @@ __global__ __launch_bounds__(256, attend_waves(T, DS, MODE)) void kv_attend(KvAt
 
 // ---- many rows: chunks of prompts ---------------------------------------------------------------------
 //
-// Four waves of NT tiles of 16 rows go through the tokens together, 64 at a time.  What bounds this is, next to the matrix
-// units (256 cycles for 32 tokens x 16 rows at 128 dimensions), the softmax on the vector units (about as long: an exp2 costs
-// four instructions) and the reads of LDS; so
+// Four or eight waves of NT tiles of 16 rows go through the tokens together, 64 at a time.  What bounds this is, next to the
+// matrix units (256 cycles for 32 tokens x 16 rows at 128 dimensions), the softmax on the vector units (about as long: an exp2
+// costs four instructions) and the reads of LDS; so
 //   - codes are widened to bf16 (f16) once per block, into LDS in the order in which lanes hold matrix operands; a wave uses
 //     each operand it reads for its NT row tiles;
 //   - the scale of a page's values is folded into the exponent: w = exp2(score + log2 v_scale - M) with M the running
 //     maximum of just that, and the softmax's sum takes w / v_scale; so a score costs one fma, one exp2, one add;
 //   - the loads of the tile after next are under way while one is computed and the next is being widened.
+// Measured: four chunks of 30 to 2048 tokens, the longest sequence 6 000, 32 heads on 8, 128 dimensions, bf16: 325 us (matrix products alone 182).
 template <int T, int DS>
 struct Many {
-    static constexpr int NT = T == kF32 || DS > 6 ? 1 : 2;
-    static constexpr int rows = 4 * NT * 16;
+    static constexpr int NT = T == kF32 || DS > 5 ? 1 : 2;  // (192 dimensions: 511 us with one, 627 with two; 160: 473, 380)
+    // Two blocks of four waves or one of eight a CU (waves of one block wait for each other, but it widens its tokens for twice
+    // the rows).  Four: 32 dimensions 166 us against 193, 64 202 against 228, 128 in f16 428 against 454, in f32 642 against 695;
+    // eight: 96 261 against 297, 128 in bf16 325 against 339, 160 380 against 640, 256 611 against 1014, but in f32 1990 against 1609,
+    // where three parts of the queries would not fit the registers.
+    static constexpr bool four = DS <= 2 || (T != kBF16 && DS == 4) || (T == kF32 && DS > 6);
+    static constexpr int kThreads = four ? 256 : 512, occupancy = DS <= 2 ? 3 : DS > 6 && four ? 1 : 2;  // occupancy: waves a SIMD
+    static constexpr int rows = kThreads / 64 * NT * 16;
     static constexpr int D = DS * 32, ND = DS * 2;
     static constexpr int side = 64 * D * 2;                // bytes of 64 keys (or values) in bf16
-    static constexpr size_t lds = 4 * side + 64;           // two buffers of both, and of the scales of four pages each
-    static constexpr int units = (D * 2 + 255) / 256;      // (8 tokens x 4 dimensions) of values a thread widens; D * 2 units in all
-    static constexpr int pieces = (D * 4 + 255) / 256;     // 16-byte pieces of keys a thread widens; D * 4 in all
+    static constexpr size_t lds = 4 * side + 80;           // two buffers of both, of the scales of four pages each, and of a tile's number
+    static constexpr int units = (D * 4 + kThreads - 1) / kThreads;  // 16 bytes of keys, and 4 tokens x 4 dimensions of values, that a thread widens; D * 4 of each in all
 };
 
+// Which rows a block takes.  An item is `rows` rows of one sequence (for one head); its cost is the number of tokens that its last
+// row sees.  Items go to the blocks by falling cost, over all sequences: blocks start in the order of their numbers, so the
+// long ones are under way first and the short ones fill up the end.  (Found by every wave for itself: 4 us a block.)
+struct Items {
+    Sequence mine;  // sequence `lane`
+    int32_t seen;   // tokens that its last row sees
+    int32_t items;
+
+    __device__ __forceinline__ Items(const KvAttendArgs& a, int lane, uint32_t G, uint32_t rows) {
+        mine.n_new = mine.start = mine.len = seen = items = 0;
+        mine.first = 0;
+        if ((uint32_t)lane < a.batch.count && sequence_of(a, lane, mine)) {
+            seen = (int32_t)min((int64_t)mine.len, a.window == 0 ? (int64_t)0x7FFFFFFF : a.window + rows);
+            items = (int32_t)(((uint64_t)mine.n_new * G + rows - 1) / rows);
+        } else {
+            mine.n_new = 0;
+        }
+    }
+    // items of sequence b that see at least `tokens`
+    __device__ __forceinline__ int32_t at_least(int b, int64_t tokens, uint32_t G, uint32_t rows) const {
+        const int32_t n = __builtin_amdgcn_readlane(items, b);
+        const uint64_t before = (uint64_t)max(tokens - 1 - __builtin_amdgcn_readlane(mine.start, b), (int64_t)0) * G / rows;
+        return tokens > __builtin_amdgcn_readlane(seen, b) ? 0 : n - (int32_t)min(before, (uint64_t)max(n - 1, 0));
+    }
+    // Item k by falling cost (in steps of 64 tokens): 64 costs are looked at at once, one a lane.
+    __device__ __forceinline__ bool find(uint32_t count, int lane, int64_t k, uint32_t G, uint32_t rows, Sequence& s, uint32_t& b, int32_t& block) const {
+        int32_t most = 0;
+        int64_t all = 0;
+        for (uint32_t i = 0; i < count; ++i) most = max(most, __builtin_amdgcn_readlane(seen, i)), all += __builtin_amdgcn_readlane(items, i);
+        if (k >= all) return false;
+        int32_t lo = 0, end = most / 64 + 1;
+        while (end - lo > 1) {
+            const int32_t step = (end - lo + 63) / 64;
+            const int64_t here = lo + (int64_t)lane * step;
+            int64_t n = 0;
+            for (uint32_t i = 0; i < count; ++i) n += at_least(i, here * 64, G, rows);
+            const uint64_t yes = __ballot(here < end && n > k);  // lane 0 always
+            lo += (63 - __builtin_clzll(yes)) * step;
+            end = min(end, lo + step);
+        }
+        // those of that cost, sequence by sequence
+        for (uint32_t i = 0; i < count; ++i) k -= at_least(i, (int64_t)(lo + 1) * 64, G, rows);
+        for (b = 0; b < count; ++b) {
+            const int32_t more = at_least(b, (int64_t)(lo + 1) * 64, G, rows), here = at_least(b, (int64_t)lo * 64, G, rows) - more;
+            if (k < here) {
+                block = __builtin_amdgcn_readlane(items, b) - more - 1 - (int32_t)k;
+                s.first = (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int32_t)(mine.first >> 32), b) << 32 | (uint32_t)__builtin_amdgcn_readlane((int32_t)mine.first, b));
+                s.n_new = __builtin_amdgcn_readlane(mine.n_new, b);
+                s.start = __builtin_amdgcn_readlane(mine.start, b);
+                s.len = __builtin_amdgcn_readlane(mine.len, b);
+                return true;
+            }
+            k -= here;
+        }
+        return false;
+    }
+};
+
+// x, but computed where it is used: what follows from it is not kept in registers through the loops.
+__device__ __forceinline__ int fresh(int x) {
+    asm volatile("" : "+v"(x));
+    return x;
+}
+
+// x is computed here, and not moved to where it is next used (with all that it is computed from).
+__device__ __forceinline__ void keep(float& x) { asm volatile("" : "+v"(x)); }
+
 template <int T, int DS>
-__global__ __launch_bounds__(256, DS <= 4 ? 2 : 1) void kv_attend_many(KvAttendArgs a) {
+__global__ __launch_bounds__((Many<T, DS>::kThreads), (Many<T, DS>::occupancy)) void kv_attend_many(KvAttendArgs a) {
     typedef Many<T, DS> M;
     constexpr bool HALF = T == kF16;
     constexpr int NQ = T == kF32 ? 3 : 1, NP = Parts<T>::value, D = M::D, ND = M::ND, NT = M::NT, side = M::side;
     extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int m = lane & 15, q4 = lane >> 4;
-    const uint32_t H = a.mem.heads, b = blockIdx.z, head = blockIdx.x % H, P = a.mem.page_tokens, G = a.q_heads / H;
-    Sequence s;
-    if (!sequence_of(a, b, s)) return;
-    const int32_t* table = a.batch.table + (uint64_t)b * a.batch.table_width;
+    const uint32_t H = a.mem.heads, head = blockIdx.x % H, P = a.mem.page_tokens, G = a.q_heads / H;
     float* scales_s = (float*)(lds + 4 * side);  // [2][8]: of keys, of values
-    const int64_t rows = (int64_t)s.n_new * G;
     const uint8_t* kc = (const uint8_t*)a.mem.k;
     const uint8_t* vc = (const uint8_t*)a.mem.v;
     const float to_log2 = __builtin_fabsf(a.scale) * kLog2e;
     const uint32_t flip = a.scale < 0.0f ? (T == kF32 ? 0x80000000u : 0x80008000u) : 0u;  // the scale's sign goes into the queries
+    Sequence s;
+    const int32_t* table = nullptr;
     // Page numbers: 64 of them in a register of the wave, refilled every 64 pages.  (Scalar loads would do, but a wait for LDS is
     // a wait for them as well.)
     int32_t held = -1, held_from = 0;
@@ -590,30 +674,168 @@ __global__ __launch_bounds__(256, DS <= 4 ? 2 : 1) void kv_attend_many(KvAttendA
         return i32x4{page_of(kb), page_of(kb + 16), page_of(kb + 32), page_of(kb + 48)};
     };
 
-    // The last rows see the most tokens: they go first.  (All sequences' last rows before the others would even out better on paper,
-    // but neighbouring blocks go to other parts of the chip in turn, and four sequences then have one each: 785 us instead of 394;
-    // with the sequences rotated, 410.)
-    const int64_t nblocks = (rows + M::rows - 1) / M::rows;
-    for (int64_t rb = nblocks - 1 - blockIdx.x / H; rb >= 0; rb -= gridDim.x / H) {
-        const int64_t row0 = rb * M::rows, row1 = min(row0 + M::rows - 1, rows - 1);
-        const int32_t pos0 = s.start + (int32_t)(row0 / G), pos1 = s.start + (int32_t)(row1 / G);
+    const bool sorted = gridDim.z == 1;  // at most 64 sequences
+    for (int64_t k = blockIdx.x / H;; k += gridDim.x / H) {
+        uint32_t b = blockIdx.z;
+        int32_t rb = 0;
+        if (sorted) {
+            if (!Items(a, lane, G, M::rows).find(a.batch.count, lane, k, G, M::rows, s, b, rb)) break;
+        } else {
+            if (!sequence_of(a, b, s)) break;
+            const int64_t n = ((int64_t)s.n_new * G + M::rows - 1) / M::rows;
+            if (k >= n) break;
+            rb = (int32_t)(n - 1 - k);
+        }
+        const int64_t rows = (int64_t)s.n_new * G;
+        table = a.batch.table + (uint64_t)b * a.batch.table_width;
+        const int64_t row0 = (int64_t)rb * M::rows;
+        const int32_t here = (int32_t)min(rows - row0, (int64_t)M::rows);  // rows of the item
+        const int32_t tok0 = (int32_t)(row0 / G);
+        const uint32_t qh0 = (uint32_t)(row0 - (int64_t)tok0 * G);
+        auto token = [&](int32_t r) { return tok0 + (int32_t)((qh0 + r) / G); };             // of row r of the item
+        auto q_head = [&](int32_t r) { return head * G + (qh0 + r) % G; };
+        const int32_t pos0 = s.start + tok0, pos1 = s.start + token(here - 1);
         int32_t lo, hi;
         range_of<false>(a, s, pos0, pos1, lo, hi);
         // this wave's rows
-        const int64_t wrow0 = row0 + wave * NT * 16, wrow1 = min(wrow0 + NT * 16 - 1, rows - 1);
-        const bool idle = wrow0 >= rows;
-        const int32_t wpos0 = s.start + (int32_t)(min(wrow0, rows - 1) / G), wpos1 = s.start + (int32_t)(wrow1 / G);
+        const int32_t wrow0 = wave * NT * 16;
+        const bool idle = wrow0 >= here;
+        const int32_t wpos0 = s.start + token(min(wrow0, here - 1)), wpos1 = s.start + token(min(wrow0 + NT * 16, here) - 1);
         const int32_t w_lo = a.window == 0 ? 0 : (int32_t)max((int64_t)0, wpos0 - a.window + 1);
-        // the tokens [lo_all, hi_all) are seen by all rows of the block
+        // the tokens [lo_all, hi_all) are seen by all rows of the block, [w_lo_all, w_hi_all) by all of the wave
+        const int32_t w_lo_all = a.window == 0 ? 0 : (int32_t)max((int64_t)0, wpos1 - a.window + 1), w_hi_all = idle ? 0 : min(max(wpos0, -1) + 1, hi);
         const int32_t lo_all = a.window == 0 ? 0 : (int32_t)max((int64_t)0, pos1 - a.window + 1), hi_all = min(max(pos0, -1) + 1, hi);
+        f32x4 o[NT][ND];
+        float top[NT], sum[NT];
+#pragma unroll
+        for (int ct = 0; ct < NT; ++ct) {
+            top[ct] = wrow0 + ct * 16 + m < here ? kNone : -kNone, sum[ct] = 0.0f;  // (a row that does not exist has no weights)
+#pragma unroll
+            for (int d = 0; d < ND; ++d) o[ct][d] = f32x4{0, 0, 0, 0};
+        }
+
+        // Places in LDS, in bytes, apart from multiples of 1 KB (a matrix operand) that go into the instructions.  Operand rows are
+        // exchanged by j (keys) and d (values), so that the pieces that neighbouring threads write lie in different banks.
+        uint32_t key_at[4], value_at[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            key_at[j] = (q4 * 16 + (m ^ ((j * 2 + (q4 >> 1)) & 7))) * 16;
+            value_at[j] = side + (q4 * 16 + (m ^ j)) * 16;
+        }
+        // ---- staging: a thread widens `pieces` 16-byte pieces of keys, and `units` of 8 tokens x 4 dimensions of values
+        float scale_r = 1.0f;  // of threads 0-7
+        constexpr int kThreads = M::kThreads;
+        u32x4 kr[M::units];
+        uint32_t vr[M::units][4];
+        const uint64_t page_bytes = (uint64_t)H * P * D;
+        const uint8_t* const kh = kc + (uint64_t)head * P * D;
+        const uint8_t* const vh = vc + (uint64_t)head * P * D;
+        auto pick = [&](i32x4 pg, int i) { return i < 2 ? (i == 0 ? pg[0] : pg[1]) : (i == 2 ? pg[2] : pg[3]); };
+        auto load = [&](int32_t kb, i32x4 pg) {
+            if (tid < 8) {
+                const int32_t page = pick(pg, tid & 3);
+                scale_r = page >= 0 ? (tid < 4 ? a.mem.k_scale : a.mem.v_scale)[(int64_t)page * H + head] : 1.0f;
+            }
+#pragma unroll
+            for (int i = 0; i < M::units; ++i) {
+                const int piece = tid + i * kThreads;
+                if (D * 4 % kThreads == 0 || piece < D * 4) {
+                    const int tok = piece / (D / 16), c = piece % (D / 16);
+                    const uint32_t page = (uint32_t)max(pick(pg, tok >> 4), 0);
+                    kr[i] = *(const u32x4*)(kh + page * page_bytes + ((kb + tok) & (P - 1)) * (uint32_t)D + c * 16);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < M::units; ++i) {
+                const int unit = tid + i * kThreads;
+                if (D * 4 % kThreads == 0 || unit < D * 4) {
+                    const int grp = unit / (D / 4), c = unit % (D / 4);
+                    const uint32_t page = (uint32_t)max(pick(pg, grp >> 2), 0);
+                    const uint8_t* p = vh + page * page_bytes + ((kb + grp * 4) & (P - 1)) * (uint32_t)D + c * 4;
+#pragma unroll
+                    for (int t = 0; t < 4; ++t) vr[i][t] = *(const uint32_t*)(p + t * D);
+                }
+            }
+        };
+        // every row of the block sees every token of the tile
+        auto plain = [&](int32_t kb, i32x4 pg) {
+            return kb >= lo_all && kb + 64 <= hi_all && (pg[0] | pg[1] | pg[2] | pg[3]) >= 0;
+        };
+        auto plain_here = [&](int32_t kb, i32x4 pg) {  // of the wave
+            return kb >= w_lo_all && kb + 64 <= w_hi_all && (pg[0] | pg[1] | pg[2] | pg[3]) >= 0;
+        };
+        // What no row sees may hold anything: it is taken for zeros.  Of NaN among the rest, nan_s[] tells the tile's waves.
+        int32_t* nan_s = (int32_t*)(scales_s + 16);
+        auto hide = [&](int32_t kb, i32x4 pg, int buf) {
+            if (!plain(kb, pg)) {
+                uint32_t nan = 0;
+                const int tid = fresh((int)threadIdx.x);
+#pragma unroll
+                for (int i = 0; i < M::units; ++i) {
+                    const int grp = (tid + i * kThreads) / (D / 4), t0 = kb + grp * 4;
+                    const bool there = pick(pg, (grp >> 2) & 3) >= 0;
+#pragma unroll
+                    for (int t = 0; t < 4; ++t) {
+                        vr[i][t] = there && t0 + t >= lo && t0 + t < hi ? vr[i][t] : 0;
+                        if (D * 4 % kThreads == 0 || tid + i * kThreads < D * 4) nan |= nan_bytes(vr[i][t]);
+                    }
+                }
+                if (nan) nan_s[buf] = kb;
+            }
+        };
+        auto store_keys = [&](int buf) {
+            unsigned char* ks = lds + buf * 2 * side;
+            if (tid < 8) scales_s[buf * 8 + tid] = scale_r;
+#pragma unroll
+            for (int i = 0; i < M::units; ++i) {
+                const int piece = tid + i * kThreads;
+                if (D * 4 % kThreads == 0 || piece < D * 4) {
+                    // token x of 32: row (x >> 3) * 4 + (x & 3) of score tile (x >> 2) & 1.  Bytes 16 c .. + 15: quarters
+                    // 2 (c & 1), 2 (c & 1) + 1 of step c / 2.  Rows are exchanged by c, so that pieces of one token go to other banks.
+                    const int tok = piece / (D / 16), c = piece % (D / 16), x = tok & 31;
+                    const int tile = (tok >> 5) * 2 + (x >> 2 & 1), row = ((x >> 3) * 4 + (x & 3)) ^ (c & 7);
+                    unsigned char* w = ks + ((tile * DS + (c >> 1)) * 64 + (c & 1) * 32 + row) * 16;
+                    *(u32x4*)w = widen<HALF>(kr[i][0], kr[i][1]);
+                    *(u32x4*)(w + 256) = widen<HALF>(kr[i][2], kr[i][3]);
+                }
+            }
+        };
+        auto store_values = [&](int buf) {
+            unsigned char* vs = lds + buf * 2 * side + side;
+#pragma unroll
+            for (int i = 0; i < M::units; ++i) {
+                const int unit = tid + i * kThreads;
+                if (D * 4 % kThreads == 0 || unit < D * 4) {
+                    const int grp = unit / (D / 4), c = unit % (D / 4);
+                    uint32_t x[4];
+                    transpose4(vr[i], x);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int d = c * 4 + e, dt = d >> 4;
+                        *(u32x2*)(vs + ((dt * 2 + (grp >> 3)) * 64 + (grp >> 1 & 3) * 16 + ((d & 15) ^ (dt & 3))) * 16 + (grp & 1) * 8) = widen4<false>(x[e]);
+                    }
+                }
+            }
+        };
+
+        const int32_t kb0 = lo & ~63;
+        i32x4 pa, pb, pc;  // pages of this tile, of the next, of the one after it
+        if (kb0 < hi) {
+            held_from = -64;
+            pa = pages(kb0);
+            pb = pages(kb0 + 64);
+            pc = pages(kb0 + 128);
+            load(kb0, pa);
+        }
+        // (the queries travel beside the first tokens)
         u32x4 qf[NT][NQ][DS];
         int32_t pos[NT];
 #pragma unroll
         for (int ct = 0; ct < NT; ++ct) {
-            const int64_t r = wrow0 + ct * 16 + m;
-            const bool live = r < rows;
-            const int32_t tok = live ? (int32_t)(r / G) : 0;
-            const uint32_t qh = head * G + (live ? (uint32_t)(r - (int64_t)tok * G) : 0);
+            const int32_t r = wrow0 + ct * 16 + m;
+            const bool live = r < here;
+            const int32_t tok = live ? token(r) : 0;
+            const uint32_t qh = live ? q_head(r) : 0;
             pos[ct] = live ? s.start + tok : -1;
             const E<T>* q = (const E<T>*)a.q + (uint64_t)(s.first + tok) * a.q_token + (uint64_t)qh * a.q_head + q4 * 8;
 #pragma unroll
@@ -637,120 +859,10 @@ __global__ __launch_bounds__(256, DS <= 4 ? 2 : 1) void kv_attend_many(KvAttendA
                 }
             }
         }
-        f32x4 o[NT][ND];
-        float top[NT], sum[NT];
-#pragma unroll
-        for (int ct = 0; ct < NT; ++ct) {
-            top[ct] = wrow0 + ct * 16 + m < rows ? kNone : -kNone, sum[ct] = 0.0f;  // (a row that does not exist has no weights)
-#pragma unroll
-            for (int d = 0; d < ND; ++d) o[ct][d] = f32x4{0, 0, 0, 0};
-        }
-
-        // Places in LDS, in bytes, apart from multiples of 1 KB (a matrix operand) that go into the instructions.  Operand rows are
-        // exchanged by j (keys) and d (values), so that the pieces that neighbouring threads write lie in different banks.
-        uint32_t key_at[4], value_at[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            key_at[j] = (q4 * 16 + (m ^ ((j * 2 + (q4 >> 1)) & 7))) * 16;
-            value_at[j] = side + (q4 * 16 + (m ^ j)) * 16;
-        }
-        // ---- staging: a thread widens `pieces` 16-byte pieces of keys, and `units` of 8 tokens x 4 dimensions of values
-        float scale_r = 1.0f;  // of threads 0-7
-        u32x4 kr[M::pieces];
-        uint32_t vr[M::units][8];
-        const uint64_t page_bytes = (uint64_t)H * P * D;
-        const uint8_t* const kh = kc + (uint64_t)head * P * D;
-        const uint8_t* const vh = vc + (uint64_t)head * P * D;
-        auto pick = [&](i32x4 pg, int i) { return i < 2 ? (i == 0 ? pg[0] : pg[1]) : (i == 2 ? pg[2] : pg[3]); };
-        auto load = [&](int32_t kb, i32x4 pg) {
-            if (tid < 8) {
-                const int32_t page = pick(pg, tid & 3);
-                scale_r = page >= 0 ? (tid < 4 ? a.mem.k_scale : a.mem.v_scale)[(int64_t)page * H + head] : 1.0f;
-            }
-#pragma unroll
-            for (int i = 0; i < M::pieces; ++i) {
-                const int piece = tid + i * 256;
-                if (D * 4 % 256 == 0 || piece < D * 4) {
-                    const int tok = piece / (D / 16), c = piece % (D / 16);
-                    const uint32_t page = (uint32_t)max(pick(pg, tok >> 4), 0);
-                    kr[i] = *(const u32x4*)(kh + page * page_bytes + ((kb + tok) & (P - 1)) * (uint32_t)D + c * 16);
-                }
-            }
-#pragma unroll
-            for (int i = 0; i < M::units; ++i) {
-                const int unit = tid + i * 256;
-                if (D * 2 % 256 == 0 || unit < D * 2) {
-                    const int grp = unit / (D / 4), c = unit % (D / 4);
-                    const uint32_t page = (uint32_t)max(pick(pg, grp >> 1), 0);
-                    const uint8_t* p = vh + page * page_bytes + ((kb + grp * 8) & (P - 1)) * (uint32_t)D + c * 4;
-#pragma unroll
-                    for (int t = 0; t < 8; ++t) vr[i][t] = *(const uint32_t*)(p + t * D);
-                }
-            }
-        };
-        // every row of the block sees every token of the tile
-        auto plain = [&](int32_t kb, i32x4 pg) {
-            return kb >= lo_all && kb + 64 <= hi_all && (pg[0] | pg[1] | pg[2] | pg[3]) >= 0;
-        };
-        auto hide = [&](int32_t kb, i32x4 pg) {
-            if (!plain(kb, pg)) {  // what no row sees may hold anything: it is taken for zeros
-#pragma unroll
-                for (int i = 0; i < M::units; ++i) {
-                    const int grp = (tid + i * 256) / (D / 4), t0 = kb + grp * 8;
-                    const bool there = pick(pg, (grp >> 1) & 3) >= 0;
-#pragma unroll
-                    for (int t = 0; t < 8; ++t) {
-                        vr[i][t] = there && t0 + t >= lo && t0 + t < hi ? vr[i][t] : 0;
-                    }
-                }
-            }
-        };
-        auto store_keys = [&](int buf) {
-            unsigned char* ks = lds + buf * 2 * side;
-            if (tid < 8) scales_s[buf * 8 + tid] = scale_r;
-#pragma unroll
-            for (int i = 0; i < M::pieces; ++i) {
-                const int piece = tid + i * 256;
-                if (D * 4 % 256 == 0 || piece < D * 4) {
-                    // token x of 32: row (x >> 3) * 4 + (x & 3) of score tile (x >> 2) & 1.  Bytes 16 c .. + 15: quarters
-                    // 2 (c & 1), 2 (c & 1) + 1 of step c / 2.  Rows are exchanged by c, so that pieces of one token go to other banks.
-                    const int tok = piece / (D / 16), c = piece % (D / 16), x = tok & 31;
-                    const int tile = (tok >> 5) * 2 + (x >> 2 & 1), row = ((x >> 3) * 4 + (x & 3)) ^ (c & 7);
-                    unsigned char* w = ks + ((tile * DS + (c >> 1)) * 64 + (c & 1) * 32 + row) * 16;
-                    *(u32x4*)w = widen<HALF>(kr[i][0], kr[i][1]);
-                    *(u32x4*)(w + 256) = widen<HALF>(kr[i][2], kr[i][3]);
-                }
-            }
-        };
-        auto store_values = [&](int buf) {
-            unsigned char* vs = lds + buf * 2 * side + side;
-#pragma unroll
-            for (int i = 0; i < M::units; ++i) {
-                const int unit = tid + i * 256;
-                if (D * 2 % 256 == 0 || unit < D * 2) {
-                    const int grp = unit / (D / 4), c = unit % (D / 4);
-                    uint32_t x[4], y[4];
-                    transpose4(vr[i], x);
-                    transpose4(vr[i] + 4, y);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const int d = c * 4 + e, dt = d >> 4;
-                        *(u32x4*)(vs + ((dt * 2 + (grp >> 2)) * 64 + (grp & 3) * 16 + ((d & 15) ^ (dt & 3))) * 16) = widen<false>(x[e], y[e]);
-                    }
-                }
-            }
-        };
-
-        const int32_t kb0 = lo & ~63;
-        i32x4 pa, pb, pc;  // pages of this tile, of the next, of the one after it
-        __syncthreads();
+        if (tid < 2) nan_s[tid] = -1;
+        __syncthreads();  // (of the last rows, too, that all waves are done)
         if (kb0 < hi) {
-            held_from = -64;
-            pa = pages(kb0);
-            pb = pages(kb0 + 64);
-            pc = pages(kb0 + 128);
-            load(kb0, pa);
-            hide(kb0, pa);
+            hide(kb0, pa, 0);
             store_keys(0);
             store_values(0);
             if (kb0 + 64 < hi) load(kb0 + 64, pb);
@@ -758,123 +870,90 @@ __global__ __launch_bounds__(256, DS <= 4 ? 2 : 1) void kv_attend_many(KvAttendA
         __syncthreads();
         int32_t kb = kb0;
         int buf = 0;
-        // One tile.  FULL: every row of the block sees every token of it, and the running reference of the softmax stays what it
-        // is.  That need not be the maximum: no score is compared with another while the sums of the weights stay below 2^11.
-        // Where one does not (rarely: in the first tiles) the answer is false, nothing has been added up, and the tile is done
-        // again with FULL = false, which looks at every score and scales what there is.  (One loop that does both holds every
-        // output twice: 500 spilled bytes a lane and twice the time.)
-        auto compute = [&](auto is_full) -> bool {
-            constexpr bool FULL = decltype(is_full)::value;
-            const unsigned char* here = lds + buf * 2 * side;
-                float c[2], lv[2], inv[2];
+        float c[2], lv[2], inv[2];  // of the tile's pages: of the scores, log2 and inverse of the values' scale
+        auto read_scales = [&] {
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    c[h] = scales_s[buf * 8 + 2 * h + (q4 >> 1)] * to_log2;
-                    const float vs = __builtin_fmaxf(scales_s[buf * 8 + 4 + 2 * h + (q4 >> 1)], 0x1p-120f);
-                    lv[h] = __builtin_amdgcn_logf(vs), inv[h] = __builtin_amdgcn_rcpf(vs);
+            for (int h = 0; h < 2; ++h) {
+                c[h] = scales_s[buf * 8 + 2 * h + (q4 >> 1)] * to_log2;
+                const float vs = __builtin_fmaxf(scales_s[buf * 8 + 4 + 2 * h + (q4 >> 1)], 0x1p-120f);
+                lv[h] = __builtin_amdgcn_logf(vs), inv[h] = __builtin_amdgcn_rcpf(vs);
+            }
+        };
+        u32x4 ring[4];  // operands are read three products ahead
+        auto read_key = [&](int e) { ring[e & 3] = *(const u32x4*)(lds + buf * 2 * side + key_at[e % DS & 3] + e * 1024); };
+        auto read_value = [&](int e) { ring[e & 3] = *(const u32x4*)(lds + buf * 2 * side + value_at[e % ND & 3] + (e % ND * 2 + e / ND) * 1024); };
+        auto pack_weights = [&](float p, float r, u32x4 (&w)[NP], int t) {
+#pragma unroll
+            for (int n = 0; n < NP; ++n) {
+                if constexpr (NP == 1) {
+                    bf16x2 x = {(__bf16)p, (__bf16)r};
+                    w[n][t] = __builtin_bit_cast(uint32_t, x);
+                } else {
+                    w[n][t] = pack_hi16(bf16_part(p, n), bf16_part(r, n));
                 }
-                    // scores: operands are read three products ahead; the next tile is widened beside them
-                    f32x4 sc[2][NT][2];
-                    u32x4 kf[4];
-                    auto read_key = [&](int e) { kf[e & 3] = *(const u32x4*)(here + key_at[e % DS & 3] + e * 1024); };
+            }
+        };
+        // A tile at an edge, the first ones, and where the softmax's reference has to move: 32 tokens at a time, so that the scores
+        // take no more registers than in the other loop.
+        auto careful = [&] {
+            read_scales();
+            const bool nan_here = __builtin_amdgcn_readfirstlane(nan_s[buf]) == kb;
 #pragma unroll
-                    for (int e = 0; e < 3 && e < 4 * DS; ++e) read_key(e);
+            for (int h = 0; h < 2; ++h) {
+                f32x4 sc[NT][2];
 #pragma unroll
-                    for (int e = 0; e < 4 * DS; ++e) {
-                        const int i = e / DS, j = e % DS;
-                        if (e + 3 < 4 * DS) read_key(e + 3);
-                        if (e == DS) store_keys(buf ^ 1);
-                        if (e == 2 * DS) store_values(buf ^ 1);
+                for (int e = 0; e < 3 && e < 2 * DS; ++e) read_key(h * 2 * DS + e);
 #pragma unroll
-                        for (int ct = 0; ct < NT; ++ct) {
-                            if (j == 0) sc[i >> 1][ct][i & 1] = f32x4{0, 0, 0, 0};
-#pragma unroll
-                            for (int n = 0; n < NQ; ++n) sc[i >> 1][ct][i & 1] = mfma<HALF>(kf[e & 3], qf[ct][n][j], sc[i >> 1][ct][i & 1]);
-                        }
-                        if (j == DS - 1) __builtin_amdgcn_sched_barrier(0);
-                    }
-                    uint32_t seen[2][NT];
-                    if constexpr (!FULL) {
-                        const int32_t lowest = a.window == 0 ? -1 : (int32_t)min(a.window, (int64_t)0x7FFFFFFF);
-#pragma unroll
-                        for (int h = 0; h < 2; ++h)
-#pragma unroll
-                            for (int ct = 0; ct < NT; ++ct) {
-                                seen[h][ct] = 0;
-                                const int32_t first = kb + h * 32 + q4 * 8, end = min(pos[ct], s.len - 1);
-                                const bool there = (q4 < 2 ? pa[2 * h] : pa[2 * h + 1]) >= 0;
-#pragma unroll
-                                for (int t = 0; t < 8; ++t) {
-                                    // (a position is at least -2^31 + 1 and a token at least 0: their difference, taken only where the token is not after the position, fits)
-                                    const bool see = there && first + t <= end && (lowest < 0 || pos[ct] - (first + t) < lowest);
-                                    seen[h][ct] |= (see ? 1u : 0u) << t;
-                                    sc[h][ct][t >> 2][t & 3] = see ? __builtin_fmaf(sc[h][ct][t >> 2][t & 3], c[h], lv[h]) : -__builtin_inff();
-                                }
-                            }
-#pragma unroll
-                        for (int ct = 0; ct < NT; ++ct) {
-                            float now = top[ct];
-#pragma unroll
-                            for (int h = 0; h < 2; ++h)
-#pragma unroll
-                                for (int t = 0; t < 8; ++t) now = __builtin_fmaxf(now, sc[h][ct][t >> 2][t & 3]);
-                            now = max_of_quarters(now);
-                            const float shrink = __builtin_amdgcn_exp2f(top[ct] - now);
-                            top[ct] = now;
-                            sum[ct] *= shrink;
-#pragma unroll
-                            for (int d = 0; d < ND; ++d) o[ct][d] *= shrink;
-                        }
-                    }
-                    u32x4 pf[2][NT][NP];
-                    float more[NT];
-                    bool over = false;
+                for (int e = 0; e < 2 * DS; ++e) {
+                    if (e + 3 < 2 * DS) read_key(h * 2 * DS + e + 3);
 #pragma unroll
                     for (int ct = 0; ct < NT; ++ct) {
-                        more[ct] = 0.0f;
+                        if (e % DS == 0) sc[ct][e / DS] = f32x4{0, 0, 0, 0};
 #pragma unroll
-                        for (int h = 0; h < 2; ++h) {
-                            const float off = FULL ? lv[h] - top[ct] : -top[ct];
-                            float p[8];
-#pragma unroll
-                            for (int t = 0; t < 8; ++t) {
-                                const float x = sc[h][ct][t >> 2][t & 3];
-                                p[t] = __builtin_amdgcn_exp2f(FULL ? __builtin_fmaf(x, c[h], off) : x + off);
-                            }
-                            const float part = ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
-                            over |= part > 2048.0f;
-                            more[ct] = __builtin_fmaf(part, inv[h], more[ct]);
-#pragma unroll
-                            for (int n = 0; n < NP; ++n)
-#pragma unroll
-                                for (int t = 0; t < 4; ++t) {
-                                    if constexpr (NP == 1) {
-                                        bf16x2 w = {(__bf16)p[2 * t], (__bf16)p[2 * t + 1]};
-                                        pf[h][ct][n][t] = __builtin_bit_cast(uint32_t, w);
-                                    } else {
-                                        pf[h][ct][n][t] = pack_hi16(bf16_part(p[2 * t], n), bf16_part(p[2 * t + 1], n));
-                                    }
-                                }
-                            __builtin_amdgcn_sched_barrier(0);
-                        }
+                        for (int n = 0; n < NQ; ++n) sc[ct][e / DS] = mfma<HALF>(ring[(h * 2 * DS + e) & 3], qf[ct][n][e % DS], sc[ct][e / DS]);
                     }
-                    if (FULL && __any(over)) return false;
+                }
+                __builtin_amdgcn_sched_barrier(0);
+                u32x4 pf[NT][NP];
+                uint32_t seen[NT];
 #pragma unroll
-                    for (int ct = 0; ct < NT; ++ct) sum[ct] += more[ct];
-                    if (kb + 128 < hi) load(kb + 128, pc);
-                    // values: likewise
-                    u32x4 vf[4];
-                    auto read_value = [&](int e) { vf[e & 3] = *(const u32x4*)(here + value_at[e % ND & 3] + (e % ND * 2 + e / ND) * 1024); };
+                for (int ct = 0; ct < NT; ++ct) {
+                    // the row sees the tokens first + [from, to) of the lane's 8 (a window reaches below 0 by 2^63 at most)
+                    const int32_t first = kb + h * 32 + (fresh(lane) >> 4) * 8, at = fresh(pos[ct]);
+                    const bool there = (q4 < 2 ? pa[2 * h] : pa[2 * h + 1]) >= 0;
+                    const int64_t least = a.window == 0 ? 0 : (int64_t)at - a.window + 1;
+                    const int32_t to = there ? min(max(min(at, s.len - 1) + 1 - first, 0), 8) : 0;
+                    const int32_t from = (int32_t)min(max(least - first, (int64_t)0), (int64_t)8);
+                    seen[ct] = ((1u << to) - 1) & ~((1u << from) - 1);
+                    float now = top[ct], p[8];
 #pragma unroll
-                    for (int e = 0; e < 3; ++e) read_value(e);
+                    for (int t = 0; t < 8; ++t) {
+                        p[t] = seen[ct] >> t & 1 ? __builtin_fmaf(sc[ct][t >> 2][t & 3], c[h], lv[h]) : -__builtin_inff();
+                        now = __builtin_fmaxf(now, p[t]);
+                    }
+                    now = max_of_quarters(now);
+                    const float shrink = __builtin_amdgcn_exp2f(top[ct] - now);
+                    top[ct] = now;
 #pragma unroll
-                    for (int e = 0; e < 2 * ND; ++e) {
-                        const int h = e / ND, d = e % ND;
-                        if (e + 3 < 2 * ND) read_value(e + 3);
-                        u32x4 x = vf[e & 3];
-                        if constexpr (!FULL) {
+                    for (int d = 0; d < ND; ++d) o[ct][d] *= shrink;
+#pragma unroll
+                    for (int t = 0; t < 8; ++t) p[t] = __builtin_amdgcn_exp2f(p[t] - now);
+                    sum[ct] = __builtin_fmaf(((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7])), inv[h], sum[ct] * shrink);
+                    keep(sum[ct]);
+#pragma unroll
+                    for (int t = 0; t < 4; ++t) pack_weights(p[2 * t], p[2 * t + 1], pf[ct], t);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+                auto products = [&](auto has_nan) {
+#pragma unroll
+                    for (int e = 0; e < 3; ++e) read_value(h * ND + e);
+#pragma unroll
+                    for (int d = 0; d < ND; ++d) {
+                        if (d + 3 < ND) read_value(h * ND + d + 3);
+                        u32x4 x = ring[(h * ND + d) & 3];
+                        if constexpr (decltype(has_nan)::value) {
                             // A NaN among values that some rows do not see must not reach those (0 * NaN): it is taken out,
-                            // and counted for each row by a product of its own.  Tiles at an edge are few.
+                            // and counted for each row by a product of its own.
                             u32x4 is_nan;
 #pragma unroll
                             for (int t = 0; t < 4; ++t) {
@@ -887,7 +966,7 @@ __global__ __launch_bounds__(256, DS <= 4 ? 2 : 1) void kv_attend_many(KvAttendA
                                 u32x4 sees;
 #pragma unroll
                                 for (int t = 0; t < 4; ++t)
-                                    sees[t] = (seen[h][ct] >> (2 * t) & 1 ? 0x3F80u : 0u) | (seen[h][ct] >> (2 * t + 1) & 1 ? 0x3F800000u : 0u);
+                                    sees[t] = (seen[ct] >> (2 * t) & 1 ? 0x3F80u : 0u) | (seen[ct] >> (2 * t + 1) & 1 ? 0x3F800000u : 0u);
                                 const f32x4 n = mfma<false>(is_nan, sees, f32x4{0, 0, 0, 0});
 #pragma unroll
                                 for (int i = 0; i < 4; ++i) o[ct][d][i] = n[i] > 0.0f ? float_of(0x7FC00000u) : o[ct][d][i];
@@ -896,10 +975,76 @@ __global__ __launch_bounds__(256, DS <= 4 ? 2 : 1) void kv_attend_many(KvAttendA
 #pragma unroll
                         for (int ct = 0; ct < NT; ++ct)
 #pragma unroll
-                            for (int n = 0; n < NP; ++n) o[ct][d] = mfma<false>(x, pf[h][ct][n], o[ct][d]);
-                        if (!FULL || e % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+                            for (int n = 0; n < NP; ++n) o[ct][d] = mfma<false>(x, pf[ct][n], o[ct][d]);
+                        __builtin_amdgcn_sched_barrier(0);
                     }
-                    return true;
+                };
+                if (nan_here) products(std::true_type());
+                else products(std::false_type());
+            }
+        };
+        // A tile of which every row of the wave sees every token, against the running reference as it is.  That need not be the
+        // maximum: no score is compared with another while the sums of the weights stay below 2^11.  Where one does not (rarely:
+        // in the first tiles) the answer is false, nothing has been added up, and the tile is done again by `careful`.  (One loop
+        // that does both holds every output twice, and so does one with a second branch beside `careful`: what is spilled then
+        // comes back from HBM, 12 us a tile instead of 4.)
+        auto simple = [&]() -> bool {
+            read_scales();
+            // scores; the next tile is widened beside them
+            f32x4 sc[2][NT][2];
+#pragma unroll
+            for (int e = 0; e < 3 && e < 4 * DS; ++e) read_key(e);
+#pragma unroll
+            for (int e = 0; e < 4 * DS; ++e) {
+                const int i = e / DS, j = e % DS;
+                if (e + 3 < 4 * DS) read_key(e + 3);
+                if (e == DS) store_keys(buf ^ 1);
+                if (e == 2 * DS) store_values(buf ^ 1);
+#pragma unroll
+                for (int ct = 0; ct < NT; ++ct) {
+                    if (j == 0) sc[i >> 1][ct][i & 1] = f32x4{0, 0, 0, 0};
+#pragma unroll
+                    for (int n = 0; n < NQ; ++n) sc[i >> 1][ct][i & 1] = mfma<HALF>(ring[e & 3], qf[ct][n][j], sc[i >> 1][ct][i & 1]);
+                }
+                if (j == DS - 1) __builtin_amdgcn_sched_barrier(0);
+            }
+            u32x4 pf[2][NT][NP];
+            float more[NT];
+            bool over = false;
+#pragma unroll
+            for (int ct = 0; ct < NT; ++ct) {
+                more[ct] = 0.0f;
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const float off = lv[h] - top[ct];
+                    float p[8];
+#pragma unroll
+                    for (int t = 0; t < 8; ++t) p[t] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[h][ct][t >> 2][t & 3], c[h], off));
+                    const float part = ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
+                    over |= part > 2048.0f;
+                    more[ct] = __builtin_fmaf(part, inv[h], more[ct]);
+#pragma unroll
+                    for (int t = 0; t < 4; ++t) pack_weights(p[2 * t], p[2 * t + 1], pf[h][ct], t);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+            }
+            if (__any(over)) return false;
+#pragma unroll
+            for (int ct = 0; ct < NT; ++ct) sum[ct] += more[ct];
+            if (kb + 128 < hi) load(kb + 128, pc);
+#pragma unroll
+            for (int e = 0; e < 3; ++e) read_value(e);
+#pragma unroll
+            for (int e = 0; e < 2 * ND; ++e) {
+                const int h = e / ND, d = e % ND;
+                if (e + 3 < 2 * ND) read_value(e + 3);
+#pragma unroll
+                for (int ct = 0; ct < NT; ++ct)
+#pragma unroll
+                    for (int n = 0; n < NP; ++n) o[ct][d] = mfma<false>(ring[e & 3], pf[h][ct][n], o[ct][d]);
+                if (e % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+            }
+            return true;
         };
         auto advance = [&] {
             pa = pb, pb = pc, pc = pages(kb + 192);
@@ -910,19 +1055,16 @@ __global__ __launch_bounds__(256, DS <= 4 ? 2 : 1) void kv_attend_many(KvAttendA
         // (behind the last tile the other buffer is filled with what the registers hold, and read by nobody)
         // Every wave passes the same barriers, one a tile, from whichever of the two loops.
         while (kb < hi) {
-            if (kb + 64 < hi) hide(kb + 64, pb);
-            if (idle || kb > wpos1 || kb + 63 < w_lo) {
-                store_keys(buf ^ 1);
-                store_values(buf ^ 1);
-                if (kb + 128 < hi) load(kb + 128, pc);
-            } else {
-                compute(std::false_type());
-            }
+            if (kb + 64 < hi) hide(kb + 64, pb, buf ^ 1);
+            store_keys(buf ^ 1);
+            store_values(buf ^ 1);
+            if (!idle && kb <= wpos1 && kb + 63 >= w_lo) careful();
+            if (kb + 128 < hi) load(kb + 128, pc);
             advance();
             bool again = false;
-            while (kb < hi && plain(kb, pa) && !again) {
-                if (kb + 64 < hi) hide(kb + 64, pb);
-                again = !compute(std::true_type());
+            while (kb < hi && plain_here(kb, pa) && !again) {
+                if (kb + 64 < hi) hide(kb + 64, pb, buf ^ 1);
+                again = !simple();
                 if (!again) advance();
             }
         }
@@ -931,10 +1073,9 @@ __global__ __launch_bounds__(256, DS <= 4 ? 2 : 1) void kv_attend_many(KvAttendA
             float total = sum[ct];
             total += __shfl_xor(total, 16);
             total += __shfl_xor(total, 32);
-            const int64_t r = wrow0 + ct * 16 + m;
-            if (r < rows) {
-                const int32_t tok = (int32_t)(r / G);
-                const uint64_t orow = (uint64_t)(s.first + tok) * a.q_heads + head * G + (uint32_t)(r - (int64_t)tok * G);
+            const int32_t r = wrow0 + ct * 16 + fresh(m);
+            if (r < here) {
+                const uint64_t orow = (uint64_t)(s.first + token(r)) * a.q_heads + q_head(r);
                 const bool none = total == 0.0f;
                 const float inv = none ? 0.0f : 1.0f / total;
                 E<T>* out = (E<T>*)a.out + orow * D + q4 * 4;
@@ -1023,9 +1164,12 @@ __global__ __launch_bounds__(kJoinThreads) void kv_join(KvAttendArgs a, Plan pla
 template <int T, int DS>
 hipError_t launch_one(const KvAttendArgs& a, const Plan& plan, hipStream_t stream) {
     if (plan.many) {
-        const uint32_t G = a.q_heads / a.mem.heads, rows = Many<T, DS>::rows;
-        const uint64_t blocks = std::min<uint64_t>(((uint64_t)plan.max_new * G + rows - 1) / rows, (1u << 30) / a.mem.heads);
-        hipLaunchKernelGGL((kv_attend_many<T, DS>), dim3((uint32_t)blocks * a.mem.heads, 1, a.batch.count), dim3(256), (Many<T, DS>::lds), stream, a);
+        // (blocks a head: as many as there can be items, or, where not all sequences are looked at, of the longest chunk)
+        const uint64_t G = a.q_heads / a.mem.heads, rows = Many<T, DS>::rows, count = a.batch.count;
+        const bool sorted = count <= 64;
+        const uint64_t blocks = std::min<uint64_t>(sorted ? std::min<uint64_t>(a.batch.tokens, plan.max_new * count) * G / rows + count : (plan.max_new * G + rows - 1) / rows,
+                                                   (1u << 30) / a.mem.heads);
+        hipLaunchKernelGGL((kv_attend_many<T, DS>), dim3((uint32_t)blocks * a.mem.heads, 1, sorted ? 1 : a.batch.count), dim3(Many<T, DS>::kThreads), (Many<T, DS>::lds), stream, a);
         return hipGetLastError();
     }
     const dim3 grid(plan.tiles * plan.splits, a.mem.heads, a.batch.count);
@@ -1062,12 +1206,12 @@ Plan plan_of(const KvAttendArgs& a, uint32_t max_new) {
     uint64_t tokens = a.n_select ? a.n_select : (uint64_t)a.batch.table_width << a.mem.page_shift;
     if (!a.n_select && a.window) tokens = std::min<uint64_t>(tokens, (uint64_t)a.window + max_new + 31);
     const uint64_t blocks = (uint64_t)p.tiles * a.mem.heads * a.batch.count;
-    // As many ranges as give some 3072 blocks, four times what the chip holds at once: sequences of different lengths even out
-    // (64 of 1 000 to 8 192 tokens, 8 heads: 147 us at 1024 blocks, 130 at 1536, 121 at 3072, 125 at 4096).  But no range
+    // As many ranges as give some 12 blocks a CU, four times what the chip holds at once: sequences of different lengths even out
+    // (64 of 1 000 to 8 192 tokens, 8 heads: 147 us at 4 a CU, 130 at 6, 121 at 12, 125 at 16).  But no range
     // shorter than 512 tokens (selected ones: 1024), where a block's start and end begin to count (500 tokens in one block 9.4 us,
     // in four 6.0 and 4.4 for the join; 2048 selected ones in two ranges 40 us, in four 46), and at most 384 of one row, or the
     // join counts (two sequences of 500 003: 384 ranges 103 + 10 us, 768 104 + 17, 256 109 + 8).
-    const uint64_t want = std::min<uint64_t>(384, std::max<uint64_t>(1, 3072 / blocks));
+    const uint64_t want = std::min<uint64_t>(384, std::max<uint64_t>(1, 12 * 256 / blocks));
     uint64_t chunk = std::max<uint64_t>(a.n_select ? 1024 : 512, (tokens + want - 1) / want);
     chunk = (chunk + 127) / 128 * 128;
     p.chunk = (uint32_t)std::min<uint64_t>(chunk, 1u << 30);

@@ -724,3 +724,55 @@ def test_workspace_covers_every_range():
                     assert rest == 0 and ranges <= 384
                     if seen <= 512:
                         assert need == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("dim", [64, 96, 128, 224])
+def test_attend_many_rows_far_scores(dtype, dim):
+    """Scores of hundreds, either way, over many tiles: the softmax's reference has to move in the middle of a chunk's walk."""
+    held, new, page, heads, hq = [700, 650, 70], [300, 400, 70], 16, 8, 16
+    s = Setup(held, page, heads, dim, seed=18)
+    t = TYPES[dtype]
+    off = offsets_of(new)
+    mem = s.memory()
+    table, lengths = s.on_gpu()
+    for mul in (60.0, -60.0, 0.0):
+        q = s.randn(off[-1], hq, dim, dtype=t) * mul
+        out, lse = mem.attend(q.cuda(), table, lengths, offsets=ints(off), max_new=max(new), return_lse=True)
+        check_attend(out, lse, attend_ref(q, s.k, s.v, s.ks, s.vs, s.table, held, off, page, dim ** -0.5), t)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("count,most", [(64, 40), (65, 40), (130, 70)])
+def test_attend_many_sequences(count, most):
+    """Up to and beyond the 64 sequences whose work is put in order: every row is written, whatever the lengths, also with none
+    held, fewer held than new, none new; and whatever the caller says is the longest chunk."""
+    page, heads, hq, dim = 16, 2, 8, 64
+    r = np.random.default_rng(count)
+    held = [int(x) for x in r.integers(0, 120, count)]
+    new = [int(x) for x in r.integers(0, most + 1, count)]
+    held[3], new[3], held[4], new[4], new[5], held[6], new[6] = 5, most, 0, 2, 0, 119, most
+    s = Setup(held, page, heads, dim, seed=count)
+    off = offsets_of(new)
+    q = s.randn(off[-1], hq, dim, dtype=torch.bfloat16)
+    mem = s.memory()
+    table, lengths = s.on_gpu()
+    ref = attend_ref(q, s.k, s.v, s.ks, s.vs, s.table, held, off, page, dim ** -0.5, 50)
+    for said in (most, 16, 100_000):
+        out, lse = mem.attend(q.cuda(), table, lengths, offsets=ints(off), max_new=said, window=50, return_lse=True)
+        check_attend(out, lse, ref, torch.bfloat16)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("held,new", [([2100], [2048]), ([513] * 4, [512] * 4), ([5000, 64, 65, 2000], [30, 64, 1, 900])])
+def test_attend_many_rows_every_item(held, new):
+    """Work in the order of its cost, over sequences that are equal, alone or very different: nothing is left out or done twice."""
+    page, heads, hq, dim = 64, 8, 32, 32
+    s = Setup(held, page, heads, dim, seed=19)
+    off = offsets_of(new)
+    q = s.randn(off[-1], hq, dim, dtype=torch.bfloat16)
+    mem = s.memory()
+    table, lengths = s.on_gpu()
+    out, lse = mem.attend(q.cuda(), table, lengths, offsets=ints(off), max_new=max(new), return_lse=True)
+    check_attend(out, lse, attend_ref(q, s.k, s.v, s.ks, s.vs, s.table, held, off, page, dim ** -0.5), torch.bfloat16)

@@ -558,7 +558,9 @@ __global__ __launch_bounds__(256, attend_waves(T, DS, MODE)) void kv_attend(KvAt
 //   - the scale of a page's values is folded into the exponent: w = exp2(score + log2 v_scale - M) with M the running
 //     maximum of just that, and the softmax's sum takes w / v_scale; so a score costs one fma, one exp2, one add;
 //   - the loads of the tile after next are under way while one is computed and the next is being widened.
-// Measured: four chunks of 30 to 2048 tokens, the longest sequence 6 000, 32 heads on 8, 128 dimensions, bf16: 325 us (matrix products alone 182).
+// Measured: four chunks of 30 to 2048 tokens, the longest sequence 6 000, 32 heads on 8, 128 dimensions, bf16: 317 us (its matrix products at the rate of a
+// large product: 182); of a block's 45 to 240 us, 2.3 a tile, 4 one at an edge, and some 25 to start and end.  Left out in turn, the
+// loads, the exp2, either product, the barrier or the widening save 5 to 15 % each: nothing of it alone is what takes the time.
 template <int T, int DS>
 struct Many {
     static constexpr int NT = T == kF32 || DS > 5 ? 1 : 2;  // (192 dimensions: 511 us with one, 627 with two; 160: 473, 380)
@@ -594,10 +596,12 @@ struct Items {
         }
     }
     // items of sequence b that see at least `tokens`
-    __device__ __forceinline__ int32_t at_least(int b, int64_t tokens, uint32_t G, uint32_t rows) const {
-        const int32_t n = __builtin_amdgcn_readlane(items, b);
-        const uint64_t before = (uint64_t)max(tokens - 1 - __builtin_amdgcn_readlane(mine.start, b), (int64_t)0) * G / rows;
-        return tokens > __builtin_amdgcn_readlane(seen, b) ? 0 : n - (int32_t)min(before, (uint64_t)max(n - 1, 0));
+    __device__ __forceinline__ int32_t at_least(int b, uint32_t tokens, uint32_t G, uint32_t rows) const {
+        const uint32_t n = __builtin_amdgcn_readlane(items, b);
+        // (rows before the first token, of a length that counts fewer tokens than there are new ones, see 0)
+        const int32_t more = tokens ? (int32_t)tokens - 1 - max(__builtin_amdgcn_readlane(mine.start, b), -(1 << 30)) : 0;
+        const uint32_t before = (uint32_t)min((uint64_t)(uint32_t)max(more, 0) * G / rows, (uint64_t)0xFFFFFFFF);
+        return tokens > (uint32_t)__builtin_amdgcn_readlane(seen, b) ? 0 : (int32_t)(n - min(before, max(n, 1u) - 1));
     }
     // Item k by falling cost (in steps of 64 tokens): 64 costs are looked at at once, one a lane.
     __device__ __forceinline__ bool find(uint32_t count, int lane, int64_t k, uint32_t G, uint32_t rows, Sequence& s, uint32_t& b, int32_t& block) const {
@@ -608,17 +612,17 @@ struct Items {
         int32_t lo = 0, end = most / 64 + 1;
         while (end - lo > 1) {
             const int32_t step = (end - lo + 63) / 64;
-            const int64_t here = lo + (int64_t)lane * step;
+            const int32_t here = min(lo + lane * step, most / 64 + 1);
             int64_t n = 0;
-            for (uint32_t i = 0; i < count; ++i) n += at_least(i, here * 64, G, rows);
+            for (uint32_t i = 0; i < count; ++i) n += at_least(i, here * 64u, G, rows);
             const uint64_t yes = __ballot(here < end && n > k);  // lane 0 always
             lo += (63 - __builtin_clzll(yes)) * step;
             end = min(end, lo + step);
         }
         // those of that cost, sequence by sequence
-        for (uint32_t i = 0; i < count; ++i) k -= at_least(i, (int64_t)(lo + 1) * 64, G, rows);
+        for (uint32_t i = 0; i < count; ++i) k -= at_least(i, (lo + 1) * 64u, G, rows);
         for (b = 0; b < count; ++b) {
-            const int32_t more = at_least(b, (int64_t)(lo + 1) * 64, G, rows), here = at_least(b, (int64_t)lo * 64, G, rows) - more;
+            const int32_t more = at_least(b, (lo + 1) * 64u, G, rows), here = at_least(b, lo * 64u, G, rows) - more;
             if (k < here) {
                 block = __builtin_amdgcn_readlane(items, b) - more - 1 - (int32_t)k;
                 s.first = (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int32_t)(mine.first >> 32), b) << 32 | (uint32_t)__builtin_amdgcn_readlane((int32_t)mine.first, b));
@@ -1008,6 +1012,7 @@ __global__ __launch_bounds__((Many<T, DS>::kThreads), (Many<T, DS>::occupancy)) 
                 }
                 if (j == DS - 1) __builtin_amdgcn_sched_barrier(0);
             }
+            __builtin_amdgcn_s_setprio(0);  // a wave in its products goes before one in its softmax: 317 us against 327
             u32x4 pf[2][NT][NP];
             float more[NT];
             bool over = false;
@@ -1029,6 +1034,7 @@ __global__ __launch_bounds__((Many<T, DS>::kThreads), (Many<T, DS>::occupancy)) 
                 }
             }
             if (__any(over)) return false;
+            __builtin_amdgcn_s_setprio(1);
 #pragma unroll
             for (int ct = 0; ct < NT; ++ct) sum[ct] += more[ct];
             if (kb + 128 < hi) load(kb + 128, pc);
@@ -1200,7 +1206,12 @@ Plan plan_of(const KvAttendArgs& a, uint32_t max_new) {
     Plan p{};
     p.max_new = max_new;
     p.splits = 1;
-    p.many = !a.n_select && (uint64_t)max_new * G / 192 * a.mem.heads * a.batch.count >= 128;
+    // Chunks that fill half of the chip at least with blocks of 128 rows, and whose rows fill them at least by half, are walked from
+    // end to end (us, cut into ranges / walked, memories of 2000 tokens, 32 heads on 8, bf16, 128 dimensions: one chunk of 256 new
+    // tokens 60 / 85, of 512 96 / 86, of 1024 100 / 89; 32 of 4 42 / 80, of 16 116 / 85; 100 of 8 132 / 238, of 32 488 / 270;
+    // in f32 one of 256 80 / 84, of 512 133 / 87).
+    const uint64_t rows = (uint64_t)max_new * G;
+    p.many = !a.n_select && rows >= 64 && (rows + 127) / 128 * a.mem.heads * a.batch.count >= 128;
     if (p.many) return p;
     p.tiles = (uint32_t)std::min<uint64_t>(((uint64_t)max_new * G + 15) / 16, 65535);
     uint64_t tokens = a.n_select ? a.n_select : (uint64_t)a.batch.table_width << a.mem.page_shift;

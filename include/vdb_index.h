@@ -287,7 +287,8 @@ int vdb_rows4_products_device(const uint8_t* d_codes, const uint8_t* d_scales, s
  * row t % page_tokens.  Codes are e4m3 (no infinities; 0x7F and 0xFF are NaN) and stand for code * scale, one f32 scale
  * per page, head and side (keys, values).
  * All calls are asynchronous on `stream`, use the current device, allocate nothing and may be captured.  Two appends that
- * touch one page must not overlap, nor an append and a read of the same page. */
+ * touch one page must not overlap, nor an append and a read of the same page; nor may two sequences of one append share a page
+ * that either writes (pages that are only read, a common prefix, may be shared). */
 typedef struct vdb_kv_memory {
     void* k;         /* [pages][heads][page_tokens][dim] e4m3, 16-byte aligned, DEVICE */
     void* v;         /* likewise */
@@ -317,7 +318,7 @@ typedef struct vdb_kv_batch {
  * With rot_dims != 0 (a multiple of 16, at most dim) the first rot_dims numbers of every key, and of every query, are turned
  * by the angles of the token's position: cos, sin [positions][rot_dims / 2] f32, 16-byte aligned; the pair is (d, d + rot_dims / 2),
  * or (2 i, 2 i + 1) with interleaved != 0; (x, y) becomes (x cos - y sin, y cos + x sin) in f32.  A position beyond the
- * tables: its key and value are not stored and its query is NaN.
+ * tables has no angles: its key is not stored (its value is), and its query, like one at a negative position, is NaN.
  * q nullable [tokens][q_heads][dim] of `dtype` (strides as above) -> q_out [tokens][q_heads][dim], turned, rounded once; rows
  * of no sequence are copied.  q_out must not overlap q.  Needs rot_dims != 0. */
 int vdb_kv_append_device(const vdb_kv_memory* memory, const vdb_kv_batch* batch, int dtype, const void* d_k, size_t k_token_stride,

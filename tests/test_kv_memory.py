@@ -776,3 +776,23 @@ def test_attend_many_rows_every_item(held, new):
     table, lengths = s.on_gpu()
     out, lse = mem.attend(q.cuda(), table, lengths, offsets=ints(off), max_new=max(new), return_lse=True)
     check_attend(out, lse, attend_ref(q, s.k, s.v, s.ks, s.vs, s.table, held, off, page, dim ** -0.5), torch.bfloat16)
+
+
+@pytest.mark.gpu
+def test_rows_with_odd_strides_of_single_dimensions():
+    """One token or one head out of something larger: a stride that nobody steps along may be any number."""
+    page, dim = 16, 32
+    for tokens, heads in ((1, 2), (3, 1), (1, 1)):
+        s = Setup([20] * tokens, page, heads, dim, seed=20)
+        mem = s.memory()
+        table, lengths = s.on_gpu()
+        k, v, q = s.randn(tokens, heads, dim), s.randn(tokens, heads, dim), s.randn(tokens, heads, dim)
+        def odd(x):
+            return x.cuda().as_strided(x.shape, (heads * dim if tokens > 1 else 5, dim if heads > 1 else 3, 1))
+        mem.append(odd(k), odd(v), table, lengths)
+        off = list(range(tokens + 1))
+        append_ref(s.k, s.ks, k, s.table, s.lengths, off, page)
+        append_ref(s.v, s.vs, v, s.table, s.lengths, off, page)
+        assert same_codes(mem.k, s.k) and same_codes(mem.v, s.v)
+        out = mem.attend(odd(q), table, lengths)
+        check_attend(out, None, attend_ref(q, s.k, s.v, s.ks, s.vs, s.table, s.lengths, off, page, dim ** -0.5), torch.float32)

@@ -21,9 +21,7 @@ def _rows(x):
     """x [tokens, heads, dim], or a copy of it, as the kernels read it: heads of contiguous numbers, 16-byte steps."""
     s = x.stride()
     if s[2] != 1 or s[0] % 8 or s[1] % 8 or s[0] < 0 or s[1] < 0 or x.data_ptr() % 16:
-        x = x.contiguous()
-        if x.data_ptr() % 16:
-            x = x.clone()
+        x = x.clone(memory_format=torch.contiguous_format)  # (contiguous() may keep the odd stride of a dimension of size 1)
     return x
 
 
@@ -32,8 +30,9 @@ class KeyValueMemory:
 
     ``k``, ``v``: float8_e4m3fn [pages, kv_heads, page_tokens, head_dim]; ``k_scale``, ``v_scale``: float32
     [pages, kv_heads].  A stored number is code * scale.  Which page holds what is the caller's: ``table`` [sequences, width]
-    int32, token t of sequence b lies in page table[b, t // page_tokens].  ``lengths`` [sequences] int32 counts a sequence's
-    tokens, the new ones of the call included, for ``append`` and ``attend`` alike."""
+    int32, token t of sequence b lies in page table[b, t // page_tokens]; a page that several sequences list is not
+    appended to.  ``lengths`` [sequences] int32 counts a sequence's
+    tokens, the new ones of the call included, for ``append`` and ``attend`` alike.  Neither call has a gradient."""
 
     def __init__(self, pages: int, page_tokens: int, kv_heads: int, head_dim: int, device="cuda"):
         code = lambda: torch.zeros((pages, kv_heads, page_tokens, head_dim), dtype=torch.uint8, device=device).view(torch.float8_e4m3fn)  # noqa: E731
@@ -74,6 +73,8 @@ class KeyValueMemory:
             raise ValueError("table [sequences, width] and lengths [sequences]: int32")
         if table.device != self.device or lengths.device != self.device or not (table.is_contiguous() and lengths.is_contiguous()):
             raise ValueError(f"table and lengths: contiguous, on {self.device}")
+        if n and not table.shape[1]:
+            raise ValueError("table: at least one page wide")
         if offsets is None:
             if tokens != n:
                 raise ValueError(f"without offsets every sequence has one new token: {tokens} rows for {n} sequences")

@@ -76,7 +76,7 @@ class Rows4:
         return out
 
     def products(self, queries, out=None):
-        """Inner products of queries [nq, dim] (or [dim]) with every row: [nq, n] (or [n]) float32, into ``out`` if given."""
+        """Inner products of queries [nq, dim] (or [dim]) with every row: [nq, n] (or [n]) float32, into ``out`` if given (no gradient)."""
         x = queries if queries.dim() == 2 else queries.unsqueeze(0)
         if queries.dim() not in (1, 2) or x.shape[1] != self.dim or x.device != self.codes.device:
             raise ValueError(f"expected queries [nq, {self.dim}] on {self.codes.device}, got {tuple(queries.shape)} on {queries.device}")

@@ -796,3 +796,28 @@ def test_rows_with_odd_strides_of_single_dimensions():
         assert same_codes(mem.k, s.k) and same_codes(mem.v, s.v)
         out = mem.attend(odd(q), table, lengths)
         check_attend(out, None, attend_ref(q, s.k, s.v, s.ks, s.vs, s.table, s.lengths, off, page, dim ** -0.5), torch.float32)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("new", [[1, 1], [200, 256]])
+def test_attend_scales_far_apart(dtype, new):
+    """Pages of zeros (whose scale is the smallest that is stored), of ordinary and of huge values in one sequence: the zeros
+    count in the softmax's sum as anything else does."""
+    held, page, heads, hq, dim = [520, 300], 16, 16, 32, 64
+    t = TYPES[dtype]
+    s = Setup(held, page, heads, dim, seed=21)
+    for b in range(2):
+        for p in range(-(-held[b] // page)):
+            i = s.table[b, p].long()
+            if (p // 5) % 3 == 0:
+                s.v.view(torch.uint8)[i] = 0
+                s.vs[i] = 2.0 ** -100
+            else:
+                s.vs[i] = 2.0 ** (-2 if (p // 5) % 3 == 1 or dtype == "f16" else 40)
+    off = offsets_of(new)
+    q = s.randn(off[-1], hq, dim, dtype=t)
+    mem = s.memory()
+    table, lengths = s.on_gpu()
+    out, lse = mem.attend(q.cuda(), table, lengths, offsets=None if max(new) == 1 else ints(off), max_new=max(new), return_lse=True)
+    check_attend(out, lse, attend_ref(q, s.k, s.v, s.ks, s.vs, s.table, held, off, page, dim ** -0.5), t)

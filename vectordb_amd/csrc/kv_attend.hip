@@ -556,7 +556,9 @@ __global__ __launch_bounds__(256, attend_waves(T, DS, MODE)) void kv_attend(KvAt
 //   - codes are widened to bf16 (f16) once per block, into LDS in the order in which lanes hold matrix operands; a wave uses
 //     each operand it reads for its NT row tiles;
 //   - the scale of a page's values is folded into the exponent: w = exp2(score + log2 v_scale - M) with M the running
-//     maximum of just that, and the softmax's sum takes w / v_scale; so a score costs one fma, one exp2, one add;
+//     maximum of just that, and the softmax's sum takes w / v_scale; so a score costs one fma, one exp2, one add.  (Where the
+//     scales of a head's pages lie so far apart that w could underflow and w / v_scale count - pages of zeros beside values of
+//     thousands do - the weight is w / v_scale from the start, and costs a product more.)
 //   - the loads of the tile after next are under way while one is computed and the next is being widened.
 // Measured: four chunks of 30 to 2048 tokens, the longest sequence 6 000, 32 heads on 8, 128 dimensions, bf16: 317 us (its matrix products at the rate of a
 // large product: 182); of a block's 45 to 240 us, 2.3 a tile, 4 one at an edge, and some 25 to start and end.  Left out in turn, the
@@ -874,13 +876,14 @@ __global__ __launch_bounds__((Many<T, DS>::kThreads), (Many<T, DS>::occupancy)) 
         __syncthreads();
         int32_t kb = kb0;
         int buf = 0;
-        float c[2], lv[2], inv[2];  // of the tile's pages: of the scores, log2 and inverse of the values' scale
+        float c[2], lv[2], inv[2], vs[2];  // of the tile's pages: scale of the scores, log2, inverse and scale of the values
+        float v_least = 0.0f;  // 2^-60 of the largest scale of values that the softmax's reference can have come from
         auto read_scales = [&] {
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 c[h] = scales_s[buf * 8 + 2 * h + (q4 >> 1)] * to_log2;
-                const float vs = __builtin_fmaxf(scales_s[buf * 8 + 4 + 2 * h + (q4 >> 1)], 0x1p-120f);
-                lv[h] = __builtin_amdgcn_logf(vs), inv[h] = __builtin_amdgcn_rcpf(vs);
+                vs[h] = __builtin_fmaxf(scales_s[buf * 8 + 4 + 2 * h + (q4 >> 1)], 0x1p-120f);
+                lv[h] = __builtin_amdgcn_logf(vs[h]), inv[h] = __builtin_amdgcn_rcpf(vs[h]);
             }
         };
         u32x4 ring[4];  // operands are read three products ahead
@@ -901,6 +904,8 @@ __global__ __launch_bounds__((Many<T, DS>::kThreads), (Many<T, DS>::occupancy)) 
         // take no more registers than in the other loop.
         auto careful = [&] {
             read_scales();
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v_least = __builtin_fmaxf(v_least, scales_s[buf * 8 + 4 + i] * 0x1p-60f);
             const bool nan_here = __builtin_amdgcn_readfirstlane(nan_s[buf]) == kb;
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
@@ -931,18 +936,17 @@ __global__ __launch_bounds__((Many<T, DS>::kThreads), (Many<T, DS>::occupancy)) 
                     seen[ct] = ((1u << to) - 1) & ~((1u << from) - 1);
                     float now = top[ct], p[8];
 #pragma unroll
-                    for (int t = 0; t < 8; ++t) {
-                        p[t] = seen[ct] >> t & 1 ? __builtin_fmaf(sc[ct][t >> 2][t & 3], c[h], lv[h]) : -__builtin_inff();
-                        now = __builtin_fmaxf(now, p[t]);
-                    }
+                    for (int t = 0; t < 8; ++t) now = __builtin_fmaxf(now, seen[ct] >> t & 1 ? __builtin_fmaf(sc[ct][t >> 2][t & 3], c[h], lv[h]) : -__builtin_inff());
                     now = max_of_quarters(now);
                     const float shrink = __builtin_amdgcn_exp2f(top[ct] - now);
                     top[ct] = now;
 #pragma unroll
                     for (int d = 0; d < ND; ++d) o[ct][d] *= shrink;
 #pragma unroll
-                    for (int t = 0; t < 8; ++t) p[t] = __builtin_amdgcn_exp2f(p[t] - now);
-                    sum[ct] = __builtin_fmaf(((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7])), inv[h], sum[ct] * shrink);
+                    for (int t = 0; t < 8; ++t) p[t] = seen[ct] >> t & 1 ? __builtin_amdgcn_exp2f(__builtin_fmaf(sc[ct][t >> 2][t & 3], c[h], -now)) : 0.0f;
+                    sum[ct] = __builtin_fmaf(sum[ct], shrink, ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7])));
+#pragma unroll
+                    for (int t = 0; t < 8; ++t) p[t] *= vs[h];
                     keep(sum[ct]);
 #pragma unroll
                     for (int t = 0; t < 4; ++t) pack_weights(p[2 * t], p[2 * t + 1], pf[ct], t);
@@ -1015,7 +1019,8 @@ __global__ __launch_bounds__((Many<T, DS>::kThreads), (Many<T, DS>::occupancy)) 
             __builtin_amdgcn_s_setprio(0);  // a wave in its products goes before one in its softmax: 317 us against 327
             u32x4 pf[2][NT][NP];
             float more[NT];
-            bool over = false;
+            // (where a page's scale is that far below, a weight times it could underflow though it counts in the sum)
+            bool over = __builtin_fminf(vs[0], vs[1]) < v_least;
 #pragma unroll
             for (int ct = 0; ct < NT; ++ct) {
                 more[ct] = 0.0f;

@@ -15,14 +15,19 @@ from .rows4 import dtype_code, on_device
 
 
 _needs = {}  # bytes of workspace by the sizes of a call
+_E4M3, _F32, _I32 = torch.float8_e4m3fn, torch.float32, torch.int32
 
 
 def _rows(x):
-    """x [tokens, heads, dim], or a copy of it, as the kernels read it: heads of contiguous numbers, 16-byte steps."""
-    s = x.stride()
-    if s[2] != 1 or s[0] % 8 or s[1] % 8 or s[0] < 0 or s[1] < 0 or x.data_ptr() % 16:
+    """x [tokens, heads, dim], or a copy of it, as the kernels read it: heads of contiguous numbers, 16-byte steps; and the
+    address and steps of that."""
+    a, b, c = x.stride()
+    at = x.data_ptr()
+    if c != 1 or a % 8 or b % 8 or a < 0 or b < 0 or at % 16:
         x = x.clone(memory_format=torch.contiguous_format)  # (contiguous() may keep the odd stride of a dimension of size 1)
-    return x
+        a, b, c = x.stride()
+        at = x.data_ptr()
+    return x, at, a, b
 
 
 class KeyValueMemory:
@@ -49,10 +54,10 @@ class KeyValueMemory:
     def _take(self, k, v, k_scale, v_scale):
         if k.dim() != 4 or k.shape != v.shape or k_scale.shape != k.shape[:2] or v_scale.shape != k.shape[:2]:
             raise ValueError("expected k, v [pages, kv_heads, page_tokens, head_dim] and k_scale, v_scale [pages, kv_heads]")
-        if k.dtype != torch.float8_e4m3fn or v.dtype != torch.float8_e4m3fn or k_scale.dtype != torch.float32 or v_scale.dtype != torch.float32:
+        if k.dtype is not _E4M3 or v.dtype is not _E4M3 or k_scale.dtype is not _F32 or v_scale.dtype is not _F32:
             raise ValueError("k, v: float8_e4m3fn; k_scale, v_scale: float32")
-        device = k.device
-        if not k.is_cuda or v.device != device or k_scale.device != device or v_scale.device != device:
+        index = k.get_device() if k.is_cuda else -1
+        if index < 0 or v.get_device() != index or k_scale.get_device() != index or v_scale.get_device() != index:
             raise ValueError("k, v, k_scale, v_scale: CUDA tensors on one device")
         if not (k.is_contiguous() and v.is_contiguous() and k_scale.is_contiguous() and v_scale.is_contiguous()):
             raise ValueError("k, v, k_scale, v_scale must be contiguous")
@@ -63,28 +68,34 @@ class KeyValueMemory:
             raise ValueError("head_dim must be a multiple of 32 in 32..256")
         self._l = _lib.lib()
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
-        self.device = device
+        self.device, self._index = k.device, index
         self.kv_heads, self.page_tokens, self.head_dim = heads, page_tokens, dim
         self._m = KvMemoryStruct(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), pages, heads, page_tokens, dim)
 
     def _batch(self, table, lengths, offsets, max_new, tokens):
-        n = lengths.shape[0]
-        if table.dtype != torch.int32 or lengths.dtype != torch.int32 or table.dim() != 2 or lengths.dim() != 1 or table.shape[0] != n:
+        n, index = lengths.shape[0], self._index
+        if table.dtype is not _I32 or lengths.dtype is not _I32 or table.dim() != 2 or lengths.dim() != 1 or table.shape[0] != n:
             raise ValueError("table [sequences, width] and lengths [sequences]: int32")
-        if table.device != self.device or lengths.device != self.device or not (table.is_contiguous() and lengths.is_contiguous()):
+        if table.get_device() != index or lengths.get_device() != index or not (table.is_contiguous() and lengths.is_contiguous()):
             raise ValueError(f"table and lengths: contiguous, on {self.device}")
-        if n and not table.shape[1]:
+        width = table.shape[1]
+        if n and not width:
             raise ValueError("table: at least one page wide")
         if offsets is None:
             if tokens != n:
                 raise ValueError(f"without offsets every sequence has one new token: {tokens} rows for {n} sequences")
-        elif offsets.dtype != torch.int32 or tuple(offsets.shape) != (n + 1,) or offsets.device != self.device or not offsets.is_contiguous():
+            at = None
+        elif offsets.dtype is not _I32 or offsets.shape != (n + 1,) or offsets.get_device() != index or not offsets.is_contiguous():
             raise ValueError(f"offsets: contiguous int32 [{n + 1}] on {self.device}")
-        return KvBatchStruct(table.data_ptr(), lengths.data_ptr(), None if offsets is None else offsets.data_ptr(), n, max(table.shape[1], 1), tokens, max_new)
+        else:
+            at = offsets.data_ptr()
+        return KvBatchStruct(table.data_ptr(), lengths.data_ptr(), at, n, width or 1, tokens, max_new)
 
     def _check_rows(self, x, heads, what):
-        if x.dim() != 3 or x.shape[2] != self.head_dim or (heads and x.shape[1] != heads) or x.device != self.device:
-            raise ValueError(f"{what}: expected [tokens, {heads or 'heads'}, {self.head_dim}] on {self.device}, got {tuple(x.shape)} on {x.device}")
+        shape = x.shape
+        if len(shape) != 3 or shape[2] != self.head_dim or (heads and shape[1] != heads) or x.get_device() != self._index:
+            raise ValueError(f"{what}: expected [tokens, {heads or 'heads'}, {self.head_dim}] on {self.device}, got {tuple(shape)} on {x.device}")
+        return shape
 
     def append(self, k, v, table, lengths, *, offsets=None, max_new=None, queries=None, cos=None, sin=None, interleaved: bool = False):
         """Stores the keys and values k, v [tokens, kv_heads, head_dim] of new tokens.
@@ -93,35 +104,41 @@ class KeyValueMemory:
         are its last ones (at most ``max_new`` of any sequence; by default all rows).  ``cos``, ``sin`` [positions, half]
         float32 turn the first 2 * half numbers of each key by its position's angles, in pairs (d, d + half), or (2 i, 2 i + 1)
         if ``interleaved``.  Returns ``queries`` [tokens, q_heads, head_dim], turned likewise (rows of no sequence: copied; None without queries)."""
-        self._check_rows(k, self.kv_heads, "k")
-        t = dtype_code(k, "k")
-        if v.shape != k.shape or v.dtype != k.dtype or v.device != k.device:
+        shape = self._check_rows(k, self.kv_heads, "k")
+        t, dtype, index = dtype_code(k, "k"), k.dtype, self._index
+        if v.shape != shape or v.dtype is not dtype or v.get_device() != index:
             raise ValueError("k and v: one shape, type and device")
-        tokens = k.shape[0]
+        tokens = shape[0]
         batch = self._batch(table, lengths, offsets, tokens if max_new is None else max_new, tokens)
         rot = positions = 0
-        if (cos is None) != (sin is None):
-            raise ValueError("cos and sin go together")
-        if cos is not None:
-            if cos.dim() != 2 or cos.shape != sin.shape or cos.dtype != torch.float32 or sin.dtype != torch.float32:
+        cos_at = sin_at = None
+        if cos is not None and sin is not None:
+            if cos.dim() != 2 or cos.shape != sin.shape or cos.dtype is not _F32 or sin.dtype is not _F32:
                 raise ValueError("cos and sin: float32 [positions, half]")
-            if cos.device != self.device or sin.device != self.device or not (cos.is_contiguous() and sin.is_contiguous()):
+            if cos.get_device() != index or sin.get_device() != index or not (cos.is_contiguous() and sin.is_contiguous()):
                 raise ValueError(f"cos and sin: contiguous, on {self.device}")
-            positions, rot = cos.shape[0], 2 * cos.shape[1]
-        k, v = _rows(k), _rows(v)
-        q = out = None
-        if queries is not None:
-            self._check_rows(queries, None, "queries")
-            if queries.shape[0] != tokens or queries.dtype != k.dtype:
-                raise ValueError(f"queries: [{tokens}, q_heads, {self.head_dim}] {k.dtype}")
-            out = queries
+            positions, rot = cos.shape
+            rot *= 2
             if rot:
-                q = _rows(queries)
-                out = torch.empty_like(q, memory_format=torch.contiguous_format)
-        ks, vs, qs = k.stride(), v.stride(), (0, 0) if q is None else q.stride()
-        on_device(self.device, self._l.vdb_kv_append_device, self._m, batch, t, k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1],
-                  cos.data_ptr() if rot else None, sin.data_ptr() if rot else None, positions, rot, interleaved,
-                  None if q is None else q.data_ptr(), qs[0], qs[1], 0 if q is None else q.shape[1], None if q is None else out.data_ptr())
+                cos_at, sin_at = cos.data_ptr(), sin.data_ptr()
+        elif cos is not None or sin is not None:
+            raise ValueError("cos and sin go together")
+        # (the tensors keep the copies alive until the launch)
+        k, k_at, k0, k1 = _rows(k)
+        v, v_at, v0, v1 = _rows(v)
+        out = queries
+        q_at = out_at = None
+        q0 = q1 = q_heads = 0
+        if queries is not None:
+            shape = self._check_rows(queries, None, "queries")
+            if shape[0] != tokens or queries.dtype is not dtype:
+                raise ValueError(f"queries: [{tokens}, q_heads, {self.head_dim}] {dtype}")
+            if rot:
+                queries, q_at, q0, q1 = _rows(queries)
+                out = torch.empty_like(queries, memory_format=torch.contiguous_format)
+                q_heads, out_at = shape[1], out.data_ptr()
+        on_device(index, self._l.vdb_kv_append_device, self._m, batch, t, k_at, k0, k1, v_at, v0, v1, cos_at, sin_at, positions, rot, interleaved,
+                  q_at, q0, q1, q_heads, out_at)
         return out
 
     def attend(self, q, table, lengths, *, offsets=None, max_new=None, scale=None, window: int = 0, select=None, return_lse: bool = False):
@@ -132,9 +149,8 @@ class KeyValueMemory:
         them; with ``select`` [sequences, kv_heads, n] int64 (one new token per sequence) it sees the tokens with these
         numbers, each as often as listed; numbers outside the sequence are skipped, as a search's padding is.
         ``scale`` is 1 / sqrt(head_dim) unless given."""
-        self._check_rows(q, None, "q")
+        tokens, q_heads, dim = self._check_rows(q, None, "q")
         t = dtype_code(q, "q")
-        tokens, q_heads, dim = q.shape
         if q_heads == 0 or q_heads % self.kv_heads:
             raise ValueError(f"q: a multiple of {self.kv_heads} heads")
         if window < 0:
@@ -144,26 +160,25 @@ class KeyValueMemory:
         if select is not None:
             if offsets is not None or window:
                 raise ValueError("select goes with one new token per sequence and no window")
-            if select.dtype != torch.int64 or select.dim() != 3 or tuple(select.shape[:2]) != (tokens, self.kv_heads) or select.device != self.device:
+            if select.dtype != torch.int64 or select.dim() != 3 or tuple(select.shape[:2]) != (tokens, self.kv_heads) or select.get_device() != self._index:
                 raise ValueError(f"select: int64 [{tokens}, {self.kv_heads}, n] on {self.device}")
             select = select.contiguous()
             n_select = select.shape[2]
             if n_select == 0:  # nothing to see: a list of one number that no sequence has
                 select, n_select = torch.full((tokens, self.kv_heads, 1), -1, dtype=torch.int64, device=self.device), 1
-        q = _rows(q)
+        q, q_at, q0, q1 = _rows(q)
         # rows of no sequence are zeros
-        make = torch.empty if offsets is None else torch.zeros
-        out = make((tokens, q_heads, dim), dtype=q.dtype, device=self.device)
-        lse = make((tokens, q_heads), dtype=torch.float32, device=self.device) if return_lse else None
+        device = self.device
+        out = (torch.empty_like if offsets is None else torch.zeros_like)(q, memory_format=torch.contiguous_format)
+        lse = (torch.empty if offsets is None else torch.zeros)((tokens, q_heads), dtype=_F32, device=device) if return_lse else None
         sizes = (self.kv_heads, self.page_tokens, dim, batch.count, batch.table_width, tokens, batch.max_new, offsets is None, q_heads, window, n_select)
         need = _needs.get(sizes)
         if need is None:
             if len(_needs) > 10000:
                 _needs.clear()
             need = _needs[sizes] = self._l.vdb_kv_attend_workspace(self._m, batch, q_heads, window, n_select)
-        work = torch.empty(need, dtype=torch.uint8, device=self.device) if need else None
-        qs = q.stride()
-        on_device(self.device, self._l.vdb_kv_attend_device, self._m, batch, t, q.data_ptr(), qs[0], qs[1], q_heads,
+        work = torch.empty(need, dtype=torch.uint8, device=device) if need else None
+        on_device(self._index, self._l.vdb_kv_attend_device, self._m, batch, t, q_at, q0, q1, q_heads,
                   float(dim) ** -0.5 if scale is None else float(scale), window, None if select is None else select.data_ptr(), n_select,
                   out.data_ptr(), None if lse is None else lse.data_ptr(), None if work is None else work.data_ptr(), need)
         return (out, lse) if return_lse else out

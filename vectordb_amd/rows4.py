@@ -20,18 +20,20 @@ def dtype_code(t, what: str) -> int:
     return code
 
 
-def on_device(device, call, *args) -> None:
-    """Calls ``call(*args, stream)`` with ``device`` current, on torch's current stream of it (as a number:
+def on_device(index, call, *args) -> None:
+    """Calls ``call(*args, stream)`` with device ``index`` current, on torch's current stream of it (as a number:
     torch.cuda.current_stream, which makes an object of it, costs the host 7 us a call)."""
-    index, current = device.index, torch._C._cuda_getDevice()
+    current = torch._C._cuda_getDevice()
     if current == index:
-        check(call(*args, torch._C._cuda_getCurrentRawStream(index)))
-        return
-    torch.cuda.set_device(index)
-    try:
-        check(call(*args, torch._C._cuda_getCurrentRawStream(index)))
-    finally:
-        torch.cuda.set_device(current)
+        status = call(*args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        torch.cuda.set_device(index)
+        try:
+            status = call(*args, torch._C._cuda_getCurrentRawStream(index))
+        finally:
+            torch.cuda.set_device(current)
+    if status:
+        check(status)
 
 
 class Rows4:
@@ -63,7 +65,7 @@ class Rows4:
         groups = (dim + 31) // 32
         out = cls(torch.empty((n, groups * 16), dtype=torch.uint8, device=rows.device),
                   torch.empty((n, groups), dtype=torch.uint8, device=rows.device), dim)
-        on_device(rows.device, out._l.vdb_rows4_pack_device, rows.data_ptr(), t, n, dim, rows.stride(0), out.codes.data_ptr(), out.scales.data_ptr())
+        on_device(rows.get_device(), out._l.vdb_rows4_pack_device, rows.data_ptr(), t, n, dim, rows.stride(0), out.codes.data_ptr(), out.scales.data_ptr())
         return out
 
     def __len__(self) -> int:
@@ -72,7 +74,7 @@ class Rows4:
     def unpack(self):
         """The values that the codes stand for, [n, dim] float32."""
         out = torch.empty((len(self), self.dim), dtype=torch.float32, device=self.codes.device)
-        on_device(out.device, self._l.vdb_rows4_unpack_device, self.codes.data_ptr(), self.scales.data_ptr(), len(self), self.dim, out.data_ptr())
+        on_device(out.get_device(), self._l.vdb_rows4_unpack_device, self.codes.data_ptr(), self.scales.data_ptr(), len(self), self.dim, out.data_ptr())
         return out
 
     def products(self, queries, out=None):
@@ -88,6 +90,6 @@ class Rows4:
             out = torch.empty((nq, n) if queries.dim() == 2 else (n,), dtype=torch.float32, device=x.device)
         elif out.dtype != torch.float32 or out.device != x.device or out.numel() != nq * n or not out.is_contiguous():
             raise ValueError(f"out: a contiguous float32 tensor of {nq} x {n} on {x.device}")
-        on_device(x.device, self._l.vdb_rows4_products_device, self.codes.data_ptr(), self.scales.data_ptr(), n, self.dim, x.data_ptr(), t, nq, x.stride(0),
+        on_device(x.get_device(), self._l.vdb_rows4_products_device, self.codes.data_ptr(), self.scales.data_ptr(), n, self.dim, x.data_ptr(), t, nq, x.stride(0),
                   out.data_ptr())
         return out

@@ -87,7 +87,7 @@ __device__ __forceinline__ uint32_t nan_bytes(uint32_t x) { return ~(((x & 0x7F7
 template <int T, int DS>
 struct Shape {
     static constexpr int D = DS * 32, ND = DS * 2, LDO = D + 4;
-    static constexpr size_t lds = (size_t)4 * 16 * LDO * 4 + 2 * 4 * 16 * 4;
+    static constexpr size_t lds(int waves) { return (size_t)waves * 16 * LDO * 4 + 2 * waves * 16 * 4; }
 };
 
 // The dimensions are cut into chunks of 128, 64 and 32, of which a lane holds 8, 4 and 2 neighbours: chunk c of DS.
@@ -108,6 +108,7 @@ struct Plan {
     uint32_t chunk;
     float* part;      // [sequence][head][tile][split][16][D + 2]
     uint32_t max_new;
+    bool wide;        // blocks of eight waves instead of four
     bool many;        // kv_attend_many, which needs none of the above
 };
 
@@ -163,11 +164,12 @@ constexpr int attend_waves(int t, int ds, int mode) {
     return ds <= 2 ? 4 : ds <= 4 ? 3 : ds <= 6 || mode == kSelected ? 2 : 1;
 }
 
-template <int T, int DS, int MODE>
-__global__ __launch_bounds__(256, attend_waves(T, DS, MODE)) void kv_attend(KvAttendArgs a, Plan plan) {
+template <int T, int DS, int MODE, int WAVES>
+__global__ __launch_bounds__(WAVES * 64, attend_waves(T, DS, MODE)) void kv_attend(KvAttendArgs a, Plan plan) {
     constexpr bool HALF = T == kF16, SEL = MODE == kSelected;
     constexpr int NQ = T == kF32 ? 3 : 1, NP = Parts<T>::value, D = DS * 32, ND = DS * 2, LDO = Shape<T, DS>::LDO;
     constexpr int VW = DS / 4 * 2 + (DS >> 1 & 1) + (DS & 1);  // words of a value that a lane holds
+    constexpr int STEP = WAVES * 32;  // tokens that a block takes at a time
     extern __shared__ float smem[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int m = lane & 15, q4 = lane >> 4;
@@ -221,18 +223,19 @@ __global__ __launch_bounds__(256, attend_waves(T, DS, MODE)) void kv_attend(KvAt
         };
         // Selected: lane l (and l + 32) looks place kb + (l & 31) of the list up, in three steps one tile apart, so that none
         // of the loads is waited for: token number, page number, then row and scales into the wave's table (two, in turn).
-        int64_t* rows_s = (int64_t*)smem + wave * 128;       // [2][32] row numbers, -1: none
+        int64_t* rows_s = (int64_t*)smem + wave * 128;       // [2][32] first bytes of rows (of row 0 for tokens that are not there)
         float* scales_s = (float*)smem + wave * 256 + 128;   // [2][64] key scales, value scales
         auto listed = [&](int32_t kb) -> int64_t {
             const int32_t i = kb + (lane & 31);
             return i < kb1 ? select[i] : -1;
         };
         auto paged = [&](int64_t t) -> int32_t { return t >= 0 && t < s.len ? a.batch.table[(uint64_t)b * a.batch.table_width + (t >> a.mem.page_shift)] : -1; };
-        auto placed = [&](int64_t t, int32_t page, int slot) {
+        auto placed = [&](int64_t t, int32_t page, int slot) -> uint32_t {
             const bool there = (uint32_t)page < (uint32_t)a.mem.pages;
             const int64_t ph = (int64_t)page * H + head;
-            if (lane < 32) rows_s[slot * 32 + lane] = there ? (ph << a.mem.page_shift) + (t & (P - 1)) : -1;
+            if (lane < 32) rows_s[slot * 32 + lane] = there ? ((ph << a.mem.page_shift) + (t & (P - 1))) * D : 0;
             scales_s[slot * 64 + lane] = there ? (lane < 32 ? a.mem.k_scale : a.mem.v_scale)[ph] : 0.0f;
+            return (uint32_t)__ballot(there);  // bit t: token t of the tile is there
         };
 
         u32x2 kw[2][DS];
@@ -240,24 +243,24 @@ __global__ __launch_bounds__(256, attend_waves(T, DS, MODE)) void kv_attend(KvAt
         auto load_keys = [&](int32_t kb, int32_t p0, int32_t p1, int slot) {
             int64_t row[2];
             if constexpr (SEL) {
-                row[0] = max(rows_s[slot * 32 + (m >> 2) * 8 + (m & 3)], (int64_t)0);
-                row[1] = max(rows_s[slot * 32 + (m >> 2) * 8 + 4 + (m & 3)], (int64_t)0);
+                row[0] = rows_s[slot * 32 + (m >> 2) * 8 + (m & 3)];
+                row[1] = rows_s[slot * 32 + (m >> 2) * 8 + 4 + (m & 3)];
             } else {
                 const int64_t r0 = (((int64_t)max(p0, 0) * H + head) << a.mem.page_shift) + (kb & (P - 1));
                 const int64_t r1 = (((int64_t)max(p1, 0) * H + head) << a.mem.page_shift) + ((kb + 16) & (P - 1)) - 16;
-                row[0] = (m < 8 ? r0 : r1) + (m >> 2) * 8 + (m & 3);
-                row[1] = row[0] + 4;
+                row[0] = ((m < 8 ? r0 : r1) + (m >> 2) * 8 + (m & 3)) * D;
+                row[1] = row[0] + 4 * D;
             }
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
-                const uint8_t* p = kc + row[t] * D + (DS > 1 ? q4 * 16 : 0);
+                const uint8_t* p = kc + row[t] + (DS > 1 ? q4 * 16 : 0);
 #pragma unroll
                 for (int j = 0; j + 1 < DS; j += 2) {
                     const u32x4 w = *(const u32x4*)(p + j * 32);
                     kw[t][j] = u32x2{w[0], w[1]};
                     kw[t][j + 1] = u32x2{w[2], w[3]};
                 }
-                if constexpr (DS & 1) kw[t][DS - 1] = *(const u32x2*)(kc + row[t] * D + key_byte<DS>(q4, DS - 1));
+                if constexpr (DS & 1) kw[t][DS - 1] = *(const u32x2*)(kc + row[t] + key_byte<DS>(q4, DS - 1));
             }
         };
         auto load_values = [&](int32_t kb, int32_t p0, int32_t p1, int slot) {
@@ -265,11 +268,11 @@ __global__ __launch_bounds__(256, attend_waves(T, DS, MODE)) void kv_attend(KvAt
             if constexpr (!SEL) {
                 const int64_t r0 = (((int64_t)max(p0, 0) * H + head) << a.mem.page_shift) + (kb & (P - 1));
                 const int64_t r1 = (((int64_t)max(p1, 0) * H + head) << a.mem.page_shift) + ((kb + 16) & (P - 1)) - 16;
-                first = (q4 < 2 ? r0 : r1) + q4 * 8;
+                first = ((q4 < 2 ? r0 : r1) + q4 * 8) * D;
             }
 #pragma unroll
             for (int t = 0; t < 8; ++t) {
-                const uint8_t* p = vc + (SEL ? max(rows_s[slot * 32 + q4 * 8 + t], (int64_t)0) : first + t) * D;
+                const uint8_t* p = vc + (SEL ? rows_s[slot * 32 + q4 * 8 + t] : first + t * D);
 #pragma unroll
                 for (int c = 0; c < DS / 4; ++c) {
                     const u32x2 y = *(const u32x2*)(p + c * 128 + m * 8);
@@ -310,23 +313,24 @@ __global__ __launch_bounds__(256, attend_waves(T, DS, MODE)) void kv_attend(KvAt
         int64_t t1 = -1, t2 = -1;                    // selected: tokens of the next tile and of the one after it
         int32_t g1 = -1;                             // page of the next tile's token
         int slot = 0;
+        uint32_t here = 0, next = 0;                 // selected: which tokens of this tile, and of the next, are there
         if (kb < kb1) {
             if constexpr (SEL) {
                 const int64_t t0 = listed(kb);
-                t1 = listed(kb + 128);
-                t2 = listed(kb + 256);
+                t1 = listed(kb + STEP);
+                t2 = listed(kb + 2 * STEP);
                 const int32_t g0 = paged(t0);
                 g1 = paged(t1);
-                placed(t0, g0, 0);
+                here = placed(t0, g0, 0);
                 __builtin_amdgcn_wave_barrier();
             } else {
                 p0 = page_of(kb), p1 = page_of(kb + 16);
-                n0 = page_of(kb + 128), n1 = page_of(kb + 144);
+                n0 = page_of(kb + STEP), n1 = page_of(kb + STEP + 16);
             }
             load_keys(kb, p0, p1, 0);
         }
-        for (; kb < kb1; kb += 128) {
-            const bool more = kb + 128 < kb1;
+        for (; kb < kb1; kb += STEP) {
+            const bool more = kb + STEP < kb1;
             load_values(kb, p0, p1, slot);
             float ks[SEL ? 8 : 1], vs[SEL ? 8 : 1];
             uint32_t have = 0;  // bit t: token t of the lane's 8 is there, and in the range that some row sees
@@ -334,16 +338,16 @@ __global__ __launch_bounds__(256, attend_waves(T, DS, MODE)) void kv_attend(KvAt
             if constexpr (SEL) {
 #pragma unroll
                 for (int t = 0; t < 8; ++t) {
-                    have |= (rows_s[slot * 32 + q4 * 8 + t] >= 0 ? 1u : 0u) << t;
                     ks[t] = scales_s[slot * 64 + q4 * 8 + t];
                     vs[t] = scales_s[slot * 64 + 32 + q4 * 8 + t];
                 }
-                full = __all(have == 255);
+                have = here >> (q4 * 8) & 255u;
+                full = here == 0xFFFFFFFFu;
                 if (more) {
-                    placed(t1, g1, slot ^ 1);
+                    next = placed(t1, g1, slot ^ 1);
                     g1 = paged(t2);
                     t1 = t2;
-                    t2 = listed(kb + 384);
+                    t2 = listed(kb + 3 * STEP);
                 }
                 __builtin_amdgcn_wave_barrier();
             } else {
@@ -373,7 +377,7 @@ __global__ __launch_bounds__(256, attend_waves(T, DS, MODE)) void kv_attend(KvAt
                 }
             }
             // the keys of the next tile travel while the values of this one are worked on
-            if (more) load_keys(kb + 128, n0, n1, slot ^ 1);
+            if (more) load_keys(kb + STEP, n0, n1, slot ^ 1);
             // ---- softmax over what the lane's row sees of its 8 tokens
             float p[8];
 #pragma unroll
@@ -488,14 +492,15 @@ __global__ __launch_bounds__(256, attend_waves(T, DS, MODE)) void kv_attend(KvAt
                 values(std::false_type());
             }
             p0 = n0, p1 = n1;
-            if constexpr (!SEL) n0 = page_of(kb + 256), n1 = page_of(kb + 272);
+            if constexpr (!SEL) n0 = page_of(kb + 2 * STEP), n1 = page_of(kb + 2 * STEP + 16);
             slot ^= 1;
+            here = next;
         }
 
-        // ---- join the four waves: each row's maximum, then sums and outputs in wave order
-        float* so = smem;                 // [4][16][LDO]
-        float* st = smem + 4 * 16 * LDO;  // [4][16] maxima
-        float* ss = st + 64;              // [4][16] sums
+        // ---- join the waves: each row's maximum, then sums and outputs in wave order
+        float* so = smem;                     // [WAVES][16][LDO]
+        float* st = smem + WAVES * 16 * LDO;  // [WAVES][16] maxima
+        float* ss = st + WAVES * 16;          // [WAVES][16] sums
         sum += __shfl_xor(sum, 16);
         sum += __shfl_xor(sum, 32);
         if (SEL) __syncthreads();  // the look-up tables of the waves lie there as well
@@ -513,20 +518,20 @@ __global__ __launch_bounds__(256, attend_waves(T, DS, MODE)) void kv_attend(KvAt
         const int row = threadIdx.x >> 4, part = threadIdx.x & 15;
         float best = kNone;
 #pragma unroll
-        for (int w = 0; w < 4; ++w) best = __builtin_fmaxf(best, st[w * 16 + row]);
-        float f[4], total = 0.0f;
+        for (int w = 0; w < WAVES; ++w) best = __builtin_fmaxf(best, st[w * 16 + row]);
+        float f[WAVES], total = 0.0f;
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
+        for (int w = 0; w < WAVES; ++w) {
             f[w] = __builtin_amdgcn_exp2f(st[w * 16 + row] - best);
             total += f[w] * ss[w * 16 + row];
         }
-        if (row0 + row < rows) {
+        if (row < 16 && row0 + row < rows) {  // (16 threads a row: the first four waves)
             float v[ND];
 #pragma unroll
             for (int d = 0; d < ND; ++d) {
                 v[d] = 0.0f;
 #pragma unroll
-                for (int w = 0; w < 4; ++w) v[d] += f[w] * so[(w * 16 + row) * LDO + part * ND + d];
+                for (int w = 0; w < WAVES; ++w) v[d] += f[w] * so[(w * 16 + row) * LDO + part * ND + d];
             }
             if (whole) {
                 const int64_t ot = (row0 + row) / G;
@@ -1184,9 +1189,16 @@ hipError_t launch_one(const KvAttendArgs& a, const Plan& plan, hipStream_t strea
         return hipGetLastError();
     }
     const dim3 grid(plan.tiles * plan.splits, a.mem.heads, a.batch.count);
-    if (a.select) hipLaunchKernelGGL((kv_attend<T, DS, kSelected>), grid, dim3(256), (Shape<T, DS>::lds), stream, a, plan);
-    else if (!a.batch.offsets) hipLaunchKernelGGL((kv_attend<T, DS, kSingle>), grid, dim3(256), (Shape<T, DS>::lds), stream, a, plan);
-    else hipLaunchKernelGGL((kv_attend<T, DS, kChunks>), grid, dim3(256), (Shape<T, DS>::lds), stream, a, plan);
+    auto launch = [&](auto kernel, int waves) { hipLaunchKernelGGL(kernel, grid, dim3(waves * 64), (Shape<T, DS>::lds(waves)), stream, a, plan); };
+    if constexpr (T != kF32 || DS <= 5) {  // (f32 in more dimensions: 256 registers a lane are too few)
+        if (plan.wide) {
+            launch(kv_attend<T, DS, kSelected, 8>, 8);
+            return hipGetLastError();
+        }
+    }
+    if (a.select) launch(kv_attend<T, DS, kSelected, 4>, 4);
+    else if (!a.batch.offsets) launch(kv_attend<T, DS, kSingle, 4>, 4);
+    else launch(kv_attend<T, DS, kChunks, 4>, 4);
     return hipGetLastError();
 }
 
@@ -1223,12 +1235,16 @@ Plan plan_of(const KvAttendArgs& a, uint32_t max_new) {
     if (!a.n_select && a.window) tokens = std::min<uint64_t>(tokens, (uint64_t)a.window + max_new + 31);
     const uint64_t blocks = (uint64_t)p.tiles * a.mem.heads * a.batch.count;
     // As many ranges as give some 12 blocks a CU, four times what the chip holds at once: sequences of different lengths even out
-    // (64 of 1 000 to 8 192 tokens, 8 heads: 147 us at 4 a CU, 130 at 6, 121 at 12, 125 at 16).  But no range
-    // shorter than 512 tokens (selected ones: 1024), where a block's start and end begin to count (500 tokens in one block 9.4 us,
-    // in four 6.0 and 4.4 for the join; 2048 selected ones in two ranges 40 us, in four 46), and at most 384 of one row, or the
-    // join counts (two sequences of 500 003: 384 ranges 103 + 10 us, 768 104 + 17, 256 109 + 8).
+    // (64 of 1 000 to 8 192 tokens, 8 heads: 147 us at 4 a CU, 130 at 6, 121 at 12, 125 at 16).  But no range shorter than 512
+    // tokens, where a block's start and end begin to count (500 tokens in one block 9.4 us, in four 6.0 and 4.4 for the join), and
+    // at most 384 of one row, or the join counts (two sequences of 500 003: 384 ranges 103 + 10 us, 768 104 + 17, 256 109 + 8).
+    // Selected tokens, whose rows and places take longer to come: where there are few rows, blocks of eight waves and ranges of
+    // 2048, or 1024 if that leaves half of the chip idle (32 sequences x 8 heads x 2048 tokens in f32: 37 us in two ranges of
+    // four waves and a join, 32 in one of eight; 1 x 8 x 2048 22.8, 24.4 in one range of eight, 19.0 in two; 64 x 8 x 2048 in bf16 76 and
+    // 66, but 48 x 8 x 2048 49 and 57: one and a half rounds of blocks).
     const uint64_t want = std::min<uint64_t>(384, std::max<uint64_t>(1, 12 * 256 / blocks));
-    uint64_t chunk = std::max<uint64_t>(a.n_select ? 1024 : 512, (tokens + want - 1) / want);
+    p.wide = a.n_select && blocks <= 512;
+    uint64_t chunk = std::max<uint64_t>(!a.n_select ? 512 : blocks >= 128 && p.wide ? 2048 : 1024, (tokens + want - 1) / want);
     chunk = (chunk + 127) / 128 * 128;
     p.chunk = (uint32_t)std::min<uint64_t>(chunk, 1u << 30);
     p.splits = (uint32_t)std::max<uint64_t>(1, (tokens + p.chunk - 1) / p.chunk);

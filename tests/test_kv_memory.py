@@ -821,3 +821,20 @@ def test_attend_scales_far_apart(dtype, new):
     table, lengths = s.on_gpu()
     out, lse = mem.attend(q.cuda(), table, lengths, offsets=None if max(new) == 1 else ints(off), max_new=max(new), return_lse=True)
     check_attend(out, lse, attend_ref(q, s.k, s.v, s.ks, s.vs, s.table, held, off, page, dim ** -0.5), t)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,dim", [("f32", 64), ("bf16", 128), ("f32", 192)])
+@pytest.mark.parametrize("count,heads,n", [(19, 2, 70), (8, 3, 2500), (130, 4, 40)])
+def test_attend_selected_batches(dtype, dim, count, heads, n):
+    """More sequences than dies, and a rest; lists in one range and in several; few rows and many."""
+    page, hq = 16, 2 * heads
+    r = np.random.default_rng(n)
+    held = [int(x) for x in r.integers(0, 200, count)]
+    s = Setup(held, page, heads, dim, seed=n)
+    q = s.randn(count, hq, dim, dtype=TYPES[dtype])
+    select = torch.randint(-5, 220, (count, heads, n), generator=s.g)
+    mem = s.memory()
+    table, lengths = s.on_gpu()
+    out, lse = mem.attend(q.cuda(), table, lengths, select=select.cuda(), return_lse=True)
+    check_attend(out, lse, attend_ref(q, s.k, s.v, s.ks, s.vs, s.table, held, list(range(count + 1)), page, dim ** -0.5, 0, select), TYPES[dtype])

@@ -52,7 +52,8 @@ class KeyValueMemory:
         return self
 
     def _take(self, k, v, k_scale, v_scale):
-        if k.dim() != 4 or k.shape != v.shape or k_scale.shape != k.shape[:2] or v_scale.shape != k.shape[:2]:
+        shape = k.shape
+        if len(shape) != 4 or v.shape != shape or k_scale.shape != shape[:2] or v_scale.shape != shape[:2]:
             raise ValueError("expected k, v [pages, kv_heads, page_tokens, head_dim] and k_scale, v_scale [pages, kv_heads]")
         if k.dtype is not _E4M3 or v.dtype is not _E4M3 or k_scale.dtype is not _F32 or v_scale.dtype is not _F32:
             raise ValueError("k, v: float8_e4m3fn; k_scale, v_scale: float32")
@@ -61,7 +62,7 @@ class KeyValueMemory:
             raise ValueError("k, v, k_scale, v_scale: CUDA tensors on one device")
         if not (k.is_contiguous() and v.is_contiguous() and k_scale.is_contiguous() and v_scale.is_contiguous()):
             raise ValueError("k, v, k_scale, v_scale must be contiguous")
-        pages, heads, page_tokens, dim = k.shape
+        pages, heads, page_tokens, dim = shape
         if page_tokens < 16 or page_tokens > 1024 or page_tokens & (page_tokens - 1):
             raise ValueError("page_tokens must be a power of two in 16..1024")
         if dim < 32 or dim > 256 or dim % 32:

@@ -10,6 +10,7 @@ import torch
 from . import _lib
 from ._lib import BF16, F16, F32, check
 
+_U8, _F32 = torch.uint8, torch.float32
 _codes = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
 
 
@@ -41,17 +42,20 @@ class Rows4:
     layout that include/vdb_index.h describes: e2m1 codes, a power-of-two scale for every 32 columns of a row."""
 
     def __init__(self, codes, scales, dim: int):
-        groups = (int(dim) + 31) // 32
+        dim = int(dim)
+        groups, index = (dim + 31) // 32, codes.get_device()
         if dim < 1:
             raise ValueError("dim must be positive")
-        if codes.dtype != torch.uint8 or scales.dtype != torch.uint8 or not codes.is_cuda or codes.device != scales.device:
+        if codes.dtype is not _U8 or scales.dtype is not _U8 or not codes.is_cuda or scales.get_device() != index:
             raise ValueError("codes and scales: uint8 CUDA tensors on one device")
-        if codes.dim() != 2 or tuple(codes.shape) != (scales.shape[0], groups * 16) or tuple(scales.shape[1:]) != (groups,):
-            raise ValueError(f"expected codes [n, {groups * 16}] and scales [n, {groups}], got {tuple(codes.shape)} and {tuple(scales.shape)}")
+        shape = codes.shape
+        if len(shape) != 2 or shape[1] != groups * 16 or scales.shape != (shape[0], groups):
+            raise ValueError(f"expected codes [n, {groups * 16}] and scales [n, {groups}], got {tuple(shape)} and {tuple(scales.shape)}")
         if not (codes.is_contiguous() and scales.is_contiguous()):
             raise ValueError("codes and scales must be contiguous")
         self._l = _lib.lib()
-        self.codes, self.scales, self.dim = codes, scales, int(dim)
+        self.codes, self.scales, self.dim = codes, scales, dim
+        self._n, self._index = shape[0], index
 
     @classmethod
     def pack(cls, rows) -> "Rows4":
@@ -69,7 +73,7 @@ class Rows4:
         return out
 
     def __len__(self) -> int:
-        return self.codes.shape[0]
+        return self._n
 
     def unpack(self):
         """The values that the codes stand for, [n, dim] float32."""
@@ -79,17 +83,19 @@ class Rows4:
 
     def products(self, queries, out=None):
         """Inner products of queries [nq, dim] (or [dim]) with every row: [nq, n] (or [n]) float32, into ``out`` if given (no gradient)."""
+        index, n = self._index, self._n
         x = queries if queries.dim() == 2 else queries.unsqueeze(0)
-        if queries.dim() not in (1, 2) or x.shape[1] != self.dim or x.device != self.codes.device:
+        if queries.dim() not in (1, 2) or x.shape[1] != self.dim or x.get_device() != index:
             raise ValueError(f"expected queries [nq, {self.dim}] on {self.codes.device}, got {tuple(queries.shape)} on {queries.device}")
         t = dtype_code(x, "queries")
-        if x.stride(1) != 1 or x.stride(0) < 0:
+        step, one = x.stride()
+        if one != 1 or step < 0:
             x = x.contiguous()
-        nq, n = x.shape[0], len(self)
+            step = x.stride(0)
+        nq = x.shape[0]
         if out is None:
-            out = torch.empty((nq, n) if queries.dim() == 2 else (n,), dtype=torch.float32, device=x.device)
-        elif out.dtype != torch.float32 or out.device != x.device or out.numel() != nq * n or not out.is_contiguous():
+            out = torch.empty((nq, n) if queries.dim() == 2 else (n,), dtype=_F32, device=x.device)
+        elif out.dtype is not _F32 or out.get_device() != index or out.numel() != nq * n or not out.is_contiguous():
             raise ValueError(f"out: a contiguous float32 tensor of {nq} x {n} on {x.device}")
-        on_device(x.get_device(), self._l.vdb_rows4_products_device, self.codes.data_ptr(), self.scales.data_ptr(), n, self.dim, x.data_ptr(), t, nq, x.stride(0),
-                  out.data_ptr())
+        on_device(index, self._l.vdb_rows4_products_device, self.codes.data_ptr(), self.scales.data_ptr(), n, self.dim, x.data_ptr(), t, nq, step, out.data_ptr())
         return out

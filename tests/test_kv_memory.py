@@ -838,3 +838,47 @@ def test_attend_selected_batches(dtype, dim, count, heads, n):
     table, lengths = s.on_gpu()
     out, lse = mem.attend(q.cuda(), table, lengths, select=select.cuda(), return_lse=True)
     check_attend(out, lse, attend_ref(q, s.k, s.v, s.ks, s.vs, s.table, held, list(range(count + 1)), page, dim ** -0.5, 0, select), TYPES[dtype])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["chunks", "many", "selected", "ranges"])
+def test_attend_captured_and_on_two_streams(kind):
+    """Each way of attention captured once and replayed with other lengths, eager calls in between on two streams at a time: every
+    result is, bit for bit, that of the same call alone."""
+    page, heads, hq, dim = 16, 8, 32, 64
+    new = dict(chunks=[20, 7], many=[300, 200], selected=[1, 1], ranges=[1, 1])[kind]
+    s = Setup([1900, 1400], page, heads, dim, seed=22)
+    off = offsets_of(new)
+    mem = s.memory()
+    table, lengths = s.on_gpu()
+    offsets = None if max(new) == 1 else ints(off)
+    select = torch.randint(-3, 2000, (2, heads, 3000), generator=s.g).cuda() if kind == "selected" else None
+    q = s.randn(off[-1], hq, dim, dtype=torch.bfloat16).cuda()
+
+    def step(lengths):
+        return mem.attend(q, table, lengths, offsets=offsets, max_new=max(new), select=select, return_lse=True)
+
+    held = [[1900, 1400], [600, 1399], [350, 230], [1, 1000], [0, 0], [1700, 320]]
+    alone = [step(ints(h)) for h in held]
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(lengths)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step(lengths)
+    other = [ints(h) for h in held]
+    torch.cuda.synchronize()
+    for turn_ in range(2):
+        for i, h in enumerate(held):
+            lengths.copy_(other[i])
+            graph.replay()
+            with torch.cuda.stream(side):
+                b = [step(x) for x in other]
+            a = [step(x) for x in other]
+            torch.cuda.synchronize()
+            assert all(torch.equal(x, y) for x, y in zip(got, alone[i]))
+            for results in (a, b):
+                assert all(torch.equal(x, y) for r, w in zip(results, alone) for x, y in zip(r, w))

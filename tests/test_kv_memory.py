@@ -882,3 +882,18 @@ def test_attend_captured_and_on_two_streams(kind):
             assert all(torch.equal(x, y) for x, y in zip(got, alone[i]))
             for results in (a, b):
                 assert all(torch.equal(x, y) for r, w in zip(results, alone) for x, y in zip(r, w))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("dim,held", [(32, [8000, 5, 3100]), (96, [9000, 513]), (160, [7900]), (256, [9100, 4096, 0]), (64, [40_000, 700, 1])])
+def test_attend_ranges_joined(dtype, dim, held):
+    """One token over so much that its tokens are cut into up to 16 ranges, or more: their joints, for each way of joining."""
+    page, heads, hq = 64, 2, 6
+    s = Setup(held, page, heads, dim, seed=dim)
+    q = s.randn(len(held), hq, dim, dtype=TYPES[dtype]) * 3
+    mem = s.memory()
+    table, lengths = s.on_gpu()
+    out, lse = mem.attend(q.cuda(), table, lengths, return_lse=True)
+    ref = attend_ref(q, s.k, s.v, s.ks, s.vs, s.table, held, list(range(len(held) + 1)), page, dim ** -0.5)
+    check_attend(out, lse, ref, TYPES[dtype])

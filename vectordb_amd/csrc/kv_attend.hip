@@ -100,7 +100,7 @@ struct Chunks {
 };
 
 // Work of one launch.  The tokens of a row tile are cut into `splits` ranges of `chunk` (a multiple of 128), one block each;
-// where more than one range holds tokens, the blocks leave (maximum, sum, output) in the workspace and kv_join adds them up
+// where more than one range holds tokens, the blocks leave (maximum, sum, output) in the workspace and kv_join_* adds them up
 // in the order of the ranges.
 struct Plan {
     uint32_t tiles;   // row tiles of 16 that have blocks of their own (more than that are walked by the blocks of range 0)
@@ -1120,14 +1120,70 @@ __global__ __launch_bounds__((Many<T, DS>::kThreads), (Many<T, DS>::occupancy)) 
     }
 }
 
-// Adds up the ranges of one row: block (row, head, sequence).  Every thread has four of its loads in flight.
-template <int T, bool SEL, int kJoinThreads>
-__global__ __launch_bounds__(kJoinThreads) void kv_join(KvAttendArgs a, Plan plan) {
-    __shared__ float red[kJoinThreads * 4], mx[kJoinThreads / 64], sums[64];
+// Adds up the ranges of a row, of which there are at most 16: a wave a row, lane i weighs range i, then each lane adds up two or
+// four dimensions, in the order of the ranges.
+template <int T, bool SEL>
+__global__ __launch_bounds__(256) void kv_join_few(KvAttendArgs a, Plan plan) {
     const uint32_t b = blockIdx.z, head = blockIdx.y, H = a.mem.heads, G = a.q_heads / H, D = a.mem.dim;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     Sequence s;
     if (!sequence_of(a, b, s)) return;
-    const int64_t row = blockIdx.x, rows = (int64_t)s.n_new * G, rt = row / 16;
+    const int64_t row = (int64_t)blockIdx.x * 4 + wave, rows = min((int64_t)s.n_new * G, (int64_t)plan.tiles * 16), rt = row / 16;
+    if (row >= rows) return;
+    int32_t lo, hi;
+    range_of<SEL>(a, s, s.start + (int32_t)(rt * 16 / G), s.start + (int32_t)(min(rt * 16 + 15, (int64_t)s.n_new * G - 1) / G), lo, hi);
+    lo &= ~31;
+    if (hi - lo <= (int32_t)plan.chunk) return;  // written by kv_attend
+    const uint32_t used = min(((uint32_t)(hi - lo) + plan.chunk - 1) / plan.chunk, plan.splits);
+    const uint64_t step = 16 * (D + 2);
+    const float* part = plan.part + ((((uint64_t)b * H + head) * plan.tiles + rt) * plan.splits * 16 + row % 16) * (D + 2);
+    const f32x2 mine = (uint32_t)lane < used ? *(const f32x2*)(part + lane * step + D) : f32x2{kNone, 0.0f};
+    float best = mine[0];
+#pragma unroll
+    for (int o = 32; o; o >>= 1) best = __builtin_fmaxf(best, __shfl_xor(best, o));
+    const float f = (uint32_t)lane < used ? __builtin_amdgcn_exp2f(mine[0] - best) : 0.0f;
+    float sum = f * mine[1];
+#pragma unroll
+    for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o);
+    const uint32_t per = D > 128 ? 4 : 2, d = lane * per;
+    if (d >= D) return;
+    f32x2 acc[2] = {{0, 0}, {0, 0}};
+    for (uint32_t i = 0; i < used; i += 8) {
+        f32x2 x[8][2];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+            const float* w = part + (uint64_t)min(i + u, used - 1) * step + d;
+            x[u][0] = *(const f32x2*)w;
+            x[u][1] = per == 4 ? *(const f32x2*)(w + 2) : f32x2{0, 0};
+        }
+#pragma unroll
+        for (int u = 0; u < 8; ++u)
+            if (i + u < used) {
+                const float g = float_of(__builtin_amdgcn_readlane(bits_of(f), i + u));
+                acc[0] += x[u][0] * g;
+                acc[1] += x[u][1] * g;
+            }
+    }
+    const int64_t ot = row / G;
+    const uint64_t orow = (uint64_t)(s.first + ot) * a.q_heads + head * G + (uint32_t)(row - ot * G);
+    const bool none = sum == 0.0f;
+    const float inv = none ? 0.0f : 1.0f / sum;
+    E<T>* out = (E<T>*)a.out + orow * D + d;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        if (i < (int)per) out[i] = (E<T>)(none ? 0.0f : acc[i >> 1][i & 1] * inv);
+    if (a.lse && lane == 0) a.lse[orow] = none ? -__builtin_inff() : (best + __builtin_amdgcn_logf(sum)) * kLn2;
+}
+
+// The same for many ranges: a block takes 32 dimensions of a row, eight threads a range, so that 64 ranges are under way at a time.
+template <int T, bool SEL>
+__global__ __launch_bounds__(512) void kv_join_long(KvAttendArgs a, Plan plan) {
+    __shared__ float mx[8], sums[8];
+    __shared__ f32x4 red[8][8];
+    const uint32_t b = blockIdx.z, head = blockIdx.y, H = a.mem.heads, G = a.q_heads / H, D = a.mem.dim, cuts = D / 32;
+    Sequence s;
+    if (!sequence_of(a, b, s)) return;
+    const int64_t row = blockIdx.x / cuts, rows = (int64_t)s.n_new * G, rt = row / 16;
     if (row >= rows) return;
     int32_t lo, hi;
     range_of<SEL>(a, s, s.start + (int32_t)(rt * 16 / G), s.start + (int32_t)(min(rt * 16 + 15, rows - 1) / G), lo, hi);
@@ -1138,53 +1194,54 @@ __global__ __launch_bounds__(kJoinThreads) void kv_join(KvAttendArgs a, Plan pla
     const float* part = plan.part + ((((uint64_t)b * H + head) * plan.tiles + rt) * plan.splits * 16 + row % 16) * (D + 2);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     float best = kNone;
-    for (uint32_t i = threadIdx.x; i < used; i += kJoinThreads) best = __builtin_fmaxf(best, part[i * step + D]);
+    for (uint32_t i = threadIdx.x; i < used; i += 512) best = __builtin_fmaxf(best, part[i * step + D]);
 #pragma unroll
     for (int o = 32; o; o >>= 1) best = __builtin_fmaxf(best, __shfl_xor(best, o));
     if (lane == 0) mx[wave] = best;
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < kJoinThreads / 64; ++w) best = __builtin_fmaxf(best, mx[w]);
-    // groups of D / 4 threads, each thread four dimensions of every groups-th range
-    const uint32_t width = D / 4, groups = kJoinThreads / width, g = threadIdx.x / width, d = threadIdx.x % width * 4;
+    for (int w = 0; w < 8; ++w) best = __builtin_fmaxf(best, mx[w]);
+    const uint32_t g = threadIdx.x >> 3, d = blockIdx.x % cuts * 32 + (threadIdx.x & 7) * 4;
     f32x4 acc = {0, 0, 0, 0};
     float total = 0.0f;
-    if (g < groups) {
-        for (uint32_t i = g; i < used; i += 4 * groups) {
-            f32x2 x[4], y[4], z[4];
+    for (uint32_t i = g; i < used; i += 4 * 64) {
+        f32x2 x[4], y[4], z[4];
 #pragma unroll
-            for (int u = 0; u < 4; ++u) {
-                const float* w = part + (uint64_t)min(i + u * groups, used - 1) * step;
-                x[u] = *(const f32x2*)(w + d), y[u] = *(const f32x2*)(w + d + 2), z[u] = *(const f32x2*)(w + D);
-            }
+        for (int u = 0; u < 4; ++u) {
+            const float* w = part + (uint64_t)min(i + u * 64, used - 1) * step;
+            x[u] = *(const f32x2*)(w + d), y[u] = *(const f32x2*)(w + d + 2), z[u] = *(const f32x2*)(w + D);
+        }
 #pragma unroll
-            for (int u = 0; u < 4; ++u) {
-                if (i + u * groups < used) {
-                    const float f = __builtin_amdgcn_exp2f(z[u][0] - best);
-                    total += f * z[u][1];
-                    acc += f32x4{x[u][0], x[u][1], y[u][0], y[u][1]} * f;
-                }
+        for (int u = 0; u < 4; ++u) {
+            if (i + u * 64 < used) {
+                const float f = __builtin_amdgcn_exp2f(z[u][0] - best);
+                total += f * z[u][1];
+                acc += f32x4{x[u][0], x[u][1], y[u][0], y[u][1]} * f;
             }
         }
-        if (d == 0) sums[g] = total;
     }
-    *(f32x4*)(red + threadIdx.x * 4) = acc;
+#pragma unroll
+    for (int o = 32; o >= 8; o >>= 1) {
+        total += __shfl_xor(total, o);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[i] += __shfl_xor(acc[i], o);
+    }
+    if (lane < 8) red[wave][lane] = acc;
+    if (lane == 0) sums[wave] = total;
     __syncthreads();
-    if (threadIdx.x < width) {
+    if (threadIdx.x < 8) {
         float sum = 0.0f;
         f32x4 v = {0, 0, 0, 0};
-        for (uint32_t i = 0; i < groups; ++i) {
-            sum += sums[i];
-            v += *(const f32x4*)(red + (i * width + threadIdx.x) * 4);
-        }
+#pragma unroll
+        for (int w = 0; w < 8; ++w) sum += sums[w], v += red[w][threadIdx.x];
         const int64_t ot = row / G;
         const uint64_t orow = (uint64_t)(s.first + ot) * a.q_heads + head * G + (uint32_t)(row - ot * G);
         const bool none = sum == 0.0f;
         const float inv = none ? 0.0f : 1.0f / sum;
-        E<T>* out = (E<T>*)a.out + orow * D + threadIdx.x * 4;
+        E<T>* out = (E<T>*)a.out + orow * D + d;
 #pragma unroll
         for (int i = 0; i < 4; ++i) out[i] = (E<T>)(none ? 0.0f : v[i] * inv);
-        if (a.lse && threadIdx.x == 0) a.lse[orow] = none ? -__builtin_inff() : (best + __builtin_amdgcn_logf(sum)) * kLn2;
+        if (a.lse && d == 0) a.lse[orow] = none ? -__builtin_inff() : (best + __builtin_amdgcn_logf(sum)) * kLn2;
     }
 }
 
@@ -1215,9 +1272,10 @@ hipError_t launch_one(const KvAttendArgs& a, const Plan& plan, hipStream_t strea
 
 template <int T, bool SEL>
 void launch_join_of(const KvAttendArgs& a, const Plan& plan, const dim3& grid, hipStream_t stream) {
-    // 512 threads a row where there are many ranges (384: 10 us against 17), 256 where there are few (6: 6.3 us against 9.5)
-    if (plan.splits > 64) hipLaunchKernelGGL((kv_join<T, SEL, 512>), grid, dim3(512), 0, stream, a, plan);
-    else hipLaunchKernelGGL((kv_join<T, SEL, 256>), grid, dim3(256), 0, stream, a, plan);
+    // (a block of 256 threads a row: 6 ranges 6.9 us, a wave 5.2; 384 ranges 17, of 512 threads 9.7, cut into 32 dimensions 6.7; 32 of
+    // them, with the attention: 25.3 us with 256 threads a row, 23.2)
+    if (plan.splits <= 16) hipLaunchKernelGGL((kv_join_few<T, SEL>), dim3((grid.x + 3) / 4, grid.y, grid.z), dim3(256), 0, stream, a, plan);
+    else hipLaunchKernelGGL((kv_join_long<T, SEL>), dim3(grid.x * (a.mem.dim / 32), grid.y, grid.z), dim3(512), 0, stream, a, plan);
 }
 
 template <int T>
@@ -1247,8 +1305,8 @@ Plan plan_of(const KvAttendArgs& a, uint32_t max_new) {
     const uint64_t blocks = (uint64_t)p.tiles * a.mem.heads * a.batch.count;
     // As many ranges as give some 12 blocks a CU, four times what the chip holds at once: sequences of different lengths even out
     // (64 of 1 000 to 8 192 tokens, 8 heads: 147 us at 4 a CU, 130 at 6, 121 at 12, 125 at 16).  But no range shorter than 512
-    // tokens, where a block's start and end begin to count (500 tokens in one block 9.4 us, in four 6.0 and 4.4 for the join), and
-    // at most 384 of one row, or the join counts (two sequences of 500 003: 384 ranges 103 + 10 us, 768 104 + 17, 256 109 + 8).
+    // tokens, where a block's start and end begin to count (500 tokens in one block 9.4 us, in four 6.0 and 4 for the join), and
+    // at most 384 of one row, or the join counts (two sequences of 500 003: 384 ranges 103 us, 768 104, 256 109, and the join 6.7 at 384).
     // Selected tokens, whose rows and places take longer to come: where there are few rows, blocks of eight waves and ranges of
     // 2048, or 1024 if that leaves half of the chip idle (32 sequences x 8 heads x 2048 tokens in f32: 37 us in two ranges of
     // four waves and a join, 32 in one of eight; 1 x 8 x 2048 22.8, 24.4 in one range of eight, 19.0 in two; 64 x 8 x 2048 in bf16 76 and

@@ -897,3 +897,34 @@ def test_attend_ranges_joined(dtype, dim, held):
     out, lse = mem.attend(q.cuda(), table, lengths, return_lse=True)
     ref = attend_ref(q, s.k, s.v, s.ks, s.vs, s.table, held, list(range(len(held) + 1)), page, dim ** -0.5)
     check_attend(out, lse, ref, TYPES[dtype])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,interleaved", [("f32", False), ("bf16", True), ("f16", False)])
+def test_append_many_large_pages(dtype, interleaved):
+    """So many pages that keys and values are stored by launches of their own, with and without queries, turned and not."""
+    held, new, page, heads, dim, hq = [1100] * 8, [1000] * 8, 128, 32, 32, 32
+    off = offsets_of(new)
+    k, v, q = (Setup([1], 16, 1, 32, seed=23 + i).randn(off[-1], heads, dim, dtype=TYPES[dtype]) for i in range(3))
+    cos, sin = angles(1100, 16)
+    for rot in (True, False):
+        s = Setup(held, page, heads, dim, seed=24)
+        mem = s.memory()
+        table, lengths = s.on_gpu()
+        angle = dict(cos=cos.cuda(), sin=sin.cuda(), interleaved=interleaved) if rot else {}
+        got = mem.append(k.cuda(), v.cuda(), table, lengths, offsets=ints(off), max_new=1000, queries=q.cuda() if rot else None, **angle)
+        whole = s.memory()  # the same, one sequence a call
+        for b in range(8):
+            rows = slice(off[b], off[b + 1])
+            one = whole.append(k[rows].cuda(), v[rows].cuda(), table[b:b + 1], lengths[b:b + 1], offsets=ints([0, 1000]), max_new=1000,
+                               queries=q[rows].cuda() if rot else None, **angle)
+            assert not rot or torch.equal(one, got[rows])
+        assert same_codes(mem.k, whole.k.cpu()) and same_codes(mem.v, whole.v.cpu())
+        assert torch.equal(mem.k_scale, whole.k_scale) and torch.equal(mem.v_scale, whole.v_scale)
+        for b in (0, 7):  # and one of them by the formula
+            rows = slice(off[b], off[b + 1])
+            ref = Setup(held, page, heads, dim, seed=24)
+            append_ref(ref.k, ref.ks, k[rows], ref.table[b:b + 1], held[b:b + 1], [0, 1000], page, *((cos, sin, interleaved) if rot else ()))
+            append_ref(ref.v, ref.vs, v[rows], ref.table[b:b + 1], held[b:b + 1], [0, 1000], page)
+            at = ref.table[b][ref.table[b] >= 0].long()
+            assert same_codes(mem.k[at.cuda()], ref.k[at]) and same_codes(mem.v[at.cuda()], ref.v[at])

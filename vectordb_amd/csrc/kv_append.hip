@@ -342,19 +342,21 @@ __global__ __launch_bounds__(256) void kv_turn(KvAppendArgs a) {
     turn_queries<T, NEXT>(a, blockIdx.x * 4ull + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), gridDim.x * 4ull);
 }
 
-// One launch for both: blocks below store_blocks are (slot, side and head, sequence), a slot being one of the pages that a
+enum { kBoth = 0, kKeys = 1, kValues = 2 };  // sides that a launch stores (kKeys: turned)
+
+// One launch for all: blocks below store_blocks are (slot, side and head, sequence), a slot being one of the pages that a
 // sequence's new tokens touch; the others turn queries.
-template <int T, int NT, int NP8, bool NEXT>
-__global__ __launch_bounds__(NT, 4) void kv_append(KvAppendArgs a, uint32_t slots, uint32_t store_blocks) {
+template <int T, int NT, int NP8, bool NEXT, int SIDES>
+__global__ __launch_bounds__(NT, SIDES == kValues ? 6 : 4) void kv_append(KvAppendArgs a, uint32_t slots, uint32_t store_blocks) {
     __shared__ uint32_t red[NT / 64];
     if (blockIdx.x >= store_blocks) {
         const uint64_t per = NT / 64;
         turn_queries<T, NEXT>(a, (blockIdx.x - store_blocks) * per + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), (gridDim.x - store_blocks) * per);
         return;
     }
-    const uint32_t sides = 2 * a.mem.heads, slot = blockIdx.x % slots, rest = blockIdx.x / slots;
-    const uint32_t b = rest / sides, head = (rest % sides) >> 1;
-    const bool is_v = rest % sides & 1;
+    const uint32_t sides = (SIDES == kBoth ? 2 : 1) * a.mem.heads, slot = blockIdx.x % slots, rest = blockIdx.x / slots;
+    const uint32_t b = rest / sides, head = (rest % sides) >> (SIDES == kBoth);
+    const bool is_v = SIDES == kBoth ? rest % sides & 1 : SIDES == kValues;
     const Span s = span_of(a.batch, b);
     if (s.end <= s.start) return;
     const uint32_t P = a.mem.page_tokens, D = a.mem.dim;
@@ -375,8 +377,13 @@ __global__ __launch_bounds__(NT, 4) void kv_append(KvAppendArgs a, uint32_t slot
         uint8_t* page = (uint8_t*)(is_v ? a.mem.v : a.mem.k) + ((uint64_t)pid * a.mem.heads + head) * P * D;
         float* scale = (is_v ? a.mem.v_scale : a.mem.k_scale) + (uint64_t)pid * a.mem.heads + head;
         const E<T>* rows = src + (uint64_t)(s.first + p * P + r0 - s.start) * token_stride;
-        if (turn) store_page<T, NT, NP8, NEXT, true>(a, rows, token_stride, p * P, r0, r1, page, scale, red);
-        else store_page<T, NT, NP8, NEXT, false>(a, rows, token_stride, p * P, r0, r1, page, scale, red);
+        if constexpr (SIDES != kValues) {
+            if (turn) {
+                store_page<T, NT, NP8, NEXT, true>(a, rows, token_stride, p * P, r0, r1, page, scale, red);
+                continue;
+            }
+        }
+        if constexpr (SIDES != kKeys) store_page<T, NT, NP8, NEXT, false>(a, rows, token_stride, p * P, r0, r1, page, scale, red);
     }
 }
 
@@ -397,17 +404,25 @@ int launch_kv_append(const KvAppendArgs& a, int dtype, uint32_t max_new, hipStre
             // Few queries go along with the keys and values, in one launch (64 tokens: 5.0 us instead of 5.4 + 3.2; 5 x 700: 15.7 instead of 15.2 + 6.9); many have
             // one of their own, with a third of the registers and so more loads on their way (8 x 8192 tokens: 436 -> 327 us).
             const bool along = a.q && a.batch.tokens * a.q_heads <= 65536;
-            auto store = [&](auto kernel, uint32_t threads) {
-                const uint64_t per = threads / 64, blocks = store_blocks + (along ? (a.batch.tokens + per - 1) / per : 0);
-                hipLaunchKernelGGL(kernel, dim3((uint32_t)blocks), dim3(threads), 0, stream, a, slots, (uint32_t)store_blocks);
+            auto store = [&](auto kernel, uint32_t threads, uint64_t stores, bool turning) {
+                const uint64_t per = threads / 64, blocks = stores + (turning ? (a.batch.tokens + per - 1) / per : 0);
+                hipLaunchKernelGGL(kernel, dim3((uint32_t)blocks), dim3(threads), 0, stream, a, slots, (uint32_t)stores);
             };
             // By the pieces of 8 numbers that a page can get: a wave with one each (a step of decoding), a wave with four, eight waves
             // with four (8 x 8192 tokens, pages of 128 x 128: 142 us; four waves with eight pieces 152, sixteen with two 209; read
-            // twice instead of held 164).
+            // twice instead of held 164).  Where there are many pages, values, which do not turn, have a launch of their own with fewer
+            // registers and so more of them under way (143 us -> 80 + 51; with 64 registers, spilled, 74).
             const uint64_t pieces = (uint64_t)std::min(max_new, a.mem.page_tokens) * a.mem.dim / 8;
-            if (pieces <= 64) store(kv_append<T, 64, 1, NEXT>, 64);
-            else if (pieces <= 256) store(kv_append<T, 64, 4, NEXT>, 64);
-            else store(kv_append<T, 512, 4, NEXT>, 512);
+            if (pieces <= 64) {
+                store(kv_append<T, 64, 1, NEXT, kBoth>, 64, store_blocks, along);
+            } else if (pieces <= 256) {
+                store(kv_append<T, 64, 4, NEXT, kBoth>, 64, store_blocks, along);
+            } else if (a.rot && store_blocks >= 4096) {
+                store(kv_append<T, 512, 4, NEXT, kKeys>, 512, store_blocks / 2, along);
+                store(kv_append<T, 512, 4, NEXT, kValues>, 512, store_blocks / 2, false);
+            } else {
+                store(kv_append<T, 512, 4, NEXT, kBoth>, 512, store_blocks, along);
+            }
             if (a.q && !along)
                 hipLaunchKernelGGL((kv_turn<T, NEXT>), dim3((uint32_t)std::min<uint64_t>((a.batch.tokens + 3) / 4, 8192)), dim3(256), 0, stream, a);
         };

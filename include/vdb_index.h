@@ -333,7 +333,8 @@ int vdb_kv_append_device(const vdb_kv_memory* memory, const vdb_kv_batch* batch,
  * token numbers instead, in any order, each as often as it is listed; numbers outside 0..lengths[b]-1 are skipped, so a
  * search's padding needs no care.  A query that sees nothing gives zeros and -infinity.
  * A token that a query does not see has no effect on its result, whatever it holds.
- * workspace: vdb_kv_attend_workspace() bytes (same sizes; n_select 0 without select; 0 bytes may be needed) of DEVICE memory, 16-byte aligned, free again once the stream has passed the
+ * workspace: vdb_kv_attend_workspace() bytes (same sizes; n_select 0 without select; 0 bytes may be needed, and are
+ * where there are no sequences or no rows) of DEVICE memory, 16-byte aligned, free again once the stream has passed the
  * call; any contents.  Calls that may overlap need workspaces of their own. */
 size_t vdb_kv_attend_workspace(const vdb_kv_memory* memory, const vdb_kv_batch* batch, size_t q_heads, size_t window, size_t n_select);
 int vdb_kv_attend_device(const vdb_kv_memory* memory, const vdb_kv_batch* batch, int dtype, const void* d_q, size_t q_token_stride,

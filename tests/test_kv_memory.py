@@ -928,3 +928,34 @@ def test_append_many_large_pages(dtype, interleaved):
             append_ref(ref.v, ref.vs, v[rows], ref.table[b:b + 1], held[b:b + 1], [0, 1000], page)
             at = ref.table[b][ref.table[b] >= 0].long()
             assert same_codes(mem.k[at.cuda()], ref.k[at]) and same_codes(mem.v[at.cuda()], ref.v[at])
+
+
+@pytest.mark.parametrize("count,tokens,offsets", [(0, 0, None), (0, 0, 16), (0, 5, 16), (3, 0, 16)])
+def test_nothing_to_attend_to_without_a_device(count, tokens, offsets):
+    """No sequences, or no new rows: no workspace and no work, for every way of attention."""
+    l = _lib.lib()
+    for heads, group, width, most in ((1, 1, 1, 0), (8, 4, 1000, 0), (8, 4, 1000, 2048), (2, 20, 100_000, 1)):
+        m = _lib.KvMemoryStruct(16, 16, 16, 16, 10, heads, 64, 128)
+        b = _lib.KvBatchStruct(16, 16, offsets, count, width, tokens, most)
+        for window, select in ((0, 0), (700, 0), (0, 5000)):
+            if select and offsets:
+                continue
+            assert l.vdb_kv_attend_workspace(m, b, heads * group, window, select) == 0
+            assert l.vdb_kv_attend_device(m, b, 0, None, 128, 64, heads * group, 1.0, window, 16 if select else None, select, None, None, None, 0, None) == _lib.VDB_OK
+
+
+@pytest.mark.gpu
+def test_nothing_to_attend_to():
+    """The same from Python: empty results of the right shape, zeros for rows of no sequence."""
+    s = Setup([40, 70], 16, 2, 64, seed=24)
+    mem = s.memory()
+    table, lengths = s.on_gpu()
+    q = s.randn(5, 4, 64).cuda()
+    out, lse = mem.attend(q[:0], table, lengths, offsets=ints([0, 0, 0]), return_lse=True)
+    assert out.shape == (0, 4, 64) and lse.shape == (0, 4)
+    out, lse = mem.attend(q[:0], table[:0], lengths[:0], return_lse=True)
+    assert out.shape == (0, 4, 64) and lse.shape == (0, 4)
+    assert mem.attend(q[:0], table[:0], lengths[:0], select=torch.zeros((0, 2, 7), dtype=torch.int64, device="cuda")).shape == (0, 4, 64)
+    assert not mem.attend(q, table[:0], lengths[:0], offsets=ints([0])).any()
+    mem.append(q[:0, :2], q[:0, :2], table, lengths, offsets=ints([0, 0, 0]))
+    assert same_codes(mem.k, s.k)

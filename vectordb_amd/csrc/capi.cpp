@@ -1932,7 +1932,7 @@ size_t vdb_kv_attend_workspace(const vdb_kv_memory* memory, const vdb_kv_batch* 
     size_t bytes = 0;
     (void)guarded([&] {
         const KvAttendArgs a = kv_attend_args(memory, batch, q_heads, window, n_select);
-        bytes = kv_attend_workspace_bytes(a, kv_max_new(batch));
+        if (a.batch.count && a.batch.tokens) bytes = kv_attend_workspace_bytes(a, kv_max_new(batch));
         return (int)VDB_OK;
     });
     return bytes;

@@ -959,3 +959,62 @@ def test_nothing_to_attend_to():
     assert not mem.attend(q, table[:0], lengths[:0], offsets=ints([0])).any()
     mem.append(q[:0, :2], q[:0, :2], table, lengths, offsets=ints([0, 0, 0]))
     assert same_codes(mem.k, s.k)
+
+
+UNDERSTATED = [
+    # held, new, heads, q heads, dim, window: tokens in ranges, and more new ones than the caller says
+    ([4000], [3], 2, 8, 64, 0),
+    ([8000, 300], [16, 20], 1, 1, 32, 0),
+    ([40_000, 1000], [9, 30], 1, 2, 128, 0),  # more than 16 ranges
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("case", UNDERSTATED, ids=lambda c: "-".join(map(str, c[0] + c[1] + list(c[2:]))))
+def test_attend_understated_max_new(dtype, case):
+    """A wrong max_new costs time only: every row of a tile whose tokens are cut into ranges is joined."""
+    held, new, heads, hq, dim, window = case
+    page = 64
+    s = Setup(held, page, heads, dim, seed=25)
+    off = offsets_of(new)
+    q = s.randn(off[-1], hq, dim, dtype=TYPES[dtype])
+    mem = s.memory()
+    table, lengths = s.on_gpu()
+    ref = attend_ref(q, s.k, s.v, s.ks, s.vs, s.table, held, off, page, dim ** -0.5, window)
+    for said in (1, 2, max(new)):
+        out, lse = mem.attend(q.cuda(), table, lengths, offsets=ints(off), max_new=said, window=window, return_lse=True)
+        check_attend(out, lse, ref, TYPES[dtype])
+
+
+@pytest.mark.gpu
+def test_attend_replayed_with_other_offsets():
+    """A step captured for one or two new tokens a sequence is replayed for other numbers of them, into the same buffers."""
+    page, heads, hq, dim, held = 64, 1, 2, 64, [4000, 2900]
+    s = Setup(held, page, heads, dim, seed=26)
+    mem = s.memory()
+    table, lengths = s.on_gpu()
+    q = s.randn(30, hq, dim, dtype=torch.float16).cuda()
+    offsets = ints([0, 1, 3])
+
+    def step():
+        return mem.attend(q, table, lengths, offsets=offsets, max_new=2, return_lse=True)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out, lse = step()
+    for off in ([0, 1, 3], [0, 16, 30], [2, 2, 19], [0, 30, 30], [0, 1, 3]):
+        offsets.copy_(ints(off))
+        graph.replay()
+        want, want_lse = step()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want) and torch.equal(lse, want_lse)
+        ref = attend_ref(q.cpu(), s.k, s.v, s.ks, s.vs, s.table, held, off, page, dim ** -0.5)
+        rows = slice(off[0], off[2])
+        check_attend(out[rows], lse[rows], [x[rows] if torch.is_tensor(x) else x for x in ref], torch.float16)
+        assert not out[:off[0]].any() and not out[off[2]:].any()

@@ -1279,8 +1279,9 @@ void launch_join_of(const KvAttendArgs& a, const Plan& plan, const dim3& grid, h
 }
 
 template <int T>
-hipError_t launch_join(const KvAttendArgs& a, const Plan& plan, uint32_t rows, hipStream_t stream) {
-    const dim3 grid(std::min(rows, plan.tiles * 16), a.mem.heads, a.batch.count);
+hipError_t launch_join(const KvAttendArgs& a, const Plan& plan, uint32_t rows, hipStream_t stream) {  // rows: of one new token
+    // (every row of a cut tile left partial results: with offsets a sequence may have more new tokens than the caller said)
+    const dim3 grid(a.batch.offsets ? plan.tiles * 16 : rows, a.mem.heads, a.batch.count);
     if (a.select) launch_join_of<T, true>(a, plan, grid, stream);
     else launch_join_of<T, false>(a, plan, grid, stream);
     return hipGetLastError();
@@ -1343,7 +1344,7 @@ hipError_t VDB_CAT(kv_attend_launch_, VDB_PART)(const KvAttendArgs& a, uint32_t 
         case 7: e = launch_one<VDB_PART, 7>(a, plan, stream); break;
         case 8: e = launch_one<VDB_PART, 8>(a, plan, stream); break;
     }
-    if (e == hipSuccess && plan.splits > 1) e = launch_join<VDB_PART>(a, plan, (uint32_t)std::min<uint64_t>((uint64_t)max_new * (a.q_heads / a.mem.heads), 1u << 30), stream);
+    if (e == hipSuccess && plan.splits > 1) e = launch_join<VDB_PART>(a, plan, a.q_heads / a.mem.heads, stream);
     return e;
 }
 

@@ -966,6 +966,9 @@ UNDERSTATED = [
     ([4000], [3], 2, 8, 64, 0),
     ([8000, 300], [16, 20], 1, 1, 32, 0),
     ([40_000, 1000], [9, 30], 1, 2, 128, 0),  # more than 16 ranges
+    ([3009], [16], 1, 1, 64, 2016),           # a window just short of a whole number of ranges, which a tile's rows pass
+    ([1500, 5000], [16, 33], 1, 1, 96, 992),
+    ([40_000], [24], 1, 1, 32, 16_368),
 ]
 
 

@@ -1302,7 +1302,8 @@ Plan plan_of(const KvAttendArgs& a, uint32_t max_new) {
     if (p.many) return p;
     p.tiles = (uint32_t)std::min<uint64_t>(((uint64_t)max_new * G + 15) / 16, 65535);
     uint64_t tokens = a.n_select ? a.n_select : (uint64_t)a.batch.table_width << a.mem.page_shift;
-    if (!a.n_select && a.window) tokens = std::min<uint64_t>(tokens, (uint64_t)a.window + max_new + 31);
+    // (what a tile can see: the 16 rows may be as many tokens, whatever max_new says, and the first is rounded down to 32)
+    if (!a.n_select && a.window) tokens = std::min<uint64_t>(tokens, (uint64_t)a.window + (a.batch.offsets ? 15 : 0) + 31);
     const uint64_t blocks = std::max<uint64_t>(1, (uint64_t)p.tiles * a.mem.heads * a.batch.count);
     // As many ranges as give some 12 blocks a CU, four times what the chip holds at once: sequences of different lengths even out
     // (64 of 1 000 to 8 192 tokens, 8 heads: 147 us at 4 a CU, 130 at 6, 121 at 12, 125 at 16).  But no range shorter than 512

@@ -1021,3 +1021,22 @@ def test_attend_replayed_with_other_offsets():
         rows = slice(off[0], off[2])
         check_attend(out[rows], lse[rows], [x[rows] if torch.is_tensor(x) else x for x in ref], torch.float16)
         assert not out[:off[0]].any() and not out[off[2]:].any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("dim", [32, 128, 224])
+def test_attend_scales_of_pages_left_behind(dtype, dim):
+    """Pages that the window has left behind may hold anything, scales included, also where a tile of tokens begins in one."""
+    held, new, page, heads, hq, window = [600, 533, 330], [400, 350, 328], 16, 8, 16, 40
+    s = Setup(held, page, heads, dim, seed=27)
+    off = offsets_of(new)
+    for b in range(3):
+        for p in range(max(0, held[b] - new[b] - window + 1) // page):
+            i = s.table[b, p].long()
+            s.ks[i], s.vs[i] = float("-inf"), (float("inf"), float("nan"), 2.0 ** 127)[p % 3]
+    q = s.randn(off[-1], hq, dim, dtype=TYPES[dtype])
+    mem = s.memory()
+    table, lengths = s.on_gpu()
+    out, lse = mem.attend(q.cuda(), table, lengths, offsets=ints(off), max_new=max(new), window=window, return_lse=True)
+    check_attend(out, lse, attend_ref(q, s.k, s.v, s.ks, s.vs, s.table, held, off, page, dim ** -0.5, window), TYPES[dtype])

@@ -754,9 +754,9 @@ __global__ __launch_bounds__((Many<T, DS>::kThreads), (Many<T, DS>::occupancy)) 
         const uint8_t* const vh = vc + (uint64_t)head * P * D;
         auto pick = [&](i32x4 pg, int i) { return i < 2 ? (i == 0 ? pg[0] : pg[1]) : (i == 2 ? pg[2] : pg[3]); };
         auto load = [&](int32_t kb, i32x4 pg) {
-            if (tid < 8) {
-                const int32_t page = pick(pg, tid & 3);
-                scale_r = page >= 0 ? (tid < 4 ? a.mem.k_scale : a.mem.v_scale)[(int64_t)page * H + head] : 1.0f;
+            if (tid < 8) {  // (a page of which no row sees a token may have any scale: it is taken for 0)
+                const int32_t page = pick(pg, tid & 3), t = kb + (tid & 3) * 16;
+                scale_r = page >= 0 && t < hi && t + 16 > lo ? (tid < 4 ? a.mem.k_scale : a.mem.v_scale)[(int64_t)page * H + head] : 0.0f;
             }
 #pragma unroll
             for (int i = 0; i < M::units; ++i) {

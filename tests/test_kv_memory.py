@@ -1040,3 +1040,19 @@ def test_attend_scales_of_pages_left_behind(dtype, dim):
     table, lengths = s.on_gpu()
     out, lse = mem.attend(q.cuda(), table, lengths, offsets=ints(off), max_new=max(new), window=window, return_lse=True)
     check_attend(out, lse, attend_ref(q, s.k, s.v, s.ks, s.vs, s.table, held, off, page, dim ** -0.5, window), TYPES[dtype])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("dim", [32, 64, 160, 256])
+@pytest.mark.parametrize("group", [1, 16, 17])
+def test_attend_selected_blocks_of_eight_waves(dtype, dim, group):
+    """Few rows of selected tokens: the waves' parts of one, sixteen and seventeen rows are joined by the threads that have a row."""
+    held, page, heads, n = [90, 0, 300], 16, 2, 333
+    s = Setup(held, page, heads, dim, seed=28)
+    q = s.randn(3, heads * group, dim, dtype=TYPES[dtype])
+    select = torch.randint(-5, 310, (3, heads, n), generator=s.g)
+    mem = s.memory()
+    table, lengths = s.on_gpu()
+    out, lse = mem.attend(q.cuda(), table, lengths, select=select.cuda(), return_lse=True)
+    check_attend(out, lse, attend_ref(q, s.k, s.v, s.ks, s.vs, s.table, held, [0, 1, 2, 3], page, dim ** -0.5, 0, select), TYPES[dtype])

@@ -526,16 +526,16 @@ __global__ __launch_bounds__(WAVES * 64, attend_waves(T, DS, MODE)) void kv_atte
         }
         __syncthreads();
         const int row = threadIdx.x >> 4, part = threadIdx.x & 15;
-        float best = kNone;
+        if (row < 16 && row0 + row < rows) {  // (16 threads a row: the first four waves; the others have no row in LDS)
+            float best = kNone;
 #pragma unroll
-        for (int w = 0; w < WAVES; ++w) best = __builtin_fmaxf(best, st[w * 16 + row]);
-        float f[WAVES], total = 0.0f;
+            for (int w = 0; w < WAVES; ++w) best = __builtin_fmaxf(best, st[w * 16 + row]);
+            float f[WAVES], total = 0.0f;
 #pragma unroll
-        for (int w = 0; w < WAVES; ++w) {
-            f[w] = __builtin_amdgcn_exp2f(st[w * 16 + row] - best);
-            total += f[w] * ss[w * 16 + row];
-        }
-        if (row < 16 && row0 + row < rows) {  // (16 threads a row: the first four waves)
+            for (int w = 0; w < WAVES; ++w) {
+                f[w] = __builtin_amdgcn_exp2f(st[w * 16 + row] - best);
+                total += f[w] * ss[w * 16 + row];
+            }
             float v[ND];
 #pragma unroll
             for (int d = 0; d < ND; ++d) {

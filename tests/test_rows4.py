@@ -240,3 +240,24 @@ def test_products_every_variant(dtype, n, dim, nq):
     assert ((y.cpu().double() - ref).abs() <= tol).all()
     again = rows.products(x.cuda())
     assert torch.equal(y, again)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("n,dim", [(40, 70), (40, 31), (5, 1), (40, 97), (140_000, 100), (9000, 700), (300, 2049)])
+@pytest.mark.parametrize("byte", [0, 1, 252, 253, 254])
+def test_products_scales_at_the_ends(dtype, n, dim, byte):
+    """The smallest and largest scales, with codes past the last column that are infinite under them: those are never used."""
+    r = np.random.default_rng(byte + dim)
+    g = -(-dim // 32)
+    codes = r.integers(0, 256, (n, g * 16), dtype=np.uint8)
+    scales = r.integers(118, 134, (n, g), dtype=np.uint8)
+    scales[::3, -1] = byte
+    if byte >= 253:  # in the columns that are used, 0 and 0.5 only: finite
+        for c in range(dim - (g - 1) * 32):
+            codes[:, (g - 1) * 16 + c // 2] &= 0x9F if c % 2 else 0xF9
+    rows = make(codes, scales, dim)
+    x = torch.from_numpy((r.standard_normal((3, dim)) * 2.0 ** -6).astype(np.float32)).to(TYPES[dtype])
+    y = rows.products(x.cuda()).cpu().numpy().astype(np.float64)
+    v, xd = values(codes, scales, dim), x.double().numpy()
+    assert (np.abs(y - xd @ v.T) <= products_bound(xd, v)).all()

@@ -93,7 +93,15 @@ __global__ __launch_bounds__(256, products_blocks(RT * KB, NCT)) void rows4_prod
                     const uint64_t at = (uint64_t)row * a.groups + min(g, a.groups - 1);
                     cw[r * KB + k] = *(const u32x4*)(a.codes + at * 16);
                     ce[r * KB + k] = a.scales[at];
-                    if ((blk + KB) * 4 > a.groups && g >= a.groups) cw[r * KB + k] = u32x4{0, 0, 0, 0}, ce[r * KB + k] = 127;
+                    if ((blk + KB) * 128 > a.dim) {  // codes past the last column are taken for 0 (scaled, they may be infinite in bf16)
+                        const int left = (int)a.dim - (int)g * 32;
+                        if (left <= 0) ce[r * KB + k] = 127;
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            const int n = left - 8 * j;
+                            cw[r * KB + k][j] &= n >= 8 ? 0xFFFFFFFFu : n > 0 ? (1u << 4 * n) - 1 : 0u;
+                        }
+                    }
                 }
             }
         };

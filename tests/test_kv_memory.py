@@ -1056,3 +1056,20 @@ def test_attend_selected_blocks_of_eight_waves(dtype, dim, group):
     table, lengths = s.on_gpu()
     out, lse = mem.attend(q.cuda(), table, lengths, select=select.cuda(), return_lse=True)
     check_attend(out, lse, attend_ref(q, s.k, s.v, s.ks, s.vs, s.table, held, [0, 1, 2, 3], page, dim ** -0.5, 0, select), TYPES[dtype])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("tokens,hq,interleaved", [(5, 4, False), (1, 1, True), (700, 96, False), (700, 96, True)])
+def test_append_queries_of_no_sequence(dtype, tokens, hq, interleaved):
+    """No sequences, but rows: the queries are copied, few of them and many, whatever their strides."""
+    s = Setup([20], 16, 2, 64, seed=29)
+    mem = s.memory()
+    cos, sin = (x.cuda() for x in angles(30, 16))
+    k = s.randn(tokens, 2, 64, dtype=TYPES[dtype]).cuda()
+    fused = s.randn(tokens, hq + 3, 64, dtype=TYPES[dtype]).cuda()
+    q = fused[:, 2:2 + hq]
+    got = mem.append(k, k, ints([]).view(0, 2), ints([]), offsets=ints([0]), queries=q, cos=cos, sin=sin, interleaved=interleaved)
+    assert torch.equal(got, q)
+    assert same_codes(mem.k, s.k) and torch.equal(mem.k_scale.cpu(), s.ks)
+    assert mem.append(k, k, ints([]).view(0, 2), ints([]), offsets=ints([0])) is None

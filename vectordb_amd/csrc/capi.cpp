@@ -1894,10 +1894,12 @@ int vdb_kv_append_device(const vdb_kv_memory* memory, const vdb_kv_batch* batch,
         if (rot_dims % 16 || rot_dims > a.mem.dim) throw std::invalid_argument("kv append: rot_dims must be a multiple of 16, at most dim");
         if (d_q && !rot_dims) throw std::invalid_argument("kv append: queries are taken to be turned, and rot_dims is 0");
         if (d_q && (q_heads < 1 || q_heads > (1u << 20))) throw std::invalid_argument("kv append: q_heads must be in 1..2^20");
-        if (a.batch.count == 0 || a.batch.tokens == 0) return (int)VDB_OK;
-        check_kv_pointers(a.mem, a.batch);
-        check_kv_rows(d_k, k_token_stride, k_head_stride, "keys");
-        check_kv_rows(d_v, v_token_stride, v_head_stride, "values");
+        if (a.batch.tokens == 0 || (a.batch.count == 0 && !d_q)) return (int)VDB_OK;
+        if (a.batch.count) {  // (without sequences there are queries to copy)
+            check_kv_pointers(a.mem, a.batch);
+            check_kv_rows(d_k, k_token_stride, k_head_stride, "keys");
+            check_kv_rows(d_v, v_token_stride, v_head_stride, "values");
+        }
         if (rot_dims) {
             check_aligned(d_cos, 16, "cos");
             check_aligned(d_sin, 16, "sin");

@@ -303,7 +303,7 @@ __device__ __forceinline__ void turn_queries(const KvAppendArgs& a, uint64_t wav
     if (first >= side_by_side) return;
     for (uint64_t t = wave; t < a.batch.tokens; t += waves) {
         uint32_t b = (uint32_t)t;
-        if (a.batch.offsets) {  // the last sequence that begins at or before t
+        if (a.batch.offsets && a.batch.count) {  // the last sequence that begins at or before t
             uint32_t lo = 0, hi = a.batch.count;
             while (hi - lo > 1) {
                 const uint32_t mid = (lo + hi) / 2;
@@ -312,7 +312,7 @@ __device__ __forceinline__ void turn_queries(const KvAppendArgs& a, uint64_t wav
             }
             b = lo;
         }
-        const Span s = span_of(a.batch, b);
+        const Span s = a.batch.count ? span_of(a.batch, b) : Span{0, 0, 0};
         const int64_t at = s.start + (int64_t)t - s.first;
         const bool any = (int64_t)t >= s.first && at < s.end;  // a row of no sequence is copied
         const bool known = any && at >= 0 && at < (int64_t)a.positions;
@@ -403,7 +403,7 @@ int launch_kv_append(const KvAppendArgs& a, int dtype, uint32_t max_new, hipStre
             constexpr bool NEXT = decltype(next)::value;
             // Few queries go along with the keys and values, in one launch (64 tokens: 5.0 us instead of 5.4 + 3.2; 5 x 700: 15.7 instead of 15.2 + 6.9); many have
             // one of their own, with a third of the registers and so more loads on their way (8 x 8192 tokens: 436 -> 327 us).
-            const bool along = a.q && a.batch.tokens * a.q_heads <= 65536;
+            const bool along = a.q && a.batch.tokens * a.q_heads <= 65536 && store_blocks;
             auto store = [&](auto kernel, uint32_t threads, uint64_t stores, bool turning) {
                 const uint64_t per = threads / 64, blocks = stores + (turning ? (a.batch.tokens + per - 1) / per : 0);
                 hipLaunchKernelGGL(kernel, dim3((uint32_t)blocks), dim3(threads), 0, stream, a, slots, (uint32_t)stores);
@@ -413,7 +413,8 @@ int launch_kv_append(const KvAppendArgs& a, int dtype, uint32_t max_new, hipStre
             // twice instead of held 164).  Where there are many pages, values, which do not turn, have a launch of their own with fewer
             // registers and so more of them under way (143 us -> 80 + 51; with 64 registers, spilled, 74).
             const uint64_t pieces = (uint64_t)std::min(max_new, a.mem.page_tokens) * a.mem.dim / 8;
-            if (pieces <= 64) {
+            if (!store_blocks) {  // no sequences: queries only
+            } else if (pieces <= 64) {
                 store(kv_append<T, 64, 1, NEXT, kBoth>, 64, store_blocks, along);
             } else if (pieces <= 256) {
                 store(kv_append<T, 64, 4, NEXT, kBoth>, 64, store_blocks, along);

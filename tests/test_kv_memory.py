@@ -1073,3 +1073,22 @@ def test_append_queries_of_no_sequence(dtype, tokens, hq, interleaved):
     assert torch.equal(got, q)
     assert same_codes(mem.k, s.k) and torch.equal(mem.k_scale.cpu(), s.ks)
     assert mem.append(k, k, ints([]).view(0, 2), ints([]), offsets=ints([0])) is None
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("new", [[1, 1], [20, 3]])
+def test_append_angles_of_no_position(new, interleaved):
+    """Tables of angles without rows: no key is stored, every value is, and every query is not a number."""
+    held, page, heads, dim = [40, 25], 16, 2, 64
+    s = Setup(held, page, heads, dim, seed=30)
+    mem = s.memory()
+    table, lengths = s.on_gpu()
+    off = offsets_of(new)
+    k, v, q = (s.randn(off[-1], h, dim, dtype=torch.bfloat16) for h in (heads, heads, 4))
+    none = torch.zeros((0, 16), device="cuda")
+    got = mem.append(k.cuda(), v.cuda(), table, lengths, offsets=None if max(new) == 1 else ints(off), queries=q.cuda(), cos=none, sin=none, interleaved=interleaved)
+    append_ref(s.v, s.vs, v, s.table, held, off, page)
+    assert same_codes(mem.k, s.k) and torch.equal(mem.k_scale.cpu(), s.ks)
+    assert same_codes(mem.v, s.v) and torch.equal(mem.v_scale.cpu(), s.vs)
+    assert torch.isnan(got).all()

@@ -1900,7 +1900,7 @@ int vdb_kv_append_device(const vdb_kv_memory* memory, const vdb_kv_batch* batch,
             check_kv_rows(d_k, k_token_stride, k_head_stride, "keys");
             check_kv_rows(d_v, v_token_stride, v_head_stride, "values");
         }
-        if (rot_dims) {
+        if (rot_dims && positions) {
             check_aligned(d_cos, 16, "cos");
             check_aligned(d_sin, 16, "sin");
         }

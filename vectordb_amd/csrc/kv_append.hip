@@ -316,9 +316,8 @@ __device__ __forceinline__ void turn_queries(const KvAppendArgs& a, uint64_t wav
         const int64_t at = s.start + (int64_t)t - s.first;
         const bool any = (int64_t)t >= s.first && at < s.end;  // a row of no sequence is copied
         const bool known = any && at >= 0 && at < (int64_t)a.positions;
-        float c[8], s8[8];  // (of position 0 and unit 0 where nothing turns)
-        const int64_t place = known ? at * (a.rot / 2) : 0;
-        load_turn<NEXT>(a.cos + place, a.sin + place, u < n.turning ? u : 0, c, s8);
+        float c[8] = {}, s8[8] = {};  // (of unit 0 where nothing turns; a position that the tables lack has none, and they may have no rows)
+        if (known) load_turn<NEXT>(a.cos + at * (a.rot / 2), a.sin + at * (a.rot / 2), u < n.turning ? u : 0, c, s8);
         const E<T>* q = (const E<T>*)a.q + t * a.q_token + d;
         E<T>* out = (E<T>*)a.q_out + t * a.q_heads * D + d;
 #pragma unroll 4

@@ -303,7 +303,7 @@ __device__ __forceinline__ void turn_queries(const KvAppendArgs& a, uint64_t wav
     if (first >= side_by_side) return;
     for (uint64_t t = wave; t < a.batch.tokens; t += waves) {
         uint32_t b = (uint32_t)t;
-        if (a.batch.offsets && a.batch.count) {  // the last sequence that begins at or before t
+        if (a.batch.offsets) {  // the last sequence that begins at or before t
             uint32_t lo = 0, hi = a.batch.count;
             while (hi - lo > 1) {
                 const uint32_t mid = (lo + hi) / 2;
@@ -312,7 +312,7 @@ __device__ __forceinline__ void turn_queries(const KvAppendArgs& a, uint64_t wav
             }
             b = lo;
         }
-        const Span s = a.batch.count ? span_of(a.batch, b) : Span{0, 0, 0};
+        const Span s = span_of(a.batch, b);
         const int64_t at = s.start + (int64_t)t - s.first;
         const bool any = (int64_t)t >= s.first && at < s.end;  // a row of no sequence is copied
         const bool known = any && at >= 0 && at < (int64_t)a.positions;
@@ -339,6 +339,18 @@ __device__ __forceinline__ void turn_queries(const KvAppendArgs& a, uint64_t wav
 template <int T, bool NEXT>
 __global__ __launch_bounds__(256) void kv_turn(KvAppendArgs a) {
     turn_queries<T, NEXT>(a, blockIdx.x * 4ull + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), gridDim.x * 4ull);
+}
+
+// Queries of a call without sequences: copied.  (The test for it in turn_queries cost kv_append up to 19 registers, and spills.)
+template <int T>
+__global__ __launch_bounds__(256) void kv_copy(KvAppendArgs a) {
+    const uint32_t D8 = a.mem.dim / 8;
+    for (uint64_t i = blockIdx.x * 256ull + threadIdx.x; i < a.batch.tokens * a.q_heads * D8; i += gridDim.x * 256ull) {
+        const uint64_t row = i / D8, t = row / a.q_heads;
+        float x[8];
+        load8<T>((const E<T>*)a.q + t * a.q_token + (row - t * a.q_heads) * a.q_head + i % D8 * 8, x);
+        store8<T>((E<T>*)a.q_out + i * 8, x);
+    }
 }
 
 enum { kBoth = 0, kKeys = 1, kValues = 2 };  // sides that a launch stores (kKeys: turned)
@@ -402,7 +414,7 @@ int launch_kv_append(const KvAppendArgs& a, int dtype, uint32_t max_new, hipStre
             constexpr bool NEXT = decltype(next)::value;
             // Few queries go along with the keys and values, in one launch (64 tokens: 5.0 us instead of 5.4 + 3.2; 5 x 700: 15.7 instead of 15.2 + 6.9); many have
             // one of their own, with a third of the registers and so more loads on their way (8 x 8192 tokens: 436 -> 327 us).
-            const bool along = a.q && a.batch.tokens * a.q_heads <= 65536 && store_blocks;
+            const bool along = a.q && a.batch.tokens * a.q_heads <= 65536;
             auto store = [&](auto kernel, uint32_t threads, uint64_t stores, bool turning) {
                 const uint64_t per = threads / 64, blocks = stores + (turning ? (a.batch.tokens + per - 1) / per : 0);
                 hipLaunchKernelGGL(kernel, dim3((uint32_t)blocks), dim3(threads), 0, stream, a, slots, (uint32_t)stores);
@@ -412,8 +424,7 @@ int launch_kv_append(const KvAppendArgs& a, int dtype, uint32_t max_new, hipStre
             // twice instead of held 164).  Where there are many pages, values, which do not turn, have a launch of their own with fewer
             // registers and so more of them under way (143 us -> 80 + 51; with 64 registers, spilled, 74).
             const uint64_t pieces = (uint64_t)std::min(max_new, a.mem.page_tokens) * a.mem.dim / 8;
-            if (!store_blocks) {  // no sequences: queries only
-            } else if (pieces <= 64) {
+            if (pieces <= 64) {
                 store(kv_append<T, 64, 1, NEXT, kBoth>, 64, store_blocks, along);
             } else if (pieces <= 256) {
                 store(kv_append<T, 64, 4, NEXT, kBoth>, 64, store_blocks, along);
@@ -426,7 +437,9 @@ int launch_kv_append(const KvAppendArgs& a, int dtype, uint32_t max_new, hipStre
             if (a.q && !along)
                 hipLaunchKernelGGL((kv_turn<T, NEXT>), dim3((uint32_t)std::min<uint64_t>((a.batch.tokens + 3) / 4, 8192)), dim3(256), 0, stream, a);
         };
-        if (a.interleaved) launch(std::true_type());
+        if (!a.batch.count)
+            hipLaunchKernelGGL(kv_copy<T>, dim3((uint32_t)std::min<uint64_t>((a.batch.tokens * a.q_heads * (a.mem.dim / 8) + 255) / 256, 8192)), dim3(256), 0, stream, a);
+        else if (a.interleaved) launch(std::true_type());
         else launch(std::false_type());
     };
     if (dtype == kF32) go(std::integral_constant<int, kF32>());

@@ -320,7 +320,8 @@ typedef struct vdb_kv_batch {
  * or (2 i, 2 i + 1) with interleaved != 0; (x, y) becomes (x cos - y sin, y cos + x sin) in f32.  A position beyond the
  * tables has no angles: its key is not stored (its value is), and its query, like one at a negative position, is NaN.
  * q nullable [tokens][q_heads][dim] of `dtype` (strides as above) -> q_out [tokens][q_heads][dim], turned, rounded once; rows
- * of no sequence are copied.  q_out must not overlap q.  Needs rot_dims != 0. */
+ * of no sequence are copied.  q_out must not overlap q.  Needs rot_dims != 0.
+ * Sequences times heads beyond four million may be refused (a launch's threads). */
 int vdb_kv_append_device(const vdb_kv_memory* memory, const vdb_kv_batch* batch, int dtype, const void* d_k, size_t k_token_stride,
                          size_t k_head_stride, const void* d_v, size_t v_token_stride, size_t v_head_stride, const float* d_cos,
                          const float* d_sin, size_t positions, size_t rot_dims, int interleaved, const void* d_q, size_t q_token_stride,

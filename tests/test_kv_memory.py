@@ -1092,3 +1092,81 @@ def test_append_angles_of_no_position(new, interleaved):
     assert same_codes(mem.k, s.k) and torch.equal(mem.k_scale.cpu(), s.ks)
     assert same_codes(mem.v, s.v) and torch.equal(mem.v_scale.cpu(), s.vs)
     assert torch.isnan(got).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("count,heads,longest,page,dim", [(1000, 64, 300, 64, 64), (300, 8, 2000, 16, 32), (65_535, 2, 1, 16, 32)])
+def test_append_without_max_new(count, heads, longest, page, dim):
+    """Many sequences and no word about the longest: the launch stays within bounds (1000 x 128 x 67 blocks of 512 threads would be
+    2^32 of them), and every token is stored."""
+    from vectordb_amd.memory import KeyValueMemory
+
+    r = np.random.default_rng(count)
+    new = [int(x) for x in r.integers(0, 9, count)]
+    new[count // 2] = longest
+    held = [n + int(x) for n, x in zip(new, r.integers(0, 30, count))]
+    off = offsets_of(new) if count < 10_000 else [0] + list(np.cumsum(new))
+    assert count != 1000 or 128 * 1000 * 512 * ((off[-1] + 2 * page - 2) // page) >= 2 ** 32
+    need = np.array([-(-h // page) for h in held])
+    at = np.cumsum(need) - need
+    width = max(int(need.max()), off[-1] // page + 2 if count < 10_000 else 0)
+    wide = np.arange(width)
+    table = torch.from_numpy(np.where(wide < need[:, None], at[:, None] + wide, -1).astype(np.int32)).cuda()
+    g = torch.Generator(device="cuda").manual_seed(count)
+    k, v = (torch.randn(off[-1], heads, dim, generator=g, device="cuda", dtype=torch.bfloat16) for _ in range(2))
+    pages = int(need.sum())
+    a, b = KeyValueMemory(pages, page, heads, dim), KeyValueMemory(pages, page, heads, dim)
+    a.append(k, v, table, ints(held), offsets=ints(off))
+    b.append(k, v, table, ints(held), offsets=ints(off), max_new=max(new))
+    for x, y in ((a.k, b.k), (a.v, b.v)):
+        assert torch.equal(x.view(torch.uint8), y.view(torch.uint8))
+    assert torch.equal(a.k_scale, b.k_scale) and torch.equal(a.v_scale, b.v_scale)
+    i = count // 2  # and the longest by the formula
+    ids = table[i, :need[i]].long()
+    ks, ref, here = torch.ones(len(ids), heads), torch.zeros(len(ids), heads, page, dim).to(E4M3), torch.arange(len(ids), dtype=torch.int32)[None]
+    append_ref(ref, ks, k[off[i]:off[i + 1]].cpu(), here, [held[i]], [0, new[i]], page)
+    assert same_codes(a.k[ids], ref) and torch.equal(a.k_scale[ids].cpu(), ks)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,page,dim,interleaved", [("f32", 16, 32, False), ("bf16", 64, 96, True), ("f16", 32, 64, False), ("bf16", 128, 64, False)])
+def test_append_one_long_among_short(dtype, page, dim, interleaved):
+    """One prompt among many short ones or none, with and without a word about the longest: pages absent, positions below 0 and
+    without angles, rows of no sequence, a last sequence that claims rows which are not there."""
+    heads, hq, count, t = 2, 3, 70, TYPES[dtype]
+    r = np.random.default_rng(page)
+    new = [int(x) for x in r.integers(0, 3, count)]
+    new[0], new[31], new[68] = 0, 17 * page + 5, page
+    held = [n + int(x) for n, x in zip(new, r.integers(0, 20, count))]
+    held[5], new[5], held[68], new[69] = 2, 6, page - 3, 2
+    s = Setup(held, page, heads, dim, seed=31, width=-(-max(held) // page))
+    s.table[31, 3], s.table[31, 7] = -1, s.ks.shape[0]
+    off = [n + 3 for n in offsets_of(new)]
+    total = off[-1] + 4
+    off[-1] += 9  # beyond the rows that there are
+    k, v, q = s.randn(total, heads, dim, dtype=t), s.randn(total, heads, dim, dtype=t), s.randn(total, hq, dim, dtype=t)
+    cos, sin = angles(max(held) - 11, 16)
+    first = Setup(held, page, heads, dim, seed=31, width=-(-max(held) // page))
+    append_ref(s.k, s.ks, k, s.table, held, off, page, cos, sin, interleaved)
+    append_ref(s.v, s.vs, v, s.table, held, off, page)
+    want = q.clone()
+    for b in range(count - 1):
+        for i in range(new[b]):
+            pos = held[b] - new[b] + i
+            want[off[b] + i] = turn(q[off[b] + i].float(), cos[pos], sin[pos], interleaved).to(t) if 0 <= pos < cos.shape[0] else torch.full_like(q[0], float("nan"))
+    for said in (None, max(new), 1):
+        mem = first.memory()
+        table, lengths = s.on_gpu()
+        got = mem.append(k.cuda(), v.cuda(), table, lengths, offsets=ints(off), max_new=said, queries=q.cuda(), cos=cos.cuda(), sin=sin.cuda(), interleaved=interleaved)
+        assert same_codes(mem.k, s.k) and same_codes(mem.v, s.v)
+        assert torch.equal(mem.k_scale.cpu(), s.ks) and torch.equal(mem.v_scale.cpu(), s.vs)
+        assert same_codes(got, want.float())
+
+
+def test_append_too_many_blocks_without_a_device():
+    """So many sequences and heads that one launch cannot have the threads: refused, not cut off."""
+    l = _lib.lib()
+    m = _lib.KvMemoryStruct(16, 16, 16, 16, 10, 100, 64, 256)
+    b = _lib.KvBatchStruct(16, 16, 16, 65_535, 4, 1 << 20, 64)
+    assert l.vdb_kv_append_device(m, b, 0, 16, 25_600, 256, 16, 25_600, 256, None, None, 0, 0, 0, None, 0, 0, 0, None, None) == _lib.VDB_ERR_INVALID
+    assert "too many" in l.vdb_last_error().decode()

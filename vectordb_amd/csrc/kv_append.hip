@@ -355,9 +355,14 @@ __global__ __launch_bounds__(256) void kv_copy(KvAppendArgs a) {
 
 enum { kBoth = 0, kKeys = 1, kValues = 2 };  // sides that a launch stores (kKeys: turned)
 
-// One launch for all: blocks below store_blocks are (slot, side and head, sequence), a slot being one of the pages that a
-// sequence's new tokens touch; the others turn queries.
-template <int T, int NT, int NP8, bool NEXT, int SIDES>
+// Slots of pages, where a launch has as many for all sequences as their rows can need: those of sequence b begin here.  (n tokens
+// touch n / P + 2 pages at most, which is no more than what lies between two of these.)
+__device__ __forceinline__ uint32_t slot_base(const KvBatch& t, uint32_t b, uint32_t page_shift) { return ((uint32_t)max(t.offsets[b], 0) >> page_shift) + 2 * b; }
+
+// One launch for all: a sequence has blocks of (slot, side and head), a slot being one of the pages that its new tokens touch, or
+// several; the blocks from store_blocks on turn queries, of whatever sequence.  With SHARED the slots are those of all sequences
+// together, and a block looks up whose its own is.
+template <int T, int NT, int NP8, bool NEXT, int SIDES, bool SHARED>
 __global__ __launch_bounds__(NT, SIDES == kValues ? 6 : 4) void kv_append(KvAppendArgs a, uint32_t slots, uint32_t store_blocks) {
     __shared__ uint32_t red[NT / 64];
     if (blockIdx.x >= store_blocks) {
@@ -365,9 +370,21 @@ __global__ __launch_bounds__(NT, SIDES == kValues ? 6 : 4) void kv_append(KvAppe
         turn_queries<T, NEXT>(a, (blockIdx.x - store_blocks) * per + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), (gridDim.x - store_blocks) * per);
         return;
     }
-    const uint32_t sides = (SIDES == kBoth ? 2 : 1) * a.mem.heads, slot = blockIdx.x % slots, rest = blockIdx.x / slots;
-    const uint32_t b = rest / sides, head = (rest % sides) >> (SIDES == kBoth);
+    const uint32_t sides = (SIDES == kBoth ? 2 : 1) * a.mem.heads, rest = blockIdx.x / slots;
+    uint32_t slot = blockIdx.x % slots, step = slots, b = rest / sides;
+    const uint32_t head = (rest % sides) >> (SIDES == kBoth);
     const bool is_v = SIDES == kBoth ? rest % sides & 1 : SIDES == kValues;
+    if constexpr (SHARED) {
+        uint32_t lo = 0, hi = a.batch.count;
+        while (hi - lo > 1) {
+            const uint32_t mid = (lo + hi) / 2;
+            if (slot_base(a.batch, mid, a.mem.page_shift) <= slot) lo = mid;
+            else hi = mid;
+        }
+        const uint32_t base = slot_base(a.batch, lo, a.mem.page_shift);
+        if (slot < base) return;
+        b = lo, slot -= base, step = slot_base(a.batch, lo + 1, a.mem.page_shift) - base;
+    }
     const Span s = span_of(a.batch, b);
     if (s.end <= s.start) return;
     const uint32_t P = a.mem.page_tokens, D = a.mem.dim;
@@ -375,7 +392,7 @@ __global__ __launch_bounds__(NT, SIDES == kValues ? 6 : 4) void kv_append(KvAppe
     const E<T>* src = (const E<T>*)(is_v ? a.v : a.k) + (uint64_t)head * (is_v ? a.v_head : a.k_head);
     const uint64_t token_stride = is_v ? a.v_token : a.k_token;
     const bool turn = !is_v && a.rot != 0;
-    for (int64_t p = (begin >> a.mem.page_shift) + slot; p * P < s.end && p < (int64_t)a.batch.table_width; p += slots) {
+    for (int64_t p = (begin >> a.mem.page_shift) + slot; p * P < s.end && p < (int64_t)a.batch.table_width; p += step) {
         const int32_t pid = a.batch.table[(uint64_t)b * a.batch.table_width + p];
         if (pid < 0 || (uint64_t)pid >= a.mem.pages) continue;
         const uint32_t r0 = p * P < begin ? (uint32_t)(begin - p * P) : 0;
@@ -401,17 +418,28 @@ __global__ __launch_bounds__(NT, SIDES == kValues ? 6 : 4) void kv_append(KvAppe
 }  // namespace
 
 int launch_kv_append(const KvAppendArgs& a, int dtype, uint32_t max_new, hipStream_t stream, std::string* err) {
-    // a sequence's max_new tokens touch at most this many pages; more of them (a wrong max_new) are walked by the same blocks
-    const uint32_t slots = (uint32_t)std::min<uint64_t>(a.batch.table_width, ((uint64_t)max_new + 2 * a.mem.page_tokens - 2) / a.mem.page_tokens);
-    const uint64_t store_blocks = (uint64_t)slots * 2 * a.mem.heads * a.batch.count;
-    if (store_blocks >= (1ull << 30)) {
-        if (err) *err = "kv_append: too many pages in one call";
+    // A sequence's max_new tokens touch at most this many pages; more of them (a wrong max_new) are walked by the same blocks.
+    const uint64_t P = a.mem.page_tokens, sides = 2ull * a.mem.heads, count = a.batch.count, total = a.batch.tokens / P + 2 * count;
+    const uint64_t each = std::min<uint64_t>(a.batch.table_width, ((uint64_t)max_new + 2 * P - 2) / P), most = (1u << 22) / sides;  // (fewer than 2^32 threads)
+    // Where that is more than twice what all rows together can need, blocks look for their sequences (a block without work costs
+    // 5 ns: a prompt of 9000 tokens beside 299 of 3, 8 heads of 128, pages of 64: 2.4 -> 0.10 ms;
+    // a thousand of 4, without max_new, 5.1 -> 0.25).
+    const bool shared = a.batch.offsets && each * count > 2 * total && total <= most;
+    const uint32_t slots = (uint32_t)(shared ? total : std::max<uint64_t>(1, std::min(each, most / std::max<uint64_t>(count, 1))));
+    const uint64_t store_blocks = slots * sides * (shared ? 1 : count);
+    // By the pieces of 8 numbers that a page can get: a wave with one each (a step of decoding), a wave with four, eight waves
+    // with four (8 x 8192 tokens, pages of 128 x 128: 142 us; four waves with eight pieces 152, sixteen with two 209; read
+    // twice instead of held 164).  Where there are many pages, values, which do not turn, have a launch of their own with fewer
+    // registers and so more of them under way (143 us -> 80 + 51; with 64 registers, spilled, 74).
+    const uint64_t pieces = (uint64_t)std::min(max_new, a.mem.page_tokens) * a.mem.dim / 8;
+    if (store_blocks > 0xFFFFFFFFu / (pieces <= 256 ? 64 : 512) - 65536) {
+        if (err) *err = "kv_append: too many sequences times heads in one call";
         return 1;
     }
     auto go = [&](auto t) {
         constexpr int T = decltype(t)::value;
-        auto launch = [&](auto next) {
-            constexpr bool NEXT = decltype(next)::value;
+        auto launch = [&](auto next, auto is_shared) {
+            constexpr bool NEXT = decltype(next)::value, SHARED = decltype(is_shared)::value;
             // Few queries go along with the keys and values, in one launch (64 tokens: 5.0 us instead of 5.4 + 3.2; 5 x 700: 15.7 instead of 15.2 + 6.9); many have
             // one of their own, with a third of the registers and so more loads on their way (8 x 8192 tokens: 436 -> 327 us).
             const bool along = a.q && a.batch.tokens * a.q_heads <= 65536;
@@ -419,28 +447,28 @@ int launch_kv_append(const KvAppendArgs& a, int dtype, uint32_t max_new, hipStre
                 const uint64_t per = threads / 64, blocks = stores + (turning ? (a.batch.tokens + per - 1) / per : 0);
                 hipLaunchKernelGGL(kernel, dim3((uint32_t)blocks), dim3(threads), 0, stream, a, slots, (uint32_t)stores);
             };
-            // By the pieces of 8 numbers that a page can get: a wave with one each (a step of decoding), a wave with four, eight waves
-            // with four (8 x 8192 tokens, pages of 128 x 128: 142 us; four waves with eight pieces 152, sixteen with two 209; read
-            // twice instead of held 164).  Where there are many pages, values, which do not turn, have a launch of their own with fewer
-            // registers and so more of them under way (143 us -> 80 + 51; with 64 registers, spilled, 74).
-            const uint64_t pieces = (uint64_t)std::min(max_new, a.mem.page_tokens) * a.mem.dim / 8;
             if (pieces <= 64) {
-                store(kv_append<T, 64, 1, NEXT, kBoth>, 64, store_blocks, along);
+                store(kv_append<T, 64, 1, NEXT, kBoth, SHARED>, 64, store_blocks, along);
             } else if (pieces <= 256) {
-                store(kv_append<T, 64, 4, NEXT, kBoth>, 64, store_blocks, along);
+                store(kv_append<T, 64, 4, NEXT, kBoth, SHARED>, 64, store_blocks, along);
             } else if (a.rot && store_blocks >= 4096) {
-                store(kv_append<T, 512, 4, NEXT, kKeys>, 512, store_blocks / 2, along);
-                store(kv_append<T, 512, 4, NEXT, kValues>, 512, store_blocks / 2, false);
+                store(kv_append<T, 512, 4, NEXT, kKeys, SHARED>, 512, store_blocks / 2, along);
+                store(kv_append<T, 512, 4, NEXT, kValues, SHARED>, 512, store_blocks / 2, false);
             } else {
-                store(kv_append<T, 512, 4, NEXT, kBoth>, 512, store_blocks, along);
+                store(kv_append<T, 512, 4, NEXT, kBoth, SHARED>, 512, store_blocks, along);
             }
             if (a.q && !along)
                 hipLaunchKernelGGL((kv_turn<T, NEXT>), dim3((uint32_t)std::min<uint64_t>((a.batch.tokens + 3) / 4, 8192)), dim3(256), 0, stream, a);
         };
-        if (!a.batch.count)
+        if (!count) {
             hipLaunchKernelGGL(kv_copy<T>, dim3((uint32_t)std::min<uint64_t>((a.batch.tokens * a.q_heads * (a.mem.dim / 8) + 255) / 256, 8192)), dim3(256), 0, stream, a);
-        else if (a.interleaved) launch(std::true_type());
-        else launch(std::false_type());
+        } else if (a.interleaved) {
+            if (shared) launch(std::true_type(), std::true_type());
+            else launch(std::true_type(), std::false_type());
+        } else {
+            if (shared) launch(std::false_type(), std::true_type());
+            else launch(std::false_type(), std::false_type());
+        }
     };
     if (dtype == kF32) go(std::integral_constant<int, kF32>());
     else if (dtype == kF16) go(std::integral_constant<int, kF16>());

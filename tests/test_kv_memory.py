@@ -1170,3 +1170,29 @@ def test_append_too_many_blocks_without_a_device():
     b = _lib.KvBatchStruct(16, 16, 16, 65_535, 4, 1 << 20, 64)
     assert l.vdb_kv_append_device(m, b, 0, 16, 25_600, 256, 16, 25_600, 256, None, None, 0, 0, 0, None, 0, 0, 0, None, None) == _lib.VDB_ERR_INVALID
     assert "too many" in l.vdb_last_error().decode()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,dim", [("f32", 32), ("bf16", 128), ("f16", 64)])
+def test_attend_one_long_among_short(dtype, dim):
+    """One prompt among many short ones or none, with and without a word about the longest; rows of no sequence before, and a last
+    sequence that claims rows which are not there."""
+    page, heads, hq, count, t = 16, 2, 8, 90, TYPES[dtype]
+    r = np.random.default_rng(dim)
+    new = [int(x) for x in r.integers(0, 4, count)]
+    new[0], new[40], new[88], new[89] = 0, 600, 70, 2
+    held = [n + int(x) for n, x in zip(new, r.integers(0, 50, count))]
+    held[5], new[5] = 3, 9
+    s = Setup(held, page, heads, dim, seed=32)
+    off = [n + 5 for n in offsets_of(new)]
+    total = off[-1]
+    off[-1] += 2
+    q = s.randn(total, hq, dim, dtype=t)
+    mem = s.memory()
+    table, lengths = s.on_gpu()
+    ref = attend_ref(q, s.k, s.v, s.ks, s.vs, s.table, held, off, page, dim ** -0.5)
+    for said in (None, max(new), 70):
+        out, lse = mem.attend(q.cuda(), table, lengths, offsets=ints(off), max_new=said, return_lse=True)
+        rows = slice(off[0], off[-2])
+        check_attend(out[rows], lse[rows], [x[rows] if torch.is_tensor(x) else x for x in ref], t)
+        assert not out[:off[0]].any() and not out[off[-2]:].any()

@@ -655,6 +655,9 @@ struct Items {
     }
 };
 
+// Places for the items of all sequences together: no fewer than there are.
+__host__ __device__ __forceinline__ int64_t many_items(const KvBatch& t, uint32_t G, uint32_t rows) { return (int64_t)(t.tokens * G / rows + t.count); }
+
 // x, but computed where it is used: what follows from it is not kept in registers through the loops.
 __device__ __forceinline__ int fresh(int x) {
     asm volatile("" : "+v"(x));
@@ -696,17 +699,25 @@ __global__ __launch_bounds__((Many<T, DS>::kThreads), (Many<T, DS>::occupancy)) 
         return i32x4{page_of(kb), page_of(kb + 16), page_of(kb + 32), page_of(kb + 48)};
     };
 
-    const bool sorted = gridDim.z == 1;  // at most 64 sequences
     for (int64_t k = blockIdx.x / H;; k += gridDim.x / H) {
-        uint32_t b = blockIdx.z;
+        uint32_t b = 0;
         int32_t rb = 0;
-        if (sorted) {
+        if (a.batch.count <= 64) {
             if (!Items(a, lane, G, M::rows).find(a.batch.count, lane, k, G, M::rows, s, b, rb)) break;
         } else {
-            if (!sequence_of(a, b, s)) break;
-            const int64_t n = ((int64_t)s.n_new * G + M::rows - 1) / M::rows;
-            if (k >= n) break;
-            rb = (int32_t)(n - 1 - k);
+            // More sequences: in their order.  Sequence b has places for its items, and one at most that stays empty, from here on.
+            if (k >= many_items(a.batch, G, M::rows)) break;
+            auto base = [&](uint32_t i) { return (int64_t)max(a.batch.offsets[i], 0) * G / M::rows + i; };
+            uint32_t end = a.batch.count;
+            while (end - b > 1) {
+                const uint32_t mid = (b + end) / 2;
+                if (base(mid) <= k) b = mid;
+                else end = mid;
+            }
+            if (!sequence_of(a, b, s)) continue;
+            const int64_t n = ((int64_t)s.n_new * G + M::rows - 1) / M::rows, at = k - base(b);
+            if (at < 0 || at >= n) continue;
+            rb = (int32_t)(n - 1 - at);
         }
         const int64_t rows = (int64_t)s.n_new * G;
         table = a.batch.table + (uint64_t)b * a.batch.table_width;
@@ -1248,12 +1259,11 @@ __global__ __launch_bounds__(512) void kv_join_long(KvAttendArgs a, Plan plan) {
 template <int T, int DS>
 hipError_t launch_one(const KvAttendArgs& a, const Plan& plan, hipStream_t stream) {
     if (plan.many) {
-        // (blocks a head: as many as there can be items, or, where not all sequences are looked at, of the longest chunk)
+        // blocks a head: as many as there can be items (fewer than 2^32 threads; the rest is walked)
         const uint64_t G = a.q_heads / a.mem.heads, rows = Many<T, DS>::rows, count = a.batch.count;
-        const bool sorted = count <= 64;
-        const uint64_t blocks = std::min<uint64_t>(sorted ? std::min<uint64_t>(a.batch.tokens, plan.max_new * count) * G / rows + count : (plan.max_new * G + rows - 1) / rows,
-                                                   (1u << 30) / a.mem.heads);
-        hipLaunchKernelGGL((kv_attend_many<T, DS>), dim3((uint32_t)blocks * a.mem.heads, 1, sorted ? 1 : a.batch.count), dim3(Many<T, DS>::kThreads), (Many<T, DS>::lds), stream, a);
+        const uint64_t items = (uint64_t)many_items(a.batch, (uint32_t)G, (uint32_t)rows);
+        const uint64_t blocks = std::min<uint64_t>(count <= 64 ? std::min<uint64_t>(items, plan.max_new * count * G / rows + count) : items, (1u << 22) / a.mem.heads);
+        hipLaunchKernelGGL((kv_attend_many<T, DS>), dim3((uint32_t)blocks * a.mem.heads), dim3(Many<T, DS>::kThreads), (Many<T, DS>::lds), stream, a);
         return hipGetLastError();
     }
     const dim3 grid(plan.tiles * plan.splits, a.mem.heads, a.batch.count);

@@ -1196,3 +1196,24 @@ def test_attend_one_long_among_short(dtype, dim):
         rows = slice(off[0], off[-2])
         check_attend(out[rows], lse[rows], [x[rows] if torch.is_tensor(x) else x for x in ref], t)
         assert not out[:off[0]].any() and not out[off[-2]:].any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dim", [32, 96, 128, 256])
+@pytest.mark.parametrize("kind", ["single", "chunks", "selected", "ranges"])
+def test_attend_bf16_results_are_rounded_once(kind, dim):
+    """Weights take part with 16 bits at least (two bf16 parts, each rounded: 2^-16 of each): a bf16 result is off by its own half
+    step, 2^-8 of it, and by what f32 sums leave, but not by 2^-8 of all that it was added up from."""
+    page, heads, hq, t = 16, 2, 6, torch.bfloat16
+    held, new = dict(single=([3, 20, 300], [1, 1, 1]), chunks=([4, 70], [3, 9]), selected=([300, 40], [1, 1]), ranges=([2500], [1]))[kind]
+    s = Setup(held, page, heads, dim, seed=33)
+    off = offsets_of(new)
+    q = s.randn(off[-1], hq, dim, dtype=t)
+    select = torch.randint(-1, 300, (2, heads, 11), generator=s.g) if kind == "selected" else None
+    mem = s.memory()
+    table, lengths = s.on_gpu()
+    got = mem.attend(q.cuda(), table, lengths, offsets=None if max(new) == 1 else ints(off), max_new=max(new), select=None if select is None else select.cuda())
+    out, _, mass, size, n = attend_ref(q, s.k, s.v, s.ks, s.vs, s.table, held, off, page, dim ** -0.5, 0, select)
+    score, many = (3 * dim + 16) * EPS * size, (n / 32 + 64) * EPS
+    tol = (2 * score[..., None] + 2.0 ** -16 + 2 * many) * mass * 1.01 + 2.0 ** -8 * 1.01 * out.abs() + 1e-38
+    assert ((got.double().cpu() - out).abs() <= tol).all()

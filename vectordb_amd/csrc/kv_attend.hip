@@ -27,10 +27,14 @@ constexpr float kNone = -3.0e38f;  // the running maximum before a row has seen 
 template <int T>
 using E = typename Elem<T>::type;
 
-// bf16 parts of p: bf16 results need one (rounded to nearest: 2^-9 of each p, of either sign), f16 two, f32 three
-template <int T>
+// bf16 parts of p: f32 results need three; two, rounded, are off by 2^-16 of each p at most, so that a bf16 result is off by its own
+// rounding alone (64 sequences of up to 8192 tokens: 122 us with one part, 124 with two).  MANY: kv_attend_many takes one for bf16 results, off
+// by 2^-8 of each p at most, of either sign.  That is a choice for speed: four chunks of up to 2048 rows 294 us, with two parts 370, and
+// a mean error against 64 bits 1.33 times that of rounding the result alone (1.52e-4 against 1.14e-4, of results of 0.069 in the
+// mean square).  (f16 weights, as fast, would lose those below 2^-24 of the largest, which a number of a value may consist of.)
+template <int T, bool MANY = false>
 struct Parts {
-    static constexpr int value = T == kBF16 ? 1 : T == kF16 ? 2 : 3;
+    static constexpr int value = T == kBF16 && MANY ? 1 : T == kF32 ? 3 : 2;
 };
 
 // 8 codes (two words) -> 8 elements of the type that scores are computed in
@@ -160,7 +164,7 @@ enum { kChunks = 0, kSingle = 1, kSelected = 2 };
 // Waves a SIMD that the registers allow (512 / waves each, without spilling).
 constexpr int attend_waves(int t, int ds, int mode) {
     if (t == kF32) return ds <= 2 ? 3 : ds <= 5 ? 2 : 1;
-    if (mode == kSingle) return ds <= 2 || (ds == 3 && t == kBF16) ? 4 : ds <= 4 ? 3 : 2;  // (bf16 at 128 would just fit four: 136 us instead of 120)
+    if (mode == kSingle) return ds <= 2 ? 4 : ds <= 4 ? 3 : 2;
     return ds <= 2 ? 4 : ds <= 4 ? 3 : ds <= 6 || mode == kSelected ? 2 : 1;
 }
 
@@ -433,15 +437,15 @@ __global__ __launch_bounds__(WAVES * 64, attend_waves(T, DS, MODE)) void kv_atte
             }
             u32x4 pf[NP];
 #pragma unroll
-            for (int n = 0; n < NP; ++n) {
+            for (int t = 0; t < 4; ++t) {
+                if constexpr (NP == 2) {  // rounded, and what is left of it (weights are finite or NaN)
+                    const bf16x2 w = {(__bf16)p[2 * t], (__bf16)p[2 * t + 1]};
+                    pf[0][t] = __builtin_bit_cast(uint32_t, w);
+                    const bf16x2 r = {(__bf16)(p[2 * t] - float_of(pf[0][t] << 16)), (__bf16)(p[2 * t + 1] - float_of(pf[0][t] & 0xFFFF0000u))};
+                    pf[1][t] = __builtin_bit_cast(uint32_t, r);
+                } else {
 #pragma unroll
-                for (int t = 0; t < 4; ++t) {
-                    if constexpr (NP == 1) {
-                        bf16x2 w = {(__bf16)p[2 * t], (__bf16)p[2 * t + 1]};
-                        pf[n][t] = __builtin_bit_cast(uint32_t, w);
-                    } else {
-                        pf[n][t] = pack_hi16(bf16_part(p[2 * t], n), bf16_part(p[2 * t + 1], n));
-                    }
+                    for (int n = 0; n < NP; ++n) pf[n][t] = pack_hi16(bf16_part(p[2 * t], n), bf16_part(p[2 * t + 1], n));
                 }
             }
             // a NaN among values that some rows of the tile do not see must not reach those (0 * NaN)
@@ -671,7 +675,7 @@ template <int T, int DS>
 __global__ __launch_bounds__((Many<T, DS>::kThreads), (Many<T, DS>::occupancy)) void kv_attend_many(KvAttendArgs a) {
     typedef Many<T, DS> M;
     constexpr bool HALF = T == kF16;
-    constexpr int NQ = T == kF32 ? 3 : 1, NP = Parts<T>::value, D = M::D, ND = M::ND, NT = M::NT, side = M::side;
+    constexpr int NQ = T == kF32 ? 3 : 1, NP = Parts<T, true>::value, D = M::D, ND = M::ND, NT = M::NT, side = M::side;
     extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int m = lane & 15, q4 = lane >> 4;

@@ -275,8 +275,9 @@ int vdb_rows4_pack_device(const void* d_rows, int dtype, size_t n, size_t dim, s
 /* The values that codes and scales stand for, [n][dim] f32. */
 int vdb_rows4_unpack_device(const uint8_t* d_codes, const uint8_t* d_scales, size_t n, size_t dim, float* d_out, void* stream);
 /* d_out[m][r] = sum over the columns of x[m] * value[r], [nq][n] f32 (so the framework's inner-product distance is
- * 1 - d_out, space_ip.hpp:13-18).  x [nq][dim] of `dtype`, x_stride elements apart.  No bit of x is lost (f32 and f16
- * values are split into bf16 parts); products are exact, sums are f32. */
+ * 1 - d_out, space_ip.hpp:13-18).  x [nq][dim] of `dtype`, x_stride elements apart.  x takes part exactly (f32 and f16
+ * values are split into bf16 parts), but for what lies below 2^-133 in an f32 value, bf16's least number, which is cut off;
+ * products are exact, sums are f32. */
 int vdb_rows4_products_device(const uint8_t* d_codes, const uint8_t* d_scales, size_t n, size_t dim, const void* d_x, int dtype,
                               size_t nq, size_t x_stride, float* d_out, void* stream);
 

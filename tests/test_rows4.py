@@ -261,3 +261,20 @@ def test_products_scales_at_the_ends(dtype, n, dim, byte):
     y = rows.products(x.cuda()).cpu().numpy().astype(np.float64)
     v, xd = values(codes, scales, dim), x.double().numpy()
     assert (np.abs(y - xd @ v.T) <= products_bound(xd, v)).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n,dim,nq", [(40, 64, 5), (600, 960, 2), (140_000, 100, 3)])
+def test_products_of_the_smallest_queries(n, dim, nq):
+    """f32 queries near and below the least normal number: what lies below 2^-133 in a value may be cut off, and nothing else."""
+    codes, scales = random_rows(n, dim, n + dim, lo=127, hi=150)
+    rows = make(codes, scales, dim)
+    r = np.random.default_rng(nq)
+    x = (r.standard_normal((nq, dim)) * np.exp2(r.integers(-149, -100, (nq, dim)))).astype(np.float32)
+    x[0, :8] = [2.0 ** -149, -2.0 ** -133, 2.0 ** -126, 2.0 ** -133 * 1.5, 0.0, 2.0 ** -110 * (1 + 2.0 ** -23), 2.0 ** -127, -2.0 ** -148]
+    y = rows.products(torch.from_numpy(x).cuda()).cpu().numpy().astype(np.float64)
+    v, xd = values(codes, scales, dim), x.astype(np.float64)
+    size = np.abs(xd) @ np.abs(v).T
+    # (products_bound's own 1e-37 is left out: a step of the smallest results is 2^-149, one for each of the roundings)
+    steps = 3 * -(-dim // 128) * 128 + 3
+    assert (np.abs(y - xd @ v.T) <= steps * (2.0 ** -24 * size + 2.0 ** -149) + 2.0 ** -133 * np.abs(v).sum(1)).all()

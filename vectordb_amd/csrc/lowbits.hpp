@@ -48,7 +48,8 @@ __device__ __forceinline__ float to_f32(_Float16 x) { return (float)x; }
 __device__ __forceinline__ float to_f32(__bf16 x) { return float_of((uint32_t)__builtin_bit_cast(uint16_t, x) << 16); }
 
 // Part `s` of x = part 0 + part 1 + part 2, each a bf16 (given as the f32 with its lower 16 bits zero): the leading bits are cut
-// off, not rounded, so no part overflows and every remainder is exact.  An infinity or a NaN stays whole in part 0.
+// off, not rounded, so no part overflows and every remainder is exact.  What lies below 2^-133, bf16's least number, is in no part
+// (of f32 values below 2^-110 that can be bits that count).  An infinity or a NaN stays whole in part 0.
 __device__ __forceinline__ float bf16_part(float x, int s) {
     const uint32_t b = bits_of(x);
     if ((b & 0x7F800000u) == 0x7F800000u) return s == 0 ? ((b & 0x007FFFFFu) ? float_of(0x7FC00000u) : x) : 0.0f;

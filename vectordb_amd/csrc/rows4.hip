@@ -28,8 +28,8 @@ struct ProductArgs {
 };
 
 // y[m][r] = sum_c x[m][c] * value[r][c] on the matrix units: 16 rows are the A operand, 16 queries the B operand.  A query in
-// f32 is three bf16 parts (f16: two) that sum to it exactly, one matrix instruction each into the same accumulator: no bit of a
-// query is lost, and the f32 accumulators see exact products.
+// f32 is three bf16 parts (f16: two) that sum to it exactly, one matrix instruction each into the same accumulator: the f32
+// accumulators see exact products (of all but what lies below 2^-133 in an f32 query).
 //
 // What bounds it is the rows' bytes.  The queries go to LDS once per block, as parts and in operand order; the blocks are
 // persistent, and a wave takes RT tiles of 16 rows by KB blocks of 128 columns at a time (16 bytes of codes and one scale a lane

@@ -12,7 +12,6 @@ typedef __attribute__((ext_vector_type(2))) float f32x2;
 typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8;
 typedef __attribute__((ext_vector_type(8))) _Float16 f16x8;
 typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2;
-typedef __attribute__((ext_vector_type(2))) _Float16 f16x2;
 typedef __attribute__((ext_vector_type(4))) int32_t i32x4;
 typedef __attribute__((ext_vector_type(4))) uint32_t u32x4;
 typedef __attribute__((ext_vector_type(2))) uint32_t u32x2;
@@ -24,19 +23,16 @@ struct Elem;
 template <>
 struct Elem<kF32> {
     typedef float type;
-    static constexpr int size = 4;
     static constexpr int splits = 3;  // bf16 parts that hold a value exactly: 24 significand bits in three times 8
 };
 template <>
 struct Elem<kF16> {
     typedef _Float16 type;
-    static constexpr int size = 2;
     static constexpr int splits = 2;  // 11 bits
 };
 template <>
 struct Elem<kBF16> {
     typedef __bf16 type;
-    static constexpr int size = 2;
     static constexpr int splits = 1;
 };
 

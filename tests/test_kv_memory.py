@@ -1217,3 +1217,29 @@ def test_attend_bf16_results_are_rounded_once(kind, dim):
     score, many = (3 * dim + 16) * EPS * size, (n / 32 + 64) * EPS
     tol = (2 * score[..., None] + 2.0 ** -16 + 2 * many) * mass * 1.01 + 2.0 ** -8 * 1.01 * out.abs() + 1e-38
     assert ((got.double().cpu() - out).abs() <= tol).all()
+
+
+@pytest.mark.gpu
+def test_gradients_are_refused():
+    """A tensor that requires a gradient: refused where torch records operations, taken where it does not."""
+    from vectordb_amd.memory import KeyValueMemory
+    from vectordb_amd.rows4 import Rows4
+
+    s = Setup([5, 20], 16, 2, 64, seed=34)
+    mem = s.memory()
+    table, lengths = s.on_gpu()
+    cos, sin = (x.cuda() for x in angles(30, 16))
+    kv, q, x = s.randn(2, 2, 64).cuda(), s.randn(2, 4, 64).cuda(), s.randn(3, 40).cuda()
+    rows = Rows4.pack(x)
+    grad = lambda t: t.clone().requires_grad_()  # noqa: E731
+    for call in [lambda f: mem.attend(f(q), table, lengths), lambda f: mem.append(f(kv), kv, table, lengths), lambda f: mem.append(kv, f(kv), table, lengths),
+                 lambda f: mem.append(kv, kv, table, lengths, queries=f(q), cos=cos, sin=sin), lambda f: mem.append(kv, kv, table, lengths, queries=f(q)),
+                 lambda f: mem.append(kv, kv, table, lengths, cos=f(cos), sin=sin), lambda f: rows.products(x, out=f(torch.zeros(3, 3, device="cuda"))),
+                 lambda f: rows.products(f(x)), lambda f: rows.products(f(x)[0]), lambda f: Rows4.pack(f(x)).codes,
+                 lambda f: KeyValueMemory.from_tensors(mem.k, mem.v, f(mem.k_scale), mem.v_scale).attend(q, table, lengths)]:
+        with pytest.raises(ValueError, match="gradient"):
+            call(grad)
+        with torch.no_grad():
+            a = call(grad)
+        b = call(lambda t: t)
+        assert (a is None and b is None) or torch.equal(a, b)

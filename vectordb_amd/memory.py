@@ -11,7 +11,7 @@ import torch
 
 from . import _lib
 from ._lib import KvBatchStruct, KvMemoryStruct
-from .rows4 import dtype_code, on_device
+from .rows4 import dtype_code, no_gradient, on_device
 
 
 _needs = {}  # bytes of workspace by the sizes of a call
@@ -37,7 +37,8 @@ class KeyValueMemory:
     [pages, kv_heads].  A stored number is code * scale.  Which page holds what is the caller's: ``table`` [sequences, width]
     int32, token t of sequence b lies in page table[b, t // page_tokens]; a page that several sequences list is not
     appended to.  ``lengths`` [sequences] int32 counts a sequence's
-    tokens, the new ones of the call included, for ``append`` and ``attend`` alike.  Neither call has a gradient."""
+    tokens, the new ones of the call included, for ``append`` and ``attend`` alike.  Neither call has a gradient: tensors that
+    require one are refused where torch records operations."""
 
     def __init__(self, pages: int, page_tokens: int, kv_heads: int, head_dim: int, device="cuda"):
         code = lambda: torch.zeros((pages, kv_heads, page_tokens, head_dim), dtype=torch.uint8, device=device).view(torch.float8_e4m3fn)  # noqa: E731
@@ -60,6 +61,8 @@ class KeyValueMemory:
         index = k.get_device() if k.is_cuda else -1
         if index < 0 or v.get_device() != index or k_scale.get_device() != index or v_scale.get_device() != index:
             raise ValueError("k, v, k_scale, v_scale: CUDA tensors on one device")
+        if k_scale.requires_grad or v_scale.requires_grad:
+            no_gradient()
         if not (k.is_contiguous() and v.is_contiguous() and k_scale.is_contiguous() and v_scale.is_contiguous()):
             raise ValueError("k, v, k_scale, v_scale must be contiguous")
         pages, heads, page_tokens, dim = shape
@@ -104,11 +107,14 @@ class KeyValueMemory:
         Row b is the last token of sequence b, or with ``offsets`` [sequences + 1] int32 rows offsets[b] .. offsets[b + 1] - 1
         are its last ones (at most ``max_new`` of any sequence; by default all rows).  ``cos``, ``sin`` [positions, half]
         float32 turn the first 2 * half numbers of each key by its position's angles, in pairs (d, d + half), or (2 i, 2 i + 1)
-        if ``interleaved``.  Returns ``queries`` [tokens, q_heads, head_dim], turned likewise (rows of no sequence: copied; None without queries)."""
+        if ``interleaved``.  Returns ``queries`` [tokens, q_heads, head_dim], turned likewise (rows of no
+        sequence: copied; None without queries; where nothing turns, ``queries`` itself)."""
         shape = self._check_rows(k, self.kv_heads, "k")
         t, dtype, index = dtype_code(k, "k"), k.dtype, self._index
         if v.shape != shape or v.dtype is not dtype or v.get_device() != index:
             raise ValueError("k and v: one shape, type and device")
+        if k.requires_grad or v.requires_grad or (queries is not None and queries.requires_grad):
+            no_gradient()
         tokens = shape[0]
         batch = self._batch(table, lengths, offsets, tokens if max_new is None else max_new, tokens)
         rot = positions = 0
@@ -118,6 +124,8 @@ class KeyValueMemory:
                 raise ValueError("cos and sin: float32 [positions, half]")
             if cos.get_device() != index or sin.get_device() != index or not (cos.is_contiguous() and sin.is_contiguous()):
                 raise ValueError(f"cos and sin: contiguous, on {self.device}")
+            if cos.requires_grad or sin.requires_grad:
+                no_gradient()
             positions, rot = cos.shape
             rot *= 2
             if rot:
@@ -152,6 +160,8 @@ class KeyValueMemory:
         ``scale`` is 1 / sqrt(head_dim) unless given."""
         tokens, q_heads, dim = self._check_rows(q, None, "q")
         t = dtype_code(q, "q")
+        if q.requires_grad:
+            no_gradient()
         if q_heads == 0 or q_heads % self.kv_heads:
             raise ValueError(f"q: a multiple of {self.kv_heads} heads")
         if window < 0:

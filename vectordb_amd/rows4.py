@@ -21,6 +21,12 @@ def dtype_code(t, what: str) -> int:
     return code
 
 
+def no_gradient() -> None:
+    """For a tensor that requires one: refused where torch records operations, or the gradient would be lost without a word."""
+    if torch.is_grad_enabled():
+        raise ValueError("no gradient passes through this call: detach the tensor, or call under torch.no_grad()")
+
+
 def on_device(index, call, *args) -> None:
     """Calls ``call(*args, stream)`` with device ``index`` current, on torch's current stream of it (as a number:
     torch.cuda.current_stream, which makes an object of it, costs the host 7 us a call)."""
@@ -63,6 +69,8 @@ class Rows4:
         if not rows.is_cuda or rows.dim() != 2:
             raise ValueError("rows: a CUDA tensor [n, dim]")
         t = dtype_code(rows, "rows")
+        if rows.requires_grad:
+            no_gradient()
         if rows.stride(1) != 1 or rows.stride(0) < 0:
             rows = rows.contiguous()
         n, dim = rows.shape
@@ -82,12 +90,15 @@ class Rows4:
         return out
 
     def products(self, queries, out=None):
-        """Inner products of queries [nq, dim] (or [dim]) with every row: [nq, n] (or [n]) float32, into ``out`` if given (no gradient)."""
+        """Inner products of queries [nq, dim] (or [dim]) with every row: [nq, n] (or [n]) float32, into ``out`` if given.
+        Has no gradient: queries that require one are refused where torch records operations."""
         index, n = self._index, self._n
         x = queries if queries.dim() == 2 else queries.unsqueeze(0)
         if queries.dim() not in (1, 2) or x.shape[1] != self.dim or x.get_device() != index:
             raise ValueError(f"expected queries [nq, {self.dim}] on {self.codes.device}, got {tuple(queries.shape)} on {queries.device}")
         t = dtype_code(x, "queries")
+        if x.requires_grad or (out is not None and out.requires_grad):
+            no_gradient()
         step, one = x.stride()
         if one != 1 or step < 0:
             x = x.contiguous()

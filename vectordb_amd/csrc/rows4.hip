@@ -93,8 +93,18 @@ __global__ __launch_bounds__(256, products_blocks(RT * KB, NCT)) void rows4_prod
                     const uint64_t at = (uint64_t)row * a.groups + min(g, a.groups - 1);
                     cw[r * KB + k] = *(const u32x4*)(a.codes + at * 16);
                     ce[r * KB + k] = a.scales[at];
-                    if ((blk + KB) * 128 > a.dim) {  // codes past the last column are taken for 0 (scaled, they may be infinite in bf16)
-                        const int left = (int)a.dim - (int)g * 32;
+                }
+            }
+        };
+        f32x4 acc[RT][NCT];
+        const int from = (m * 4 + q4) * 4;  // the lane that loaded this lane's piece
+        auto multiply = [&](uint32_t blk, u32x4 cw[RT * KB], uint32_t ce[RT * KB]) {
+            if ((blk + KB) * 128 > a.dim) {  // codes past the last column are taken for 0 (scaled, they may be infinite in bf16)
+#pragma unroll
+                for (int k = 0; k < KB; ++k) {
+                    const int left = (int)a.dim - (int)((blk + k) * 4 + (lane & 3)) * 32;
+#pragma unroll
+                    for (int r = 0; r < RT; ++r) {
                         if (left <= 0) ce[r * KB + k] = 127;
 #pragma unroll
                         for (int j = 0; j < 4; ++j) {
@@ -104,10 +114,6 @@ __global__ __launch_bounds__(256, products_blocks(RT * KB, NCT)) void rows4_prod
                     }
                 }
             }
-        };
-        f32x4 acc[RT][NCT];
-        const int from = (m * 4 + q4) * 4;  // the lane that loaded this lane's piece
-        auto multiply = [&](uint32_t blk, u32x4 cw[RT * KB], uint32_t ce[RT * KB]) {
 #pragma unroll
             for (int p = 0; p < RT * KB; ++p) {
 #pragma unroll

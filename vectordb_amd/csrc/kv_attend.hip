@@ -579,8 +579,8 @@ __global__ __launch_bounds__(WAVES * 64, attend_waves(T, DS, MODE)) void kv_atte
 //     scales of a head's pages lie so far apart that w could underflow and w / v_scale count - pages of zeros beside values of
 //     thousands do - the weight is w / v_scale from the start, and costs a product more.)
 //   - the loads of the tile after next are under way while one is computed and the next is being widened.
-// Measured: four chunks of 30 to 2048 tokens, the longest sequence 6 000, 32 heads on 8, 128 dimensions, bf16: 317 us (its matrix
-// products at the rate of a large product: 182); of a block's 45 to 240 us, 2.3 a tile, 4 one at an edge, and some 25 to start
+// Measured: four chunks of 30 to 2048 tokens, the longest sequence 6 000, 32 heads on 8, 128 dimensions, bf16: 284 us, 325 in the first
+// launches, before the clock has risen (its matrix products at the rate of a large product: 182); then, of a block's 45 to 240 us, 2.3 a tile, 4 one at an edge, and some 25 to start
 // and end.  Left out in turn, the loads, the exp2, either product, the barrier or the widening save 5 to 15 % each: nothing of it
 // alone is what takes the time.
 template <int T, int DS>

@@ -1243,3 +1243,22 @@ def test_gradients_are_refused():
             a = call(grad)
         b = call(lambda t: t)
         assert (a is None and b is None) or torch.equal(a, b)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("count,heads,group,dim", [(130, 1, 64, 32), (70, 2, 200, 64), (40, 4, 70, 128)])
+def test_attend_one_token_of_many_heads(dtype, count, heads, group, dim):
+    """One new token a sequence, without offsets, but so many query heads a key head that the kernel for many rows takes them, up to
+    and beyond the 64 sequences whose work it puts in order."""
+    page = 16
+    r = np.random.default_rng(count)
+    held = [int(x) for x in r.integers(0, 150, count)]
+    s = Setup(held, page, heads, dim, seed=35)
+    q = s.randn(count, heads * group, dim, dtype=TYPES[dtype])
+    mem = s.memory()
+    table, lengths = s.on_gpu()
+    for window in (0, 30):
+        out, lse = mem.attend(q.cuda(), table, lengths, window=window, return_lse=True)
+        ref = attend_ref(q, s.k, s.v, s.ks, s.vs, s.table, held, list(range(count + 1)), page, dim ** -0.5, window)
+        check_attend(out, lse, ref, TYPES[dtype])

@@ -711,7 +711,7 @@ __global__ __launch_bounds__((Many<T, DS>::kThreads), (Many<T, DS>::occupancy)) 
         } else {
             // More sequences: in their order.  Sequence b has places for its items, and one at most that stays empty, from here on.
             if (k >= many_items(a.batch, G, M::rows)) break;
-            auto base = [&](uint32_t i) { return (int64_t)max(a.batch.offsets[i], 0) * G / M::rows + i; };
+            auto base = [&](uint32_t i) { return (int64_t)(a.batch.offsets ? max(a.batch.offsets[i], 0) : (int32_t)i) * G / M::rows + i; };
             uint32_t end = a.batch.count;
             while (end - b > 1) {
                 const uint32_t mid = (b + end) / 2;
